@@ -57,7 +57,8 @@ enum {
   NK_INVALID_SCALE = 15,     /* AttentionError::InvalidScale (value = scale) */
   NK_NO_VALID_TARGETS = 16,  /* AttentionError::NoValidAttentionTargets (index = (b*Sq + q)*Hq + h) */
   NK_ZERO_PARTITION = 17,    /* AttentionError::ZeroPartition (index as above) */
-  NK_TOKEN_OUT_OF_RANGE = 18 /* EmbeddingError::TokenOutOfRange (actual = token id, expected = vocab, index = position) */
+  NK_TOKEN_OUT_OF_RANGE = 18, /* EmbeddingError::TokenOutOfRange (actual = token id, expected = vocab, index = position) */
+  NK_PAGE_OUT_OF_RANGE = 19  /* a page id outside the pool (host: actual = id, expected = pages, index = position) */
 };
 
 typedef struct nk_error_info {
@@ -693,6 +694,144 @@ nk_status nk_attention_gqa(const uint16_t *q, const uint16_t *k_cache, const uin
                            int32_t out_dtype, void *workspace, size_t workspace_bytes,
                            void *stream);
 nk_status nk_attention_check(const void *workspace, int64_t *first_bad_row, void *stream);
+
+/* ===================================================== paged KV cache ====
+ * Sequences of their own lengths over one pool of pages (the reference's
+ * KvCache, cache.rs:74-110, holds one sequence per cache).  The token at
+ * position p of the sequence in table row r is slot p % page_size of page
+ * table[r][p / page_size].  Pages may be shared by sequences (forks); which
+ * page is whose is the caller's bookkeeping (nk_paged.PagedKvCache).
+ *
+ * Device arrays are checked on the device: a page id outside the pool, or
+ * batch arrays that contradict one another or the bounds given beside them
+ * (start not ascending or past `tokens`, more new tokens than max_new or than
+ * kv_len, kv_len past max_kv or the table, rows outside the table), leave the
+ * sequence's outputs unwritten or its pages unread, never touch memory out of
+ * range, and are reported by nk_device_status as NK_PAGE_OUT_OF_RANGE or
+ * NK_INVALID_PARAMS.  All calls are asynchronous, allocate nothing and can be
+ * captured into a CUDA graph; arrays named host are read before the call
+ * returns. */
+typedef struct nk_kv_pages {
+  int64_t layers, pages, kv_heads;
+  int64_t page_size; /* 16, 32, 64 or 128 tokens */
+  int64_t head_dim;  /* 64 or 128 */
+  uint16_t *k, *v;   /* bf16 [layers, pages, kv_heads, page_size, head_dim], 16-byte aligned */
+  /* bf16 [layers, pages, kv_heads, head_dim]: smallest and largest key value
+   * of each channel over the page's written slots (what nk_kv_block_select
+   * reads); both NULL: not kept. */
+  uint16_t *k_min, *k_max;
+  const int32_t *table; /* [table_rows, table_ld] page ids */
+  int64_t table_rows, table_ld;
+} nk_kv_pages;
+
+/* The ragged batch of one step.  Sequence b has new tokens start[b] ..
+ * start[b+1]-1 of the token buffers (q, k_new, v_new); they are the last ones
+ * of its kv_len[b] cached tokens. */
+typedef struct nk_kv_batch {
+  int64_t seqs;          /* <= 65535 */
+  int64_t tokens;        /* rows of the token buffers */
+  const int32_t *start;  /* [seqs + 1] */
+  const int32_t *kv_len; /* [seqs], the new tokens included */
+  const int32_t *rows;   /* [seqs] table row of each sequence; NULL: row b */
+  int64_t max_new;       /* bound of start[b+1] - start[b] */
+  int64_t max_kv;        /* bound of kv_len[b] */
+} nk_kv_batch;
+
+/* Stores the batch's new keys and values (bf16, ld_* elements between tokens,
+ * a multiple of 8, 16-byte aligned) in their pages of `layer`, and extends
+ * the bounds of the pages touched.  A page written here must belong to one
+ * sequence of the batch only. */
+nk_status nk_kv_pages_append(const nk_kv_pages *kv, int64_t layer, const nk_kv_batch *batch,
+                             const uint16_t *k_new, int64_t ld_k, const uint16_t *v_new,
+                             int64_t ld_v, void *stream);
+
+/* Copies page src_host[i] to page dst_host[i] in every layer: keys, values
+ * and bounds (the copy before a write into a shared page; the partial page of
+ * a fork).  Refused: ids outside the pool, a destination that appears twice
+ * or is a source too. */
+nk_status nk_kv_pages_copy(const nk_kv_pages *kv, const int32_t *src_host,
+                           const int32_t *dst_host, int64_t count, void *stream);
+
+/* dst[offset_host[i]] = value_host[i] on the device (offset_host NULL: dst[i]):
+ * table rows and batch arrays that the host plans, ordered by the stream.
+ * Refused: offsets outside dst or repeated. */
+nk_status nk_kv_table_write(int32_t *dst, int64_t dst_len, const int64_t *offset_host,
+                            const int32_t *value_host, int64_t count, void *stream);
+
+/* Moves kept tokens together in every layer: of sequence b, the token at
+ * position base[b] + keep[b*keep_ld + i] goes to position base[b] + i, for
+ * i < n_keep[b]; keep is strictly ascending and base + keep < kv_len.  The
+ * bounds of the pages that hold positions base[b] .. base[b]+n_keep[b]-1 (and
+ * of the page that holds base[b] when that is not its first slot) are
+ * recomputed over the positions below base[b] + n_keep[b]; new_len[b] (may be
+ * NULL) is set to that sum.  All arrays are device arrays, so that the
+ * outcome of a verification needs no host.
+ * dst_table NULL: in place (the accepted path of a draft tree closes up).
+ * Otherwise the tokens go to the pages of dst_table [seqs, dst_ld] (a context
+ * thinned into fresh pages); a page written must not be read as a source.
+ * Refused entries (not ascending, past kv_len) leave their slot unwritten. */
+typedef struct nk_kv_compact_args {
+  int64_t seqs;             /* <= 65535 */
+  const int32_t *rows;      /* [seqs] table row of each sequence; NULL: row b */
+  const int32_t *kv_len;    /* [seqs] */
+  const int32_t *base;      /* [seqs] */
+  const int32_t *keep; int64_t keep_ld;
+  const int32_t *n_keep;    /* [seqs], <= max_keep */
+  int64_t max_keep;         /* <= keep_ld */
+  const int32_t *dst_table; int64_t dst_ld;
+  int32_t *new_len;         /* [seqs] or NULL */
+} nk_kv_compact_args;
+nk_status nk_kv_pages_compact(const nk_kv_pages *kv, const nk_kv_compact_args *args,
+                              void *stream);
+
+/* Attention of the batch's new tokens over their sequences' pages.  q bf16
+ * [tokens, q_heads * head_dim] (ld_q elements between tokens, a multiple of
+ * 8), out [tokens, q_heads * head_dim] f32 or bf16 (NK_DTYPE_*).  Token i of
+ * sequence b stands at position P + i, P = kv_len[b] - new tokens, and
+ * attends, with scores scale * q.k (default 1/sqrt(head_dim)):
+ *   - without masks, every position up to its own (decode steps, prefill
+ *     chunks);
+ *   - with tree_mask [tokens], every position below P and the new token j
+ *     whose bit j is set (drafted tokens: a branch's ancestors and itself);
+ *     max_new <= 64;
+ *   - with blocks [tokens, kv_heads, max_blocks], the positions up to its own
+ *     that lie in the listed blocks of page_size tokens.  Entries are
+ *     ascending; one that is negative, past the token's position or not
+ *     larger than the entry before it is skipped.
+ * A token that may attend nothing gets 0.  Positions it may not attend do
+ * not reach its output, whatever they hold (infinities and NaN too).  Rows of
+ * out behind the last sequence stay as they were.
+ * workspace: nk_attention_paged_workspace_bytes for the same batch bounds
+ * (0 bytes: NULL). */
+typedef struct nk_paged_attention_args {
+  const uint16_t *q; int64_t ld_q;
+  int64_t q_heads;
+  const uint64_t *tree_mask;              /* [tokens] or NULL */
+  const int32_t *blocks; int64_t max_blocks; /* [tokens, kv_heads, max_blocks] or NULL */
+  int32_t has_scale; float scale;
+  void *out; int32_t out_dtype;
+} nk_paged_attention_args;
+nk_status nk_attention_paged_workspace_bytes(const nk_kv_pages *kv, const nk_kv_batch *batch,
+                                             const nk_paged_attention_args *args, size_t *bytes);
+nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_batch *batch,
+                             const nk_paged_attention_args *args, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
+/* The blocks (pages) that each new token's query reads, one list per KV head:
+ * blocks [tokens, kv_heads, top_k] int32, ascending, -1 behind the last.  For
+ * a token at position p the blocks 0 .. p / page_size are eligible; the first
+ * `sink` and the last `local` are always taken, the others by the score
+ *   max over the KV head's query heads g of Σ_c q[g][c] * (q[g][c] >= 0 ?
+ *   k_max[c] : k_min[c]),
+ * the largest q.k that the block's bounds allow, summed in 64 bits; equal
+ * scores go to the lower block, NaN ranks last.  sink >= 0, local >= 1,
+ * sink + local <= top_k.  Needs k_min and k_max. */
+nk_status nk_kv_block_select_workspace_bytes(const nk_kv_pages *kv, const nk_kv_batch *batch,
+                                             size_t *bytes);
+nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_batch *batch,
+                             const uint16_t *q, int64_t ld_q, int64_t q_heads, int64_t top_k,
+                             int64_t sink, int64_t local, int32_t *blocks, void *workspace,
+                             size_t workspace_bytes, void *stream);
 
 /* ============================================ decoder steps around projections ====
  * Embedding gather, block residual + RMSNorm, greedy pick. */

@@ -1,0 +1,84 @@
+// paged.cuh — the paged KV cache as the kernels see it: pool geometry, the
+// ragged batch, and the checks every kernel makes of device arrays.
+#pragma once
+
+#include "nk_common.cuh"
+
+namespace nk {
+
+struct PagePool {
+  int layers, pages, heads, ps, ps_log2;
+  const int32_t *table;
+  int64_t table_ld;
+  int table_rows;
+};
+
+struct PageBatch {
+  const int32_t *start, *kv_len, *rows;
+  int64_t tokens;
+  int seqs, max_new, max_kv;
+};
+
+// Host checks of nk_kv_pages / nk_kv_batch shared by the entry points (no
+// device work), and their kernel forms.
+nk_status check_pages(const nk_kv_pages *kv, int64_t layer);
+nk_status check_batch(const nk_kv_pages *kv, const nk_kv_batch *b);
+inline PagePool page_pool(const nk_kv_pages &kv) {
+  PagePool p{};
+  p.layers = (int)kv.layers;
+  p.pages = (int)kv.pages;
+  p.heads = (int)kv.kv_heads;
+  p.ps = (int)kv.page_size;
+  p.ps_log2 = __builtin_ctz((unsigned)kv.page_size);
+  p.table = kv.table;
+  p.table_ld = kv.table_ld;
+  p.table_rows = (int)kv.table_rows;
+  return p;
+}
+inline PageBatch page_batch(const nk_kv_batch &b) {
+  PageBatch p{};
+  p.start = b.start;
+  p.kv_len = b.kv_len;
+  p.rows = b.rows;
+  p.tokens = b.tokens;
+  p.seqs = (int)b.seqs;
+  p.max_new = (int)b.max_new;
+  p.max_kv = (int)b.max_kv;
+  return p;
+}
+
+// First error of a kernel stays in the device word.
+__device__ __forceinline__ void report(int *err, int code) { atomicCAS(err, 0, code); }
+
+struct SeqView {
+  int first, count;      // new tokens: rows first .. first+count-1 of the token buffers
+  int len;               // cached tokens, the new ones included
+  const int32_t *table;  // the sequence's pages
+};
+
+// Sequence s of the batch; false (reported once per calling block by
+// `report_it`) when the arrays contradict one another or their bounds.
+__device__ __forceinline__ bool load_seq(const PagePool &p, const PageBatch &b, int s, SeqView &v,
+                                         int *err, bool report_it) {
+  v.first = b.start[s];
+  const int end = b.start[s + 1];
+  v.count = end - v.first;
+  v.len = b.kv_len[s];
+  const int row = b.rows ? b.rows[s] : s;
+  const bool good = v.first >= 0 && end >= v.first && end <= b.tokens && v.count <= b.max_new &&
+                    v.len >= v.count && v.len <= b.max_kv &&
+                    (int64_t)v.len <= p.table_ld * (int64_t)p.ps && row >= 0 &&
+                    row < p.table_rows;
+  if (!good) {
+    if (report_it) report(err, NK_INVALID_PARAMS);
+    return false;
+  }
+  v.table = p.table + (int64_t)row * p.table_ld;
+  return true;
+}
+
+__device__ __forceinline__ bool page_ok(const PagePool &p, int page) {
+  return (unsigned)page < (unsigned)p.pages;
+}
+
+}  // namespace nk

@@ -22,13 +22,14 @@ OK, INVALID_SHAPE, LENGTH_MISMATCH, INVALID_PARAMS, INT4_OUT_OF_RANGE = 0, 1, 2,
 NON_FINITE_INPUT, INVALID_ROW_COUNT, UNSUPPORTED, DEVICE_ERROR, TIMEOUT = 5, 6, 7, 8, 9
 WORKSPACE_TOO_SMALL, INVALID_DELTA_T, EMPTY_INPUT, NEGATIVE_EPSILON = 10, 11, 12, 13
 HEAD_COUNT_MISMATCH, INVALID_SCALE, NO_VALID_TARGETS, ZERO_PARTITION = 14, 15, 16, 17
-TOKEN_OUT_OF_RANGE = 18
+TOKEN_OUT_OF_RANGE, PAGE_OUT_OF_RANGE = 18, 19
 STATUS_NAMES = {
     0: "Ok", 1: "InvalidShape", 2: "LengthMismatch", 3: "InvalidParams",
     4: "Int4OutOfRange", 5: "NonFiniteInput", 6: "InvalidRowCount", 7: "Unsupported",
     8: "DeviceError", 9: "Timeout", 10: "WorkspaceTooSmall", 11: "InvalidDeltaT",
     12: "EmptyInput", 13: "NegativeEpsilon", 14: "HeadCountMismatch", 15: "InvalidScale",
     16: "NoValidAttentionTargets", 17: "ZeroPartition", 18: "TokenOutOfRange",
+    19: "PageOutOfRange",
 }
 F32, BF16 = 0, 1
 EPI_RELU2 = 1
@@ -93,6 +94,37 @@ class NkScanArgs(_c.Structure):
         ("y", _p), ("ld_y", _i64),
         ("final_state", _p),
         ("check_delta_t", _i32),
+    ]
+
+
+class NkKvPages(_c.Structure):
+    _fields_ = [
+        ("layers", _i64), ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64),
+        ("head_dim", _i64), ("k", _p), ("v", _p), ("k_min", _p), ("k_max", _p),
+        ("table", _p), ("table_rows", _i64), ("table_ld", _i64),
+    ]
+
+
+class NkKvBatch(_c.Structure):
+    _fields_ = [
+        ("seqs", _i64), ("tokens", _i64), ("start", _p), ("kv_len", _p), ("rows", _p),
+        ("max_new", _i64), ("max_kv", _i64),
+    ]
+
+
+class NkKvCompactArgs(_c.Structure):
+    _fields_ = [
+        ("seqs", _i64), ("rows", _p), ("kv_len", _p), ("base", _p), ("keep", _p),
+        ("keep_ld", _i64), ("n_keep", _p), ("max_keep", _i64), ("dst_table", _p),
+        ("dst_ld", _i64), ("new_len", _p),
+    ]
+
+
+class NkPagedAttentionArgs(_c.Structure):
+    _fields_ = [
+        ("q", _p), ("ld_q", _i64), ("q_heads", _i64), ("tree_mask", _p), ("blocks", _p),
+        ("max_blocks", _i64), ("has_scale", _i32), ("scale", _f), ("out", _p),
+        ("out_dtype", _i32),
     ]
 
 
@@ -194,6 +226,15 @@ _SIGS = {
     "nk_embedding_lookup": (_i32, [_p, _i32, _sz, _p, _i64, _i64, _i64, _p, _i32, _sz, _i32, _p]),
     "nk_add_rms_norm_rows": (_i32, [_p, _p, _i64, _i64, _p, _sz, _f, _p, _p, _i32, _p]),
     "nk_argmax_rows": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _p]),
+    "nk_kv_pages_append": (_i32, [_p, _i64, _p, _p, _i64, _p, _i64, _p]),
+    "nk_kv_pages_copy": (_i32, [_p, _p, _p, _i64, _p]),
+    "nk_kv_table_write": (_i32, [_p, _i64, _p, _p, _i64, _p]),
+    "nk_kv_pages_compact": (_i32, [_p, _p, _p]),
+    "nk_attention_paged_workspace_bytes": (_i32, [_p, _p, _p, _p]),
+    "nk_attention_paged": (_i32, [_p, _i64, _p, _p, _p, _sz, _p]),
+    "nk_kv_block_select_workspace_bytes": (_i32, [_p, _p, _p]),
+    "nk_kv_block_select": (_i32, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _sz,
+                                  _p]),
     "nk_set_stage_timing": (_i32, [_i32]),
     "nk_moe_stage_times": (_i32, [_p, _i32, _p]),
 }
@@ -764,6 +805,316 @@ def attention_check(workspace, stream=None) -> int:
     r = ctypes.c_int64(0)
     call("nk_attention_check", ptr(workspace), ctypes.byref(r), stream_ptr(stream))
     return r.value
+
+
+# ------------------------------------------------------------- paged KV cache
+def _expect(t, name, dtype, dim, device=None):
+    """A device tensor of the given type and rank whose last dimension is dense."""
+    if t.dtype != dtype or t.dim() != dim:
+        raise TypeError(f"{name} must be {dtype} with {dim} dimensions, got {t.dtype} "
+                        f"{tuple(t.shape)}")
+    if not t.is_cuda:
+        raise RuntimeError("libnk entry points take device tensors")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the pages on {device}")
+    if t.numel() and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be dense in its last dimension")
+
+
+def _expect_ints(t, name, n, device):
+    import torch
+
+    _expect(t, name, torch.int32, 1, device)
+    if t.numel() != n:
+        raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
+
+
+class _OnDevice:
+    """Runs libnk calls on the pages' device, whichever is current, and keeps
+    temporaries alive for an explicit stream."""
+
+    def __init__(self, device, stream):
+        import torch
+
+        self._guard = None
+        if torch.cuda.current_device() != device.index:
+            self._guard = torch.cuda.device(device)
+        self.stream = stream
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+        self.ptr = stream_ptr(self.stream)
+        return self
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+    def hold(self, *tensors):
+        """Memory handed to this stream is not given out again before the
+        stream's queued work is done with it."""
+        if self.stream is not None:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+
+
+class KvPages:
+    """A pool of KV pages and the table that strings them into sequences
+    (nk_kv_pages): k, v bf16 [layers, pages, kv_heads, page_size, head_dim],
+    table int32 [sequences, blocks]; k_min, k_max bf16 [layers, pages,
+    kv_heads, head_dim] hold the channel bounds of each page's keys, which
+    kv_block_select reads (optional).  nk_paged.PagedKvCache manages one."""
+
+    def __init__(self, k, v, table, *, k_min=None, k_max=None):
+        import torch
+
+        _expect(k, "k", torch.bfloat16, 5)
+        dev = k.device
+        _expect(v, "v", torch.bfloat16, 5, dev)
+        _expect(table, "table", torch.int32, 2, dev)
+        if v.shape != k.shape or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("k and v must be contiguous and of one shape")
+        if (k_min is None) != (k_max is None):
+            raise ValueError("k_min and k_max go together")
+        for t, name in ((k_min, "k_min"), (k_max, "k_max")):
+            if t is not None:
+                _expect(t, name, torch.bfloat16, 4, dev)
+                if t.shape != k.shape[:3] + k.shape[4:] or not t.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous [layers, pages, kv_heads, "
+                                     "head_dim]")
+        self.k, self.v, self.table, self.k_min, self.k_max = k, v, table, k_min, k_max
+        self.layers, self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = dev
+        self._struct = NkKvPages(*k.shape, ptr(k), ptr(v), ptr(k_min), ptr(k_max), ptr(table),
+                                 table.shape[0], table.stride(0) if table.shape[0] > 1
+                                 else table.shape[1])
+        self._ref = ctypes.byref(self._struct)
+
+    def batch(self, start, kv_len, tokens, max_new, max_kv, rows=None) -> NkKvBatch:
+        """The ragged batch of one step (nk_kv_batch): start int32 [n + 1],
+        kv_len int32 [n], rows int32 [n] or None on the pages' device."""
+        n = kv_len.numel()
+        _expect_ints(start, "start", n + 1, self.device)
+        _expect_ints(kv_len, "kv_len", n, self.device)
+        if rows is not None:
+            _expect_ints(rows, "rows", n, self.device)
+        return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(), ptr(rows), max_new,
+                         max_kv)
+
+
+def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max_kv=None,
+                    rows=None, layer: int = 0, stream=None) -> None:
+    """Stores new keys and values (bf16 [tokens, kv_heads * head_dim], any row
+    stride that is a multiple of 8) at the last positions of their sequences
+    (nk_kv_pages_append).  max_kv defaults to what the table can hold."""
+    import torch
+
+    width = pages.kv_heads * pages.head_dim
+    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
+        _expect(t, name, torch.bfloat16, 2, pages.device)
+        if t.shape != (k_new.shape[0], width):
+            raise ValueError(f"{name} must be [tokens, {width}]")
+    tokens = k_new.shape[0]
+    b = pages.batch(start, kv_len, tokens, max_new, _max_kv(pages, max_kv), rows)
+    with _OnDevice(pages.device, stream) as on:
+        call("nk_kv_pages_append", pages._ref, layer, ctypes.byref(b), k_new.data_ptr(),
+             k_new.stride(0) if tokens > 1 else width, v_new.data_ptr(),
+             v_new.stride(0) if tokens > 1 else width, on.ptr)
+
+
+def _max_kv(pages: KvPages, max_kv):
+    return max_kv if max_kv is not None else pages.table.shape[1] * pages.page_size
+
+
+def _host_ints(a, dtype):
+    import numpy as np
+
+    return np.ascontiguousarray(np.asarray(a).reshape(-1), dtype=dtype)
+
+
+def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
+    """Page dst[i] becomes a copy of page src[i] in every layer
+    (nk_kv_pages_copy); src, dst are host sequences of page ids."""
+    import numpy as np
+
+    s, d = _host_ints(src, np.int32), _host_ints(dst, np.int32)
+    if s.size != d.size:
+        raise ValueError("src and dst must have one length")
+    with _OnDevice(pages.device, stream) as on:
+        call("nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size, on.ptr)
+
+
+def kv_table_write(dst, values, offsets=None, stream=None) -> None:
+    """dst.view(-1)[offsets[i]] = values[i] (nk_kv_table_write; offsets None:
+    the first len(values) entries); dst is a contiguous int32 device tensor,
+    values and offsets are host sequences."""
+    import numpy as np
+    import torch
+
+    if dst.dtype != torch.int32 or not dst.is_contiguous():
+        raise TypeError("dst must be a contiguous int32 tensor")
+    _require_cuda(dst)
+    v = _host_ints(values, np.int32)
+    o = None if offsets is None else _host_ints(offsets, np.int64)
+    if o is not None and o.size != v.size:
+        raise ValueError("offsets and values must have one length")
+    with _OnDevice(dst.device, stream) as on:
+        call("nk_kv_table_write", ptr(dst), dst.numel(), None if o is None else o.ctypes.data,
+             v.ctypes.data, v.size, on.ptr)
+
+
+def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, dst_table=None,
+                     new_len=None, stream=None):
+    """Token base[b] + keep[b, i] of sequence b moves to position base[b] + i
+    (nk_kv_pages_compact), in place or into the pages of dst_table; all
+    arguments int32 on the device, keep [n, max_keep] strictly ascending.
+    Returns the new lengths base + n_keep."""
+    import torch
+
+    n, dev = kv_len.numel(), pages.device
+    for t, name in ((kv_len, "kv_len"), (base, "base"), (n_keep, "n_keep")):
+        _expect_ints(t, name, n, dev)
+    if rows is not None:
+        _expect_ints(rows, "rows", n, dev)
+    _expect(keep, "keep", torch.int32, 2, dev)
+    if keep.shape[0] != n:
+        raise ValueError("keep must have a row for each sequence")
+    if dst_table is not None:
+        _expect(dst_table, "dst_table", torch.int32, 2, dev)
+        if dst_table.shape[0] != n:
+            raise ValueError("dst_table must have a row for each sequence")
+    if new_len is not None:
+        _expect_ints(new_len, "new_len", n, dev)
+    with _OnDevice(dev, stream) as on:
+        if new_len is None:
+            new_len = torch.empty(n, dtype=torch.int32, device=dev)
+            on.hold(new_len)
+        width = keep.shape[1]
+        a = NkKvCompactArgs(n, ptr(rows), ptr(kv_len), ptr(base), ptr(keep),
+                            keep.stride(0) if n > 1 else width, ptr(n_keep), width,
+                            ptr(dst_table), 0 if dst_table is None else
+                            (dst_table.stride(0) if n > 1 else dst_table.shape[1]), ptr(new_len))
+        call("nk_kv_pages_compact", pages._ref, ctypes.byref(a), on.ptr)
+    return new_len
+
+
+def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=None, max_kv=None,
+                    tree_mask=None, blocks=None, rows=None, layer: int = 0, scale=None,
+                    out_dtype=BF16, out=None, workspace=None, stream=None):
+    """Attention of new tokens over their sequences' pages (nk_attention_paged).
+
+    q bf16 [tokens, q_heads * head_dim]; sequence b's tokens are rows
+    start[b] .. start[b+1]-1 and the last ones of its kv_len[b] positions.
+    Without masks a token attends every position up to its own; with tree_mask
+    (int64 [tokens], bit j: the sequence's new token j) every cached position
+    and the drafts of its branch; with blocks (int32 [tokens, kv_heads, n],
+    kv_block_select) the listed blocks.  max_q and max_kv bound the new tokens
+    and the length of a sequence (defaults: all tokens, the table's width);
+    close bounds cost less.  Returns [tokens, q_heads * head_dim] in bf16, or
+    f32 with out_dtype=F32; rows that belong to no sequence stay as they were
+    (a new `out` is not initialised).  workspace: optional uint8 device tensor
+    of attention_paged_workspace_bytes."""
+    import torch
+
+    dev = pages.device
+    _expect(q, "q", torch.bfloat16, 2, dev)
+    tokens, width = q.shape
+    if width != q_heads * pages.head_dim:
+        raise ValueError(f"q must be [tokens, {q_heads * pages.head_dim}]")
+    if tree_mask is not None:
+        _expect(tree_mask, "tree_mask", torch.int64, 1, dev)
+        if tree_mask.numel() != tokens:
+            raise ValueError("tree_mask must hold a word for each token")
+    if blocks is not None:
+        _expect(blocks, "blocks", torch.int32, 3, dev)
+        if blocks.shape[:2] != (tokens, pages.kv_heads) or not blocks.is_contiguous():
+            raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
+    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q,
+                    _max_kv(pages, max_kv), rows)
+    with _OnDevice(dev, stream) as on:
+        if out is None:
+            out = torch.empty(tokens, width, device=dev,
+                              dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
+            on.hold(out)
+        elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
+            raise ValueError("out must be contiguous, of q's shape and on its device")
+        a = NkPagedAttentionArgs(q.data_ptr(), q.stride(0) if tokens > 1 else width, q_heads,
+                                 ptr(tree_mask), ptr(blocks),
+                                 0 if blocks is None else blocks.shape[2],
+                                 0 if scale is None else 1, 0.0 if scale is None else scale,
+                                 out.data_ptr(), _dtype_code(out))
+        br, ar = ctypes.byref(b), ctypes.byref(a)
+        if workspace is None:
+            need = ctypes.c_size_t(0)
+            call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
+            if need.value:
+                workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+                on.hold(workspace)
+        call("nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace),
+             0 if workspace is None else workspace.numel(), on.ptr)
+    return out
+
+
+def attention_paged_workspace_bytes(pages: KvPages, tokens: int, seqs: int, q_heads: int, *,
+                                    max_q: int, max_kv: int, max_blocks: int = 0) -> int:
+    """Scratch bytes of attention_paged for these bounds (max_blocks > 0: the
+    form with block lists of that width)."""
+    b = NkKvBatch(seqs, tokens, 16, 16, 16, max_q, max_kv)  # only the bounds are read
+    a = NkPagedAttentionArgs(None, q_heads * pages.head_dim, q_heads, None,
+                             16 if max_blocks else None, max_blocks, 0, 0.0, None, BF16)
+    need = ctypes.c_size_t(0)
+    call("nk_attention_paged_workspace_bytes", pages._ref, ctypes.byref(b), ctypes.byref(a),
+         ctypes.byref(need))
+    return need.value
+
+
+def kv_block_select(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *, sink: int = 1,
+                    local: int = 1, max_q=None, max_kv=None, rows=None, layer: int = 0, out=None,
+                    workspace=None, stream=None):
+    """The blocks each token's query reads (nk_kv_block_select): int32 [tokens,
+    kv_heads, top_k], ascending, -1 behind the last; the first `sink` and last
+    `local` blocks and those whose key bounds allow the largest scores."""
+    import torch
+
+    dev = pages.device
+    _expect(q, "q", torch.bfloat16, 2, dev)
+    tokens, width = q.shape
+    if width != q_heads * pages.head_dim:
+        raise ValueError(f"q must be [tokens, {q_heads * pages.head_dim}]")
+    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q,
+                    _max_kv(pages, max_kv), rows)
+    with _OnDevice(dev, stream) as on:
+        if out is None:
+            out = torch.empty(tokens, pages.kv_heads, max(top_k, 1), dtype=torch.int32, device=dev)
+            on.hold(out)
+        else:
+            _expect(out, "out", torch.int32, 3, dev)
+            if out.shape != (tokens, pages.kv_heads, top_k) or not out.is_contiguous():
+                raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
+        br = ctypes.byref(b)
+        if workspace is None:
+            need = ctypes.c_size_t(0)
+            call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
+            workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+            on.hold(workspace)
+        call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(),
+             q.stride(0) if tokens > 1 else width, q_heads, top_k, sink, local, ptr(out),
+             ptr(workspace), workspace.numel(), on.ptr)
+    return out
+
+
+def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *,
+                           sink: int = 1, local: int = 1, max_q=None, max_kv=None, rows=None,
+                           layer: int = 0, scale=None, out_dtype=BF16, out=None, stream=None):
+    """kv_block_select, then attention_paged over the chosen blocks; returns
+    (out, blocks)."""
+    blocks = kv_block_select(q, pages, start, kv_len, q_heads, top_k, sink=sink, local=local,
+                             max_q=max_q, max_kv=max_kv, rows=rows, layer=layer, stream=stream)
+    return attention_paged(q, pages, start, kv_len, q_heads, max_q=max_q, max_kv=max_kv,
+                           blocks=blocks, rows=rows, layer=layer, scale=scale,
+                           out_dtype=out_dtype, out=out, stream=stream), blocks
 
 
 # ------------------------------------------------- decoder steps around projections

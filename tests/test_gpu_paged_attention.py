@@ -1,0 +1,409 @@
+"""Attention over paged caches on the B200 against the formula in 64 bits.
+
+Tolerance, element by element.  With weights w (sum 1) and values v the
+kernel rounds each weight to bf16 (at most 2^-8 of it, so 2^-8 sum w|v| in
+all), sums 128 exact products of a score in f32 (128 * 2^-22 * sum|q k| *
+scale <= 2^-11 relative in a weight for unit-variance inputs, which also
+covers the exponential and the f32 sums), and rounds a bf16 result once
+(2^-8 of it):  |error| <= (2^-8 + 2^-11) sum w|v| + [bf16] 2^-8 |out|."""
+import numpy as np
+import pytest
+import torch
+
+import nk
+import nk_paged
+from gpu_util import dev
+from paged_ref import Paged, attention, bf16, chosen_blocks, ints, starts, tree_masks
+
+pytestmark = pytest.mark.gpu
+
+
+def _close(got, want, mag, f32=False):
+    got = got.double().cpu().numpy().reshape(want.shape)
+    tol = (2.0**-8 + 2.0**-11) * mag + (0 if f32 else 2.0**-8) * np.abs(want)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    bad = ~same & ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:4], got[bad][:4], want[bad][:4], tol[bad][:4])
+
+
+def _reference(c, q, counts, q_heads, kind, masks=None, lists=None, scale=None, layer=0):
+    """[tokens, q_heads, d] and magnitudes for the whole batch."""
+    outs, mags, at = [], [], 0
+    for s, t in enumerate(counts):
+        n = int(c.lens[s])
+        seen = np.zeros((t, c.heads if lists is not None else 1, n), bool)
+        for i in range(t):
+            pos = n - t + i
+            if kind == "tree":
+                seen[i, 0, :n - t] = True
+                seen[i, 0, n - t:] = masks[s][i]
+            elif kind == "blocks":
+                for h in range(c.heads):
+                    for b in lists[at + i][h]:
+                        if 0 <= b <= pos // c.ps:
+                            seen[i, h, b * c.ps:min(pos + 1, (b + 1) * c.ps)] = True
+            else:
+                seen[i, 0, :pos + 1] = True
+        k, v = c.tokens(c.k, s, layer), c.tokens(c.v, s, layer)
+        o, m = attention(q[at:at + t], k, v, seen, c.d ** -0.5 if scale is None else scale)
+        outs.append(o)
+        mags.append(m)
+        at += t
+    return np.concatenate(outs), np.concatenate(mags)
+
+
+CASES = [  # ps, d, kv heads, group, lens, counts
+    (16, 64, 1, 1, [1], [1]),                                   # one token in all
+    (64, 128, 2, 16, [1025], [1]),                              # split over keys
+    (64, 128, 2, 16, [64, 63, 65, 700, 1], [1, 1, 1, 1, 1]),    # page and tile edges
+    (32, 64, 4, 4, [777, 31, 200], [7, 3, 0]),                  # a sequence without queries
+    (16, 128, 3, 5, [129, 300], [9, 64]),                       # odd heads, 45 and 320 rows
+    (128, 64, 2, 8, [513, 1000, 128], [64, 33, 2]),
+    (128, 128, 1, 32, [640], [5]),
+    (16, 64, 2, 2, [2000], [1]),
+    (64, 128, 1, 1, [90, 5000], [64, 17])]
+
+
+@pytest.mark.parametrize("ps,d,kv,group,lens,counts", CASES)
+@pytest.mark.parametrize("kind", ["causal", "tree"])
+def test_matches_the_formula(cuda, ps, d, kv, group, lens, counts, kind):
+    c = Paged(ps + d + len(lens), lens, kv, ps, d)  # NaN wherever no token is
+    H, T = kv * group, sum(counts)
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    pages = c.device()
+    masks, words = [], []
+    for t in counts:
+        w, seen = tree_masks(c.rng, t)
+        masks.append(seen)
+        words.append(w)
+    tree = torch.from_numpy(np.concatenate(words)).cuda() if kind == "tree" else None
+    want, mag = _reference(c, q, counts, H, kind, masks)
+    for dt in (nk.BF16, nk.F32):
+        got = nk.attention_paged(dev(q.reshape(T, H * d)).bfloat16(), pages, ints(starts(counts)),
+                                 ints(lens), H, max_q=max(counts), max_kv=max(lens),
+                                 tree_mask=tree, out_dtype=dt)
+        nk.device_status()
+        _close(got, want, mag, dt == nk.F32)
+
+
+@pytest.mark.parametrize("ps,d,kv,group,lens,count", [
+    (64, 128, 2, 4, [300], 300), (16, 64, 2, 2, [1000, 257], 257), (32, 128, 1, 8, [190], 130)])
+def test_prefill_chunks(cuda, ps, d, kv, group, lens, count):
+    c = Paged(3, lens, kv, ps, d)
+    counts = [min(count, n) for n in lens]
+    T, H = sum(counts), kv * group
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    got = nk.attention_paged(dev(q.reshape(T, -1)).bfloat16(), c.device(), ints(starts(counts)),
+                             ints(lens), H, max_q=max(counts), max_kv=max(lens))
+    nk.device_status()
+    want, mag = _reference(c, q, counts, H, "causal")
+    _close(got, want, mag)
+
+
+def test_loose_bounds_layers_scale_and_strided_queries(cuda):
+    """max_q and max_kv far above what the batch holds, the second of two
+    layers, rows of other sequences between, q a view of a fused projection,
+    and rows behind the last sequence that keep what they held."""
+    c = Paged(8, [100, 40, 333], 2, 32, 64, layers=2, width=40)
+    H, d = 4, 64
+    counts, rows = [3, 2], [2, 0]
+    q = bf16(c.rng.standard_normal((8, H, d)))
+    wide = torch.randn(8, H * d + 128, device="cuda").bfloat16()
+    wide[:, 64:64 + H * d] = dev(q.reshape(8, -1)).bfloat16()
+    out = torch.full((8, H * d), 5.0, device="cuda")
+    got = nk.attention_paged(wide[:, 64:64 + H * d], c.device(), ints(starts(counts)),
+                             ints([333, 100]), H, rows=ints(rows), layer=1, scale=0.3, out=out)
+    nk.device_status()
+    o = Paged.__new__(Paged)
+    o.__dict__.update(c.__dict__)
+    o.table, o.lens = c.table[rows], c.lens[rows]
+    want, mag = _reference(o, q, counts, H, "causal", scale=0.3, layer=1)
+    # the score error bound scales with the scale: 0.3 / 0.125 of the default's
+    _close(got[:5], want, mag * (1 + 2.0**-3), True)
+    assert (got[5:] == 5.0).all()
+
+
+def test_rows_that_see_nothing_are_zero(cuda):
+    c = Paged(2, [5, 9], 1, 16, 64)
+    q = bf16(c.rng.standard_normal((7, 2, 64)))
+    words = [0, 1, 0b11, 0, 0b10000, 0, 0]  # five drafts without a prefix, then two with one
+    got = nk.attention_paged(dev(q.reshape(7, -1)).bfloat16(), c.device(), ints([0, 5, 7]),
+                             ints([5, 9]), 2, max_q=5, max_kv=9, out_dtype=nk.F32,
+                             tree_mask=torch.tensor(words, device="cuda"))
+    nk.device_status()
+    seen = [np.array([[w >> j & 1 for j in range(5)] for w in words[:5]], bool),
+            np.zeros((2, 2), bool)]
+    want, mag = _reference(c, q, [5, 2], 2, "tree", seen)
+    _close(got, want, mag, True)
+    assert not got[0].any() and not got[3].any() and got[5].any()
+
+
+@pytest.mark.parametrize("group,T", [(1, 6), (8, 6), (16, 9)])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_masked_infinities_and_nan_do_not_reach_a_row(cuda, value, group, T):
+    """One branch's draft holds an infinity or NaN in its key, another in its
+    value: rows of other branches are exact, rows that see them get what the
+    formula gives."""
+    c = Paged(6, [70 + T], 2, 16, 64)
+    H = 2 * group
+    words, seen = tree_masks(c.rng, T)
+    seen[:] = np.eye(T, dtype=bool)
+    seen[4, 1] = True
+    words = np.array([sum(1 << int(j) for j in np.flatnonzero(r)) for r in seen], np.int64)
+    p, s = c.slot(0, 70 + 1)
+    c.v[0, p, 0, s, 3] = value            # seen by drafts 1 and 4
+    p, s = c.slot(0, 70 + 2)
+    c.k[0, p, 1, s, 5] = value            # seen by draft 2
+    q = bf16(np.abs(c.rng.standard_normal((T, H, 64))) + 0.1)
+    got = nk.attention_paged(dev(q.reshape(T, -1)).bfloat16(), c.device(), ints([0, T]),
+                             ints([70 + T]), H, max_q=T, max_kv=70 + T, out_dtype=nk.F32,
+                             tree_mask=torch.from_numpy(words).cuda())
+    nk.device_status()
+    want, mag = _reference(c, q, [T], H, "tree", [seen])
+    clean = [0, 3] + list(range(5, T))
+    assert np.isfinite(want[clean]).all()
+    mag = np.where(np.isfinite(mag), mag, 0)
+    _close(got, want, mag, True)
+
+
+def test_causal_chunk_with_an_infinite_value(cuda):
+    c = Paged(7, [90], 1, 32, 128)
+    p, s = c.slot(0, 60)
+    c.v[0, p, 0, s, 100] = np.inf
+    q = bf16(c.rng.standard_normal((50, 2, 128)))
+    got = nk.attention_paged(dev(q.reshape(50, -1)).bfloat16(), c.device(), ints([0, 50]),
+                             ints([90]), 2, max_q=50, max_kv=90)
+    nk.device_status()
+    want, mag = _reference(c, q, [50], 2, "causal")
+    assert np.isfinite(want[:20]).all() and np.isinf(want[20:, :, 100]).all()
+    _close(got, want, np.where(np.isfinite(mag), mag, 0))
+
+
+def test_minus_infinite_scores_leave_no_weight(cuda):
+    # every key of the sequence scores -inf: as if nothing were seen
+    c = Paged(1, [40], 1, 16, 64)
+    c.k[0, c.table[0]] = -np.inf
+    q = np.ones((1, 1, 64), np.float32)
+    got = nk.attention_paged(dev(q.reshape(1, -1)).bfloat16(), c.device(), ints([0, 1]),
+                             ints([40]), 1, max_q=1, max_kv=40)
+    nk.device_status()
+    assert not got.any()
+
+
+@pytest.mark.parametrize("start,kv_len,rows,edit,code", [
+    ([0, 2], [65], None, None, nk.INVALID_PARAMS), ([0, 2], [1], None, None, nk.INVALID_PARAMS),
+    ([2, 0], [40], None, None, nk.INVALID_PARAMS), ([0, 3], [40], None, None, nk.INVALID_PARAMS),
+    ([0, 2], [40], [1], None, nk.INVALID_PARAMS),
+    ([0, 2], [40], None, 10**6, nk.PAGE_OUT_OF_RANGE),
+    ([0, 2], [40], None, -1, nk.PAGE_OUT_OF_RANGE)])
+def test_contradicting_batches_are_reported(cuda, start, kv_len, rows, edit, code):
+    c = Paged(1, [40], 2, 16, 64, width=4)
+    if edit is not None:
+        c.table[0, 1] = edit
+    pages = c.device()
+    q = torch.randn(2, 256, device="cuda").bfloat16()
+    out = torch.full((2, 256), 9.0, device="cuda")
+    r = None if rows is None else ints(rows)
+    nk.attention_paged(q, pages, ints(start), ints(kv_len), 4, max_q=2, max_kv=64, rows=r, out=out)
+    with pytest.raises(nk.NkError) as e:
+        nk.device_status()
+    assert e.value.code == code
+    if code == nk.INVALID_PARAMS:
+        assert (out == 9.0).all()
+    else:
+        assert torch.isfinite(out).all()  # the page is not read
+    lists = torch.full((2, 2, 3), 7, dtype=torch.int32, device="cuda")
+    nk.kv_block_select(q, pages, ints(start), ints(kv_len), 4, 3, max_q=2, max_kv=64, rows=r,
+                       out=lists)
+    try:
+        nk.device_status()
+    except nk.NkError as e2:
+        assert e2.code == code
+    if code == nk.INVALID_PARAMS:
+        assert (lists == 7).all()
+
+
+@pytest.mark.parametrize("lens,T,H,kv", [([2000], 1, 32, 2), ([300, 1200, 64], 2, 8, 8),
+                                         ([700], 64, 16, 1)])
+def test_captured_and_on_another_stream(cuda, lens, T, H, kv):
+    """Two graphs with workspaces of their own replayed in turn on new inputs,
+    and two calls in flight on two streams."""
+    c = Paged(4, lens, kv, 64, 64)
+    pages, counts = c.device(), [T] * len(lens)
+    args = (ints(starts(counts)), ints(lens), H)
+    kw = dict(max_q=T, max_kv=max(lens))
+    n = T * len(lens)
+    qs = [torch.randn(n, H * 64, device="cuda").bfloat16() for _ in range(4)]
+    want = [nk.attention_paged(q, pages, *args, **kw) for q in qs]
+    static = [torch.empty_like(qs[0]) for _ in range(2)]
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(nk.attention_paged(static[i], pages, *args, **kw))
+        graphs.append(g)
+    for pair in ((0, 1), (2, 3)):
+        for i in range(2):
+            static[i].copy_(qs[pair[i]])
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[pair[i]])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [nk.attention_paged(qs[i], pages, *args, stream=streams[i % 2], **kw)
+           for i in range(4)]
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert torch.equal(got[i], want[i])
+    nk.device_status()
+
+
+def test_explicit_workspace(cuda):
+    c = Paged(4, [3000], 2, 64, 64)
+    pages, q = c.device(), torch.randn(1, 256, device="cuda").bfloat16()
+    need = nk.attention_paged_workspace_bytes(pages, 1, 1, 4, max_q=1, max_kv=3000)
+    assert need > 0
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    args = (q, pages, ints([0, 1]), ints([3000]), 4)
+    a = nk.attention_paged(*args, max_q=1, max_kv=3000, workspace=ws)
+    b = nk.attention_paged(*args, max_q=1, max_kv=3000)
+    assert torch.equal(a, b)
+    with pytest.raises(nk.NkError) as e:
+        nk.attention_paged(*args, max_q=1, max_kv=3000, workspace=ws[:need - 16])
+    assert e.value.code == nk.WORKSPACE_TOO_SMALL
+
+
+# -------------------------------------------------------------- block lists
+SELECT = [  # ps, d, kv, group, lens, counts, top_k, sink, local
+    (16, 64, 1, 1, [5], [1], 3, 1, 1),                       # one block, a longer list
+    (64, 128, 2, 16, [4000, 64, 65], [1, 1, 1], 8, 1, 2),
+    (32, 64, 8, 4, [900, 333], [2, 3], 9, 2, 1),
+    (16, 128, 2, 3, [5000, 15], [1, 2], 64, 0, 1),
+    (128, 64, 1, 8, [20000], [1], 5, 1, 1),
+    (16, 64, 2, 2, [700], [40], 6, 3, 3)]                    # nothing left to rank
+
+
+@pytest.mark.parametrize("ps,d,kv,group,lens,counts,top_k,sink,local", SELECT)
+def test_block_select_and_sparse_attention(cuda, ps, d, kv, group, lens, counts, top_k, sink,
+                                           local):
+    c = Paged(ps + d + top_k, lens, kv, ps, d)
+    H, T = kv * group, sum(counts)
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    lists = np.full((T, kv, top_k), -1, np.int32)
+    at = 0
+    for s, t in enumerate(counts):
+        for i in range(t):
+            n = (int(lens[s]) - t + i) // ps + 1
+            for h in range(kv):
+                x = chosen_blocks(q[at, h * group:(h + 1) * group], c.lo[0, c.table[s, :n], h],
+                                  c.hi[0, c.table[s, :n], h], n, top_k, sink, local)
+                lists[at, h, :len(x)] = x
+            at += 1
+    want, mag = _reference(c, q, counts, H, "blocks", lists=lists)
+    out, blocks = nk.attention_paged_sparse(dev(q.reshape(T, -1)).bfloat16(), c.device(),
+                                            ints(starts(counts)), ints(lens), H, top_k, sink=sink,
+                                            local=local, max_q=max(counts), max_kv=max(lens))
+    nk.device_status()
+    assert np.array_equal(blocks.cpu().numpy(), lists)
+    _close(out, want, mag)
+
+
+def test_block_select_ties_and_nan(cuda):
+    """Equal scores go to the lower block; a block whose score is NaN is last."""
+    ps, d = 16, 64
+    c = Paged(0, [16 * 40], 1, ps, d)
+    c.lo[:], c.hi[:] = -1.0, 1.0                    # every block ties
+    c.hi[0, c.table[0, 20]] = np.nan
+    c.lo[0, c.table[0, 20]] = np.nan
+    c.hi[0, c.table[0, 33], 0, 2] = 50.0
+    q = np.ones((1, 1, d), np.float32)
+    q[0, 0, 1::2] = -1
+    pages = c.device()
+    args = (dev(q.reshape(1, -1)).bfloat16(), pages, ints([0, 1]), ints([16 * 40]), 1)
+    got = nk.kv_block_select(*args, 6, sink=1, local=1, max_q=1, max_kv=640)
+    assert got.cpu().numpy()[0, 0].tolist() == [0, 1, 2, 3, 33, 39]
+    got = nk.kv_block_select(*args, 39, sink=0, local=1, max_q=1, max_kv=640)
+    assert got.cpu().numpy()[0, 0].tolist() == [j for j in range(40) if j != 20]
+    nk.device_status()
+
+
+def test_lists_with_repeated_and_foreign_blocks(cuda):
+    """Entries that are negative, repeated or past the token are skipped."""
+    c = Paged(3, [100, 50], 2, 16, 64)
+    q = bf16(c.rng.standard_normal((2, 4, 64)))
+    lists = np.array([[[0, 0, 3, 3, 6, 9], [-1, 2, 2, 5, 4, 10**6]],
+                      [[-7, -1, -1, -1, -1, -1], [1, 3, 3, 4, 4, 5]]], np.int32)
+    clean = [[[0, 3, 6], [2, 5]], [[], [1, 3]]]
+    got = nk.attention_paged(dev(q.reshape(2, -1)).bfloat16(), c.device(), ints([0, 1, 2]),
+                             ints([100, 50]), 4, max_q=1, max_kv=100, out_dtype=nk.F32,
+                             blocks=ints(lists))
+    nk.device_status()
+    want, mag = _reference(c, q, [1, 1], 4, "blocks", lists=clean)
+    _close(got, want, mag, True)
+    assert not got[1, :128].any()
+
+
+# ------------------------------------------------------- together, as in use
+def test_drafting_and_sparse_reading_over_one_cache(cuda):
+    """Prefill of two prompts, a fork, a drafted tree verified and accepted,
+    then a sparse step: each attention equals the formula over the tokens that
+    the sequence holds by then."""
+    heads, d, ps, group = 2, 64, 16, 4
+    H = heads * group
+    r = np.random.default_rng(1)
+    cache = nk_paged.PagedKvCache(80, heads, d, max_seqs=4, max_len=400, page_size=ps)
+    kv = {}
+
+    def feed(seqs, counts):
+        step = cache.step(seqs, counts)
+        k, v, q = (bf16(r.standard_normal((step.tokens, n, d))) for n in (heads, heads, H))
+        t = lambda a: dev(a.reshape(step.tokens, -1)).bfloat16()  # noqa: E731
+        cache.append(step, t(k), t(v))
+        at = 0
+        for s, c in zip(seqs, counts):
+            old = kv.get(s, np.zeros((2, 0, heads, d), np.float32))
+            kv[s] = np.concatenate([old, np.stack([k[at:at + c], v[at:at + c]])], 1)
+            at += c
+        return step, q, t(q)
+
+    def check(got, q, step, masks=None, lists=None):
+        at = 0
+        for s, c in zip(step.seqs, step.counts):
+            n = kv[s].shape[1]
+            seen = np.tri(c, n, n - c, dtype=bool)[:, None]
+            if masks is not None:
+                seen[:, 0, n - c:] = masks[s]
+            if lists is not None:
+                seen = np.repeat(seen, heads, 1)
+                for i in range(c):
+                    for h in range(heads):
+                        hit = np.isin(np.arange(n) // ps, lists[at + i, h])
+                        seen[i, h] &= hit
+            o, m = attention(q[at:at + c], kv[s][0].transpose(1, 0, 2),
+                             kv[s][1].transpose(1, 0, 2), seen, d**-0.5)
+            _close(got[at:at + c], o, m)
+            at += c
+
+    a, b = cache.new_sequence(), cache.new_sequence()
+    step, q, qd = feed([a, b], [130, 75])
+    check(cache.attend(qd, step, H), q, step)
+    c = cache.fork(a)
+    kv[c] = kv[a].copy()
+    words, masks, seqs = [], {}, [b, c, a]
+    for s in seqs:
+        w, masks[s] = tree_masks(r, 11)
+        words.append(w)
+    step, q, qd = feed(seqs, [11, 11, 11])
+    tree = torch.from_numpy(np.concatenate(words)).cuda()
+    check(cache.attend(qd, step, H, tree_mask=tree), q, step, masks)
+    keep = [sorted(np.flatnonzero(masks[s][10]).tolist()) for s in seqs]
+    cache.accept(step, keep)
+    for s, row in zip(seqs, keep):
+        n = kv[s].shape[1] - 11
+        kv[s] = kv[s][:, list(range(n)) + [n + i for i in row]]
+    for _ in range(3):
+        step, q, qd = feed([c, a, b], [1, 2, 1])
+        out, lists = cache.attend_sparse(qd, step, H, 4, sink=1, local=1)
+        check(out, q, step, lists=lists.cpu().numpy())
+    nk.device_status()

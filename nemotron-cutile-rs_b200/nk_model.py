@@ -24,6 +24,7 @@ import torch
 
 import nk
 import nk_mamba
+import nk_paged
 
 
 @dataclass
@@ -68,11 +69,16 @@ class AttentionMixer:
         self.hq, self.hkv, self.d = q_heads, kv_heads, head_dim
         self.ws = None
 
-    def forward(self, x, batch, seq, cache: nk.KvCache, workspace=None):
-        """workspace: optional one-element list holding a buffer shared by layers."""
+    def forward(self, x, batch, seq, cache, workspace=None):
+        """cache: nk.KvCache, or the PagedLayer of a paged state.  workspace:
+        optional one-element list holding a buffer shared by layers."""
         q = nk.gemm(x, self.wq, out_dtype=torch.bfloat16)
         k = nk.gemm(x, self.wk, out_dtype=torch.bfloat16)
         v = nk.gemm(x, self.wv, out_dtype=torch.bfloat16)
+        if isinstance(cache, PagedLayer):
+            cache.cache.append(cache.step, k, v, layer=cache.layer)
+            o = cache.cache.attend(q, cache.step, self.hq, layer=cache.layer)
+            return nk.gemm(o, self.wo, out_dtype=torch.float32)
         cache.append(k, v, seq)
         slot = workspace if workspace is not None else [self.ws]
         o, slot[0] = nk.attention_gqa(q, cache, seq, self.hq, causal=True, out_dtype=nk.BF16,
@@ -80,6 +86,15 @@ class AttentionMixer:
         if workspace is None:
             self.ws = slot[0]
         return nk.gemm(o, self.wo, out_dtype=torch.float32)
+
+
+class PagedLayer:
+    """One attention layer of a paged decoder state: the cache that the layers
+    share, the layer's index in it, the batch's sequences and the step that
+    the current forward has reserved."""
+
+    def __init__(self, cache: nk_paged.PagedKvCache, layer, seqs):
+        self.cache, self.layer, self.seqs, self.step = cache, layer, seqs, None
 
 
 class Decoder:
@@ -160,13 +175,25 @@ class Decoder:
         return ("attention", m)
 
     # ---- state ----------------------------------------------------------------
-    def new_state(self, batch, max_len):
-        """Per-layer caches: KV caches (attention), conv + SSM states (Mamba)."""
+    def new_state(self, batch, max_len, page_size=None):
+        """Per-layer caches: KV caches (attention), conv + SSM states (Mamba).
+        With page_size the attention layers share one paged cache
+        (nk_paged.PagedKvCache), a sequence per row of the batch."""
         c = self.cfg
         C = c.mamba_heads * c.mamba_head_dim
         st = []
+        paged = seqs = None
+        if page_size is not None and "attention" in c.layer_kinds:
+            paged = nk_paged.PagedKvCache(batch * (-(-max_len // page_size)), c.kv_heads,
+                                          c.head_dim, max_seqs=batch, max_len=max_len,
+                                          page_size=page_size,
+                                          layers=c.layer_kinds.count("attention"), bounds=False,
+                                          device=self.dev)
+            seqs = [paged.new_sequence() for _ in range(batch)]
         for kind, _ in self.layers:
-            if kind == "attention":
+            if kind == "attention" and paged is not None:
+                st.append(PagedLayer(paged, sum(isinstance(x, PagedLayer) for x in st), seqs))
+            elif kind == "attention":
                 st.append(nk.KvCache(batch, c.kv_heads, c.head_dim,
                                      ((max_len + 63) // 64) * 64, device=self.dev))
             elif kind == "mamba":
@@ -183,6 +210,11 @@ class Decoder:
         or of every row with logits_rows="all"."""
         c = self.cfg
         rows = batch * seq
+        paged = [st for st in state if isinstance(st, PagedLayer)]
+        if paged:  # the layers' slots of this step are the same
+            step = paged[0].cache.step(paged[0].seqs, [seq] * batch)
+            for st in paged:
+                st.step = step
         h = nk.embedding_lookup(self.embed, tokens, c.vocab, c.hidden, out_dtype=torch.float32,
                                 check=False)
         h, normed = nk.add_rms_norm_rows(h, None, self.norms[0], c.eps)
@@ -200,12 +232,13 @@ class Decoder:
             last = normed
         return nk.gemm(last, self.lm_head, out_dtype=torch.float32)
 
-    def generate(self, prompt, steps, max_len=None):
+    def generate(self, prompt, steps, max_len=None, page_size=None):
         """Greedy decoding: prompt int32 [batch, T] on the device; returns the
         generated ids [batch, steps] (int32, device).  No host synchronisation
-        between steps."""
+        between steps.  page_size: keep the KV cache in pages of that many
+        tokens."""
         batch, T = prompt.shape
-        state = self.new_state(batch, max_len or T + steps)
+        state = self.new_state(batch, max_len or T + steps, page_size=page_size)
         logits = self.forward(prompt.reshape(-1).contiguous(), batch, T, state)
         out = torch.empty(batch, steps, dtype=torch.int32, device=prompt.device)
         tok = nk.argmax_rows(logits)

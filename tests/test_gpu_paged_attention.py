@@ -11,8 +11,9 @@ import pytest
 import torch
 
 import nk
+import nk_model
 import nk_paged
-from gpu_util import dev
+from gpu_util import dev, host, rel_err, rng
 from paged_ref import Paged, attention, bf16, chosen_blocks, ints, starts, tree_masks
 
 pytestmark = pytest.mark.gpu
@@ -407,3 +408,26 @@ def test_drafting_and_sparse_reading_over_one_cache(cuda):
         out, lists = cache.attend_sparse(qd, step, H, 4, sink=1, local=1)
         check(out, q, step, lists=lists.cpu().numpy())
     nk.device_status()
+
+
+def test_decoder_over_pages_matches_the_contiguous_cache(cuda):
+    """The hybrid decoder, prefill and steps, over both caches: the same
+    projections, weights of the softmax rounded to bf16 in both (the contiguous
+    path normalises before the rounding), so the logits agree within the
+    decoder's own bar."""
+    tiny = dict(vocab=512, hidden=128, pattern="M*E*", mamba_heads=4, mamba_head_dim=32,
+                mamba_groups=2, mamba_state=32, conv_kernel=4, experts=8, top_k=2, moe_inter=64,
+                shared_inter=128, q_heads=4, kv_heads=2, head_dim=64, std=0.08)
+    model = nk_model.Decoder(nk_model.DecoderConfig(**tiny))
+    B, T, steps = 3, 21, 4
+    toks = rng(4).integers(0, 512, (B, T + steps)).astype(np.int32)
+    plain, paged = model.new_state(B, T + steps), model.new_state(B, T + steps, page_size=16)
+    feed = [(toks[:, :T], T)] + [(toks[:, T + s:T + s + 1], 1) for s in range(steps)]
+    for ids, n in feed:
+        ids = dev(ids.reshape(-1).copy())
+        x = model.forward(ids, B, n, plain)
+        y = model.forward(ids, B, n, paged)
+        assert rel_err(host(y), host(x)) <= 2e-2
+    nk.device_status()
+    out = model.generate(dev(toks[:, :T].copy()), steps, page_size=32)
+    assert out.shape == (B, steps) and int(out.min()) >= 0 and int(out.max()) < 512

@@ -14,7 +14,7 @@
 // product, as the operand type of the tensor cores asks, while l sums the
 // unrounded p.
 //
-// Tiles of 64 keys come by TMA (boxes of 64 channels x the keys of one page)
+// Tiles of 128 keys come by TMA (boxes of 64 channels x the keys of one page)
 // into a ring of shared-memory stages, in the 128-byte swizzle that ldmatrix
 // reads without bank conflicts.
 #include <cudaTypedefs.h>
@@ -24,7 +24,7 @@
 
 namespace nk {
 
-constexpr int kTile = 64;  // keys of a stage
+constexpr int kTile = 128;  // keys of a stage
 
 struct PagedAttn {
   PagePool pool;
@@ -39,9 +39,9 @@ struct PagedAttn {
   float scale_log2;  // scale * log2(e): exp(scale * s) = 2^(scale_log2 * s)
   void *out;
   int out_f32;
-  int splits, split_tiles;  // key tiles of a split
-  float *part_o;            // [splits][tokens * q_heads][head_dim], unnormalised
-  float2 *part_ml;          // [splits][tokens * q_heads]: m (in log2 units), l
+  float *part_o;          // [2 * blocks][row tile][head_dim], unnormalised
+  float2 *part_ml;        // [2 * blocks][row tile]: m (in log2 units), l
+  struct MergeJob *jobs;  // [blocks]
   int *err;
 };
 
@@ -76,511 +76,733 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<uint32_t *>(&v);
 }
 
-// Byte offset of (key, channel) in a tile: halves of 64 channels, 128-byte
-// rows, 16-byte chunks XORed with the row (TMA's 128-byte swizzle).
-__device__ __forceinline__ uint32_t tile_offset(int key, int chan) {
-  return (uint32_t)((chan >> 6) * (kTile * 128) + key * 128 +
-                    (((chan & 63) * 2) ^ ((key & 7) * 16)));
+// Byte offset of (row, column) in a matrix of ROWS rows of bf16 held as strips
+// of 64 columns: 128-byte rows, 16-byte chunks XORed with the row (TMA's
+// 128-byte swizzle, which ldmatrix reads without bank conflicts).
+template <int ROWS>
+__device__ __forceinline__ uint32_t strip_offset(int row, int col) {
+  return (uint32_t)((col >> 6) * (ROWS * 128) + row * 128 + (((col & 63) * 2) ^ ((row & 7) * 16)));
 }
 
-// What a block works on.
-struct Work {
+// --------------------------------------------------------------- scheduling
+// A unit is one row tile of one KV head of one sequence; it costs a tile per
+// 128 keys.  Blocks are persistent and share the tiles of all units evenly:
+// block c takes tiles c*per .. (c+1)*per-1 of the list (sequence, unit, key
+// tile), so ragged lengths leave no block idle and the loader streams across
+// unit borders.  The first and the last unit of a block may be parts; parts go
+// to slots of the workspace (2c for the block's first piece, 2c+1 for a later
+// one) and the block in which a split unit begins describes it to the merge.
+struct Piece {
   SeqView seq;
-  int head;         // KV head
-  int row0, rows;   // rows row0 .. row0+rows-1 of the sequence's count * group
-  int prefix;       // cached tokens before the new ones
-  int keys;         // keys 0 .. keys-1 (dense) or list slots * page size (blocks)
-  int pos;          // blocks: the token's position
+  int head;        // KV head
+  int row0, rows;  // rows row0 .. row0+rows-1 of the sequence's count * group
+  int prefix;      // cached tokens before the new ones
+  int keys;        // keys of the unit: positions (dense), list slots * page size
+  int pos;         // block lists: the token's position
   const int32_t *list;
+  int t0, t1;      // key tiles of this piece
+  bool first, last;  // it holds the unit's first / last tile
+  int unit_at;       // list index of the unit's first tile
 };
+
+struct MergeJob {
+  int slot0, parts;  // parts: blocks that the unit is split over, 0: none begins here
+  int first_token, row0, rows, head;
+  int pad[2];
+};
+
+// Units of a sequence and tiles of each; 0 units when the arrays contradict.
+template <int R>
+__device__ __forceinline__ void seq_units(const PagedAttn &a, int b, SeqView &seq, int &units,
+                                          int &tiles, bool report_it) {
+  units = tiles = 0;
+  if (!load_seq(a.pool, a.batch, b, seq, a.err, report_it) || seq.count == 0) return;
+  if (a.blocks) {
+    units = a.pool.heads * seq.count * ((a.group + R - 1) / R);
+    const int held = (seq.len + a.pool.ps - 1) >> a.pool.ps_log2;
+    const int nb = held < a.max_blocks ? held : a.max_blocks;
+    tiles = ((nb << a.pool.ps_log2) + kTile - 1) / kTile;
+  } else {
+    units = a.pool.heads * ((seq.count * a.group + R - 1) / R);
+    tiles = (seq.len + kTile - 1) / kTile;
+  }
+}
 
 template <int R>
-__device__ __forceinline__ bool find_work(const PagedAttn &a, Work &w, bool report_it) {
-  if (!load_seq(a.pool, a.batch, blockIdx.z, w.seq, a.err, report_it)) return false;
-  w.prefix = w.seq.len - w.seq.count;
-  const int heads = a.pool.heads;
-  w.head = blockIdx.y % heads;
-  const int tile = blockIdx.y / heads;
-  if (a.blocks) {
-    const int gt = (a.group + R - 1) / R;
-    const int token = tile / gt, g0 = (tile % gt) * R;
-    if (token >= w.seq.count) return false;
-    w.row0 = token * a.group + g0;
-    w.rows = a.group - g0 < R ? a.group - g0 : R;
-    w.pos = w.prefix + token;
-    w.list = a.blocks + ((int64_t)(w.seq.first + token) * heads + w.head) * a.max_blocks;
-    w.keys = a.max_blocks << a.pool.ps_log2;
-  } else {
-    const int total = w.seq.count * a.group;
-    w.row0 = tile * R;
-    if (w.row0 >= total) return false;
-    w.rows = total - w.row0 < R ? total - w.row0 : R;
-    w.pos = 0;
-    w.list = nullptr;
-    w.keys = w.seq.len;
-    if (!a.mask) {  // causal: up to the tile's last token
-      const int last = w.prefix + (w.row0 + w.rows - 1) / a.group + 1;
-      if (last < w.keys) w.keys = last;
+struct Cursor {
+  int b, unit, units, tiles, t;
+  int left, at;  // tiles left to the block; list index of the next tile
+  SeqView seq;
+
+  // The next piece; false at the end of the block's share.  Every lane of a
+  // warp takes the same steps.
+  __device__ __forceinline__ bool next(const PagedAttn &a, Piece &p) {
+    if (left <= 0) return false;
+    while (unit >= units) {
+      if (++b >= a.batch.seqs) return false;
+      seq_units<R>(a, b, seq, units, tiles, false);
+      unit = 0;
+      t = 0;
     }
+    const int n = tiles - t < left ? tiles - t : left;
+    p.seq = seq;
+    p.prefix = seq.len - seq.count;
+    p.t0 = t;
+    p.t1 = t + n;
+    p.first = t == 0;
+    p.last = t + n == tiles;
+    p.unit_at = at - t;
+    // Head-major: the row tiles that read the same keys run side by side.
+    int tile = 0;
+    p.head = unit;
+    if (units != a.pool.heads) {
+      const int per_head = units / a.pool.heads;
+      p.head = unit / per_head;
+      tile = unit - p.head * per_head;
+    }
+    if (a.blocks) {
+      const int gt = (a.group + R - 1) / R;
+      const int token = tile / gt, g0 = (tile % gt) * R;
+      p.row0 = token * a.group + g0;
+      p.rows = a.group - g0 < R ? a.group - g0 : R;
+      p.pos = p.prefix + token;
+      p.list = a.blocks + ((int64_t)(seq.first + token) * a.pool.heads + p.head) * a.max_blocks;
+      // Entries behind the last block hold -1: no tiles for them.
+      const int e0 = (int)(((int64_t)p.t0 * kTile) >> a.pool.ps_log2);
+      int64_t e1 = ((int64_t)p.t1 * kTile + a.pool.ps - 1) >> a.pool.ps_log2;
+      if (e1 > a.max_blocks) e1 = a.max_blocks;
+      int n_list = 0;
+      for (int e = e0; e < e1; e += 32) {
+        const int x = e + (int)(threadIdx.x & 31);
+        const uint32_t hit = __ballot_sync(0xffffffffu, x < e1 && p.list[x] >= 0);
+        if (hit) n_list = e + 32 - __clz(hit);
+      }
+      p.keys = n_list << a.pool.ps_log2;
+    } else {
+      const int total = seq.count * a.group;
+      p.row0 = tile * R;
+      p.rows = total - p.row0 < R ? total - p.row0 : R;
+      p.pos = 0;
+      p.list = nullptr;
+      p.keys = seq.len;
+      if (!a.mask) {  // causal: up to the row tile's last token
+        const int lim = p.prefix + (p.row0 + p.rows - 1) / a.group + 1;
+        if (lim < p.keys) p.keys = lim;
+      }
+    }
+    const int have = (p.keys + kTile - 1) / kTile;
+    if (p.t1 > have) p.t1 = have > p.t0 ? have : p.t0;
+    left -= n;
+    at += n;
+    t += n;
+    if (t == tiles) {
+      t = 0;
+      ++unit;
+    }
+    return true;
   }
-  return true;
-}
-
-// Output row of row r of the block's tile: (token, query head).
-__device__ __forceinline__ int64_t out_row(const PagedAttn &a, const Work &w, int r) {
-  const int x = w.row0 + r;
-  return ((int64_t)w.seq.first + x / a.group) * a.q_heads + w.head * a.group + x % a.group;
-}
-
-// Warps: 4 compute warps, RW of them over rows (16 each) and 4/RW over the
-// keys of a tile; warp 4 loads.
-template <int D, int RW, int STAGES>
-struct Cfg {
-  static constexpr int kRows = 16 * RW;
-  static constexpr int kKeyWarps = 4 / RW;
-  static constexpr int kTileBytes = kTile * D * 2;
-  static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kSmem = STAGES * kStageBytes + 1024;
 };
 
-template <int D, int RW, int STAGES>
-__global__ void __launch_bounds__(160, (D == 128 && STAGES > 3) ? 1 : 2)
-    paged_attn_kernel(const __grid_constant__ CUtensorMap kmap,
-                      const __grid_constant__ CUtensorMap vmap, const PagedAttn a) {
-  using C = Cfg<D, RW, STAGES>;
-  constexpr int R = C::kRows, KW = C::kKeyWarps;
-  constexpr int NK = kTile / KW;  // keys of a warp per tile
-  constexpr int NT = NK / 8;      // score fragments
-  constexpr int OT = D / 8;       // output fragments
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                              ~uintptr_t(1023));
-  __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ __align__(16) int limits[STAGES][4];  // written keys of each 16-key group
-  __shared__ int abort_flag, list_len;
-  __shared__ uint32_t odd_keys[2];   // keys of the tile that hold an infinity or NaN
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Work w;
-  if (!find_work<R>(a, w, threadIdx.x == 0)) return;
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 4);
-    }
-    fence_mbar_init();
-    abort_flag = 0;
-    list_len = 0;
+// The block's share of the tile list, in `share`.  Called by all THREADS
+// threads; ends with a barrier.  The host has checked that the list is shorter
+// than 2^31.
+template <int R, int THREADS>
+__device__ __forceinline__ void find_share(const PagedAttn &a, Cursor<R> &share, int *sh_per) {
+  __shared__ int warp_total[THREADS / 32];
+  const int n = a.batch.seqs;
+  const int chunk = n <= THREADS ? 1 : (n + THREADS - 1) / THREADS;
+  const int b0 = threadIdx.x * chunk, b1 = b0 + chunk < n ? b0 + chunk : n;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int sum = 0;
+  Cursor<R> c;
+  c.units = c.tiles = 0;
+  for (int b = b0; b < b1; ++b) {
+    seq_units<R>(a, b, c.seq, c.units, c.tiles, blockIdx.x == 0);
+    sum += c.units * c.tiles;
+  }
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) warp_total[warp] = scan;
+  if (threadIdx.x == 0) share.left = 0;
+  __syncthreads();
+  int total = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_total[w];
+    total += warp_total[w];
+  }
+  before += scan - sum;
+  const int per = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
+  const unsigned begin = (unsigned)per * blockIdx.x;
+  if (begin >= (unsigned)before && begin < (unsigned)before + sum) {
+    // One thread's sequences hold it.
+    int at = before, b = b0;
+    if (chunk > 1)
+      for (; b < b1; ++b) {
+        seq_units<R>(a, b, c.seq, c.units, c.tiles, false);
+        const int w = c.units * c.tiles;
+        if ((int)begin < at + w) break;
+        at += w;
+      }
+    c.b = b;
+    c.at = (int)begin;
+    c.left = total - (int)begin < per ? total - (int)begin : per;
+    const int off = (int)begin - at;
+    c.unit = (int)((unsigned)off / (unsigned)c.tiles);
+    c.t = off - c.unit * c.tiles;
+    share = c;
+    *sh_per = per;
   }
   __syncthreads();
-  if (w.list) {  // entries behind the last block hold -1: no tiles for them
-    int n = 0;
-    for (int i = threadIdx.x; i < a.max_blocks; i += blockDim.x)
-      if (w.list[i] >= 0) n = i + 1;
-    atomicMax(&list_len, n);
-    __syncthreads();
-    w.keys = list_len << a.pool.ps_log2;
-  }
-  const int tiles_all = (w.keys + kTile - 1) / kTile;
-  const int t0 = blockIdx.x * a.split_tiles;
-  const int t1 = t0 + a.split_tiles < tiles_all ? t0 + a.split_tiles : tiles_all;
+}
 
-  float o[OT][4];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < OT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+// Output row of row r of a piece: (token, query head).
+__device__ __forceinline__ int64_t out_row(const PagedAttn &a, int first_token, int head, int x) {
+  return ((int64_t)first_token + x / a.group) * a.q_heads + head * a.group + x % a.group;
+}
 
-  if (warp == 4) {
-    // ------------------------------------------------------------- loader
-    // Lane = (page of the tile, channel half, K or V): up to 16 boxes.
-    const int per = a.pool.ps >= kTile ? 1 : kTile >> a.pool.ps_log2;  // pages of a tile
-    const int box_rows = a.pool.ps < kTile ? a.pool.ps : kTile;
-    const int boxes = per * (D / 64) * 2;
-    const int c = lane % per, half = (lane / per) % (D / 64), is_v = lane / (per * (D / 64));
-    int page_next = 0, block_next = 0;
-    auto lookup = [&](int t) {  // block and page of this lane's box of tile t
-      const int key0 = t * kTile + c * box_rows;
-      int b = key0 >> a.pool.ps_log2;
-      page_next = -1;
-      block_next = -1;
-      if (lane >= boxes || key0 >= w.keys) return;
-      if (w.list) {
-        const int e = b;
-        b = w.list[e];
-        if (b < 0 || b > (w.pos >> a.pool.ps_log2) || (e > 0 && b <= w.list[e - 1])) return;
+__device__ __forceinline__ void store_out(const PagedAttn &a, int64_t at, float x, float y) {
+  if (a.out_f32)
+    *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at) = make_float2(x, y);
+  else
+    *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + at) = pack_bf16(x, y);
+}
+
+// Up to 32 rows: warp products on the whole block.  8 compute warps work on
+// one tile of 128 keys together:
+//   scores   warp w takes keys 16w .. 16w+15 for all rows,
+//   maximum  a row's maximum over the warps meets in shared memory,
+//   weights  each warp writes its 16 columns of P (bf16),
+//   values   warp w takes columns w*D/8 .. of the output over all 128 keys,
+// so an output lives in one place (D/8 columns a warp: 8 or 4 registers a row
+// tile), K, V and P are read from shared memory by whole tiles, and there is
+// nothing to join over the warps at the end but l.  A ninth warp loads.  One
+// block an SM with a ring of 192 KB, which covers HBM's latency several times.
+template <int D, int MT>
+struct Cfg {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kPBytes = kRows * kTile * 2;
+  static constexpr int kSmem = kStages * kStageBytes + kQBytes + kPBytes + 1024;
+  static constexpr int kThreads = 288;
+};
+
+// Producer warp of both attention kernels: streams the block's tiles into the
+// ring.  Lane = (page of the tile, channel strip, K or V): up to 32 boxes of 64
+// channels x one page.  Pages are looked up 32 at a time, a lane each, one
+// batch ahead of the loads.
+template <int D, int R, int STAGES>
+__device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
+                                          const CUtensorMap *kmap, const CUtensorMap *vmap,
+                                          uint8_t *ring, uint64_t *full, uint64_t *empty,
+                                          int (*limits)[8], int *abort_flag) {
+  constexpr int kTileBytes = kTile * D * 2;
+  const int lane = threadIdx.x & 31;
+  const int box_rows = a.pool.ps, npg = kTile >> a.pool.ps_log2;  // pages of a tile
+  const int boxes = npg * (D / 64) * 2;
+  const int c = lane & (npg - 1), strip = (lane / npg) % (D / 64), is_v = lane / (npg * (D / 64));
+  Piece p;
+  int i = 0;
+  while (cur.next(a, p)) {
+    const int last = (p.keys - 1) >> a.pool.ps_log2;  // last block or list entry
+    int page_ahead, block_ahead;
+    auto lookup = [&](int e) {  // block e + lane of the unit
+      e += lane;
+      int b = e <= last ? e : -1;
+      if (p.list && b >= 0) {
+        b = p.list[e];
+        if (b > (p.pos >> a.pool.ps_log2) || (e > 0 && b <= p.list[e - 1])) b = -1;
       }
-      block_next = b;
-      const int page = w.seq.table[b];
-      if (page_ok(a.pool, page)) page_next = page;
-      else report(a.err, NK_PAGE_OUT_OF_RANGE);
+      block_ahead = b;
+      page_ahead = b >= 0 ? p.seq.table[b] : -1;
     };
-    if (t0 < t1) lookup(t0);
-    for (int t = t0, i = 0; t < t1; ++t, ++i) {
+    int base = p.t0 * npg;  // block of lane 0; a tile's blocks lie in one batch
+    int page_now = 0, block_now = 0;
+    lookup(base);
+    base -= 32;
+    for (int t = p.t0; t < p.t1; ++t, ++i) {
       const int s = i % STAGES;
-      const int page = page_next, block = block_next;
-      if (t + 1 < t1) lookup(t + 1);  // in flight while this tile waits
-      if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, &abort_flag)) break;
-      const bool load = page >= 0;
-      const int within = a.pool.ps > kTile ? (t * kTile) & (a.pool.ps - 1) : 0;
-      if (lane < per && half == 0 && is_v == 0) {
+      const int e = t * npg + c;
+      if (t * npg - base >= 32) {  // the same for all lanes
+        base += 32;
+        page_now = page_ahead;
+        block_now = block_ahead;
+        if (base + 32 <= last) lookup(base + 32);
+      }
+      int page = __shfl_sync(0xffffffffu, page_now, (e - base) & 31);
+      const int block = __shfl_sync(0xffffffffu, block_now, (e - base) & 31);
+      const bool room = i < STAGES || mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, room)) return;  // the lanes leave together
+      if (block >= 0 && !page_ok(a.pool, page)) {
+        report(a.err, NK_PAGE_OUT_OF_RANGE);
+        page = -1;
+      }
+      const bool have = block >= 0 && page >= 0;
+      const bool load = have && lane < boxes;
+      if (lane < npg) {
         // Keys of the box that the rows may see: up to the last position.
         int n = 0;
-        if (load) {
-          n = w.list ? w.pos + 1 - ((block << a.pool.ps_log2) + within)
-                     : w.keys - (t * kTile + c * box_rows);
+        if (have) {
+          n = p.list ? p.pos + 1 - (block << a.pool.ps_log2) : p.keys - (e << a.pool.ps_log2);
           n = n < 0 ? 0 : (n > box_rows ? box_rows : n);
         }
         for (int g = 0; g < box_rows / 16; ++g)
-          limits[s][c * (box_rows / 16) + g] = n - 16 * g < 0 ? 0 : (n - 16 * g > 16 ? 16 : n - 16 * g);
+          limits[s][c * (box_rows / 16) + g] =
+              n - 16 * g < 0 ? 0 : (n - 16 * g > 16 ? 16 : n - 16 * g);
       }
       const uint32_t mine = __ballot_sync(0xffffffffu, load);
-      __syncwarp();
       if (lane == 0)
         mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(mine) * (uint32_t)box_rows * 128u);
       __syncwarp();
       if (load) {
-        uint8_t *dst = smem + s * C::kStageBytes + is_v * C::kTileBytes + half * (kTile * 128) +
+        uint8_t *dst = ring + s * 2 * kTileBytes + is_v * kTileBytes + strip * (kTile * 128) +
                        c * box_rows * 128;
-        const int64_t row = a.layer_row +
-                            (((int64_t)page * a.pool.heads + w.head) << a.pool.ps_log2) + within;
-        tma_load_2d(dst, is_v ? &vmap : &kmap, &full[s], half * 64, (int)row);
-      }
-    }
-    // The copies in flight land before the block's memory is given up.
-    const int issued = t1 - t0;
-    if (abort_flag && issued > 0) {
-      for (int s = 0; s < STAGES; ++s)
-        for (int ph = 0; ph < 2; ++ph) {
-          const uint64_t start = nk_globaltimer();
-          while (!mbar_try_wait(&full[s], ph) && nk_globaltimer() - start < 1000000ull) {
-          }
-        }
-    }
-  } else {
-    // ------------------------------------------------------------ compute
-    const int rw = warp % RW, kw = warp / RW;
-    const int quad = lane >> 2, qc = (lane & 3) * 2;
-    // Rows of this lane: quad and quad + 8 of the warp's 16.
-    uint32_t qf[D / 16][4];
-    int pos_row[2];       // causal: last position the row sees
-    uint64_t tree[2];
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int r = rw * 16 + quad + hh * 8;
-      const bool live = r < w.rows;
-      const int x = w.row0 + r;
-      const uint16_t *qr =
-          a.q + ((int64_t)w.seq.first + x / a.group) * a.ld_q +
-          ((int64_t)w.head * a.group + x % a.group) * D;
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][hh] = live ? *reinterpret_cast<const uint32_t *>(qr + k * 16 + qc) : 0u;
-        qf[k][hh + 2] = live ? *reinterpret_cast<const uint32_t *>(qr + k * 16 + 8 + qc) : 0u;
-      }
-      pos_row[hh] = w.prefix + x / a.group;
-      tree[hh] = a.mask && live ? a.mask[w.seq.first + x / a.group] : 0;
-    }
-    // Positions from here on are not seen by every row of the tile.
-    const int all_see = w.list ? 0x7fffffff
-                               : (a.mask ? w.prefix : w.prefix + w.row0 / a.group + 1);
-    auto allowed = [&](int hh, int p) {  // p < keys
-      if (a.mask) return p < w.prefix || ((tree[hh] >> (p - w.prefix)) & 1) != 0;
-      return p <= pos_row[hh];
-    };
-
-    for (int t = t0, i = 0; t < t1; ++t, ++i) {
-      const int s = i % STAGES;
-      if (!mbar_wait(&full[s], (i / STAGES) & 1, &abort_flag)) break;
-      uint8_t *kt = smem + s * C::kStageBytes, *vt = kt + C::kTileBytes;
-      const int4 lim = *reinterpret_cast<const int4 *>(limits[s]);
-      const bool tail = (lim.x + lim.y + lim.z + lim.w) < kTile;
-      const bool partial = (t + 1) * kTile > all_see && !w.list;
-      uint64_t odd = 0;
-      if (tail || partial) {
-        // Values that a row may not see are multiplied by a weight of 0, so
-        // what lies behind the last key becomes 0, and keys that only some
-        // rows see are searched for infinities and NaN (0 * inf is NaN).
-        if (threadIdx.x < 2) odd_keys[threadIdx.x] = 0;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int key = threadIdx.x >> 1, part = threadIdx.x & 1;  // half of the key's channels
-        const int g = key >> 4;
-        const int lg = g == 0 ? lim.x : (g == 1 ? lim.y : (g == 2 ? lim.z : lim.w));
-        const bool dead = (key & 15) >= lg;
-        const bool some = partial && !dead && t * kTile + key >= all_see;
-        bool found = false;
-        if (dead || some) {
-#pragma unroll
-          for (int ch = 0; ch < D / 16; ++ch) {
-            uint4 *p = reinterpret_cast<uint4 *>(vt + tile_offset(key, part * (D / 2) + ch * 8));
-            if (dead) {
-              *p = make_uint4(0, 0, 0, 0);
-            } else {
-              const uint4 x = *p;
-              const uint32_t word[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                found |= (word[j] & 0x7f80u) == 0x7f80u ||
-                         (word[j] & 0x7f800000u) == 0x7f800000u;
-            }
-          }
-        }
-        if (found) atomicOr(&odd_keys[key >> 5], 1u << (key & 31));
-        if (dead) fence_proxy_async_smem();  // before the stage is loaded again
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        odd = (uint64_t)odd_keys[1] << 32 | odd_keys[0];
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // read by all before the next tile's reset
-      }
-
-      // Scores of the warp's NK keys.
-      float sc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sc[n][j] = 0.0f;
-      const uint32_t kb = smem_u32(kt), vb = smem_u32(vt);
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-#pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-          uint32_t b[4];
-          const int mtx = lane >> 3;
-          ldsm4(b, kb + tile_offset(kw * NK + n * 8 + (mtx >> 1) * 8 + (lane & 7),
-                                    k * 16 + (mtx & 1) * 8));
-          mma16816(sc[n], qf[k], b[0], b[1]);
-          mma16816(sc[n + 1], qf[k], b[2], b[3]);
-        }
-      }
-      if (tail || partial) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = kw * NK + n * 8 + qc + (j & 1);
-            const int g = key >> 4;
-            const int lg = g == 0 ? lim.x : (g == 1 ? lim.y : (g == 2 ? lim.z : lim.w));
-            bool ok = (key & 15) < lg;
-            if (ok && partial) ok = allowed(j >> 1, t * kTile + key);
-            if (!ok) sc[n][j] = -INFINITY;
-          }
-      }
-      // Running maximum and sum, two rows a lane, four lanes a row.
-      float corr[2], mu[2];
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * hh], sc[n][2 * hh + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[hh], mx * a.scale_log2);
-        // No key so far: any finite shift will do, and keeps -inf - -inf out.
-        mu[hh] = mn == -INFINITY ? 0.0f : mn;
-        corr[hh] = exp2_approx(m[hh] - mu[hh]);
-        m[hh] = mn;
-        l[hh] *= corr[hh];
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = exp2_approx(sc[n][j] * a.scale_log2 - mu[j >> 1]);
-          sc[n][j] = p;
-          l[j >> 1] += p;
-        }
-#pragma unroll
-      for (int n = 0; n < OT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[n][j] *= corr[j >> 1];
-
-      if (odd) {
-        // Rare: an infinity or NaN in a key that some rows see.  Its terms are
-        // added by hand for the rows that see it, then its values become 0.
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int key = kw * NK + n * 8 + e;
-            if (!((odd >> key) & 1)) continue;
-            const int src = (lane & ~3) | (e >> 1);
-            const float p0 = __shfl_sync(0xffffffffu, sc[n][e & 1], src);
-            const float p1 = __shfl_sync(0xffffffffu, sc[n][2 + (e & 1)], src);
-            const int p = t * kTile + key;
-            const bool see0 = allowed(0, p), see1 = allowed(1, p);
-#pragma unroll
-            for (int f = 0; f < OT; ++f)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float v = __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
-                    vt + tile_offset(key, f * 8 + qc + j)));
-                if (see0) o[f][j] += p0 * v;
-                if (see1) o[f][2 + j] += p1 * v;
-              }
-          }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int key = threadIdx.x >> 1, part = threadIdx.x & 1;
-        if ((odd >> key) & 1) {
-#pragma unroll
-          for (int ch = 0; ch < D / 16; ++ch)
-            *reinterpret_cast<uint4 *>(vt + tile_offset(key, part * (D / 2) + ch * 8)) =
-                make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
-
-      // O += P V
-#pragma unroll
-      for (int kk = 0; kk < NK / 16; ++kk) {
-        const uint32_t pa[4] = {pack_bf16(sc[2 * kk][0], sc[2 * kk][1]),
-                                pack_bf16(sc[2 * kk][2], sc[2 * kk][3]),
-                                pack_bf16(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
-                                pack_bf16(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
-#pragma unroll
-        for (int n = 0; n < OT; n += 2) {
-          uint32_t b[4];
-          const int mtx = lane >> 3;
-          ldsm4_t(b, vb + tile_offset(kw * NK + kk * 16 + (mtx & 1) * 8 + (lane & 7),
-                                      n * 8 + (mtx >> 1) * 8));
-          mma16816(o[n], pa, b[0], b[1]);
-          mma16816(o[n + 1], pa, b[2], b[3]);
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-    }
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 1);
-      l[hh] += __shfl_xor_sync(0xffffffffu, l[hh], 2);
-    }
-  }
-  __syncthreads();  // every tile is read: the ring is free
-  if (abort_flag) {
-    if (threadIdx.x == 0) report(a.err, NK_TIMEOUT);
-    return;
-  }
-
-  if (KW > 1) {
-    // Join the key warps of each row group through shared memory, in order.
-    const int rw = warp % RW, kw = warp / RW;
-    float *buf = reinterpret_cast<float *>(smem);  // [KW-1][RW][32 lanes][OT*4+4]
-    constexpr int W = OT * 4 + 4;
-    if (warp < 4 && kw > 0) {
-      float *p = buf + (((kw - 1) * RW + rw) * W) * 32 + lane;
-#pragma unroll
-      for (int n = 0; n < OT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[(n * 4 + j) * 32] = o[n][j];
-      p[(OT * 4) * 32] = m[0];
-      p[(OT * 4 + 1) * 32] = m[1];
-      p[(OT * 4 + 2) * 32] = l[0];
-      p[(OT * 4 + 3) * 32] = l[1];
-    }
-    __syncthreads();
-    if (warp < 4 && kw == 0) {
-      for (int x = 1; x < KW; ++x) {
-        const float *p = buf + (((x - 1) * RW + rw) * W) * 32 + lane;
-        float ca[2], cb[2];
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const float mo = p[(OT * 4 + hh) * 32];
-          const float mn = fmaxf(m[hh], mo);
-          const float mu = mn == -INFINITY ? 0.0f : mn;
-          ca[hh] = exp2_approx(m[hh] - mu);
-          cb[hh] = exp2_approx(mo - mu);
-          m[hh] = mn;
-          l[hh] = l[hh] * ca[hh] + p[(OT * 4 + 2 + hh) * 32] * cb[hh];
-        }
-#pragma unroll
-        for (int n = 0; n < OT; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[n][j] = o[n][j] * ca[j >> 1] + p[(n * 4 + j) * 32] * cb[j >> 1];
-      }
-    }
-  }
-  if (warp < RW) {
-    const int quad = lane >> 2, qc = (lane & 3) * 2;
-#pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const int r = warp * 16 + quad + hh * 8;
-      if (r >= w.rows) continue;
-      const int64_t row = out_row(a, w, r);
-      if (a.splits > 1) {
-        const int64_t at = (int64_t)blockIdx.x * a.batch.tokens * a.q_heads + row;
-        if ((lane & 3) == 0) a.part_ml[at] = make_float2(m[hh], l[hh]);
-        if (t0 >= t1) continue;  // no key in the range: l = 0 says so
-        float *p = a.part_o + at * D + qc;
-#pragma unroll
-        for (int n = 0; n < OT; ++n)
-          *reinterpret_cast<float2 *>(p + n * 8) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
-      } else {
-        const float inv = l[hh] == 0.0f ? 0.0f : 1.0f / l[hh];
-#pragma unroll
-        for (int n = 0; n < OT; ++n) {
-          const float x = o[n][2 * hh] * inv, y = o[n][2 * hh + 1] * inv;
-          if (a.out_f32)
-            *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + row * D + n * 8 + qc) =
-                make_float2(x, y);
-          else
-            *reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(a.out) + row * D + n * 8 + qc) =
-                pack_bf16(x, y);
-        }
+        const int64_t row =
+            a.layer_row + (((int64_t)page * a.pool.heads + p.head) << a.pool.ps_log2);
+        tma_load_2d(dst, is_v ? vmap : kmap, &full[s], strip * 64, (int)row);
       }
     }
   }
 }
 
-// Joins the splits of a row in their order: warp per (token, query head).
-// Only rows that belong to a sequence are written.
-template <int D>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const PagedAttn a) {
-  const int s = blockIdx.y, lane = threadIdx.x & 31;
-  SeqView seq;
-  if (!load_seq(a.pool, a.batch, s, seq, a.err, false)) return;
-  const int x = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (x >= seq.count * a.q_heads) return;
-  const int64_t rows = a.batch.tokens * a.q_heads;
-  const int64_t row = (int64_t)seq.first * a.q_heads + x;
-  constexpr int V = D / 32;
-  float mx = -INFINITY;
-  for (int i = lane; i < a.splits; i += 32) mx = fmaxf(mx, a.part_ml[i * rows + row].x);
-  for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
-  const float mu = mx == -INFINITY ? 0.0f : mx;
-  float l = 0.0f, o[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) o[j] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
-    const float2 ml = a.part_ml[i * rows + row];
-    const float c = exp2_approx(ml.x - mu);
-    if (ml.y == 0.0f) continue;  // the split had no key
-    l += ml.y * c;
-    const float *p = a.part_o + (i * rows + row) * D + lane * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] += p[j] * c;
+// After an abort: the copies in flight land (or 1 ms passes) before the
+// block's memory is given up.
+__device__ __forceinline__ void drain_ring(uint64_t *full, int stages) {
+  for (int s = 0; s < stages; ++s)
+    for (int ph = 0; ph < 2; ++ph) {
+      const uint64_t start = nk_globaltimer();
+      while (!mbar_try_wait(&full[s], ph) && nk_globaltimer() - start < 1000000ull) {
+      }
+    }
+}
+
+// Barrier of the 256 compute threads that also ORs a flag.
+__device__ __forceinline__ bool compute_vote(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void compute_sync() {
+  asm volatile("bar.sync 1, 256;" ::: "memory");
+}
+
+template <int D, int MT>
+__global__ void __launch_bounds__(288, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap,
+                      const __grid_constant__ PagedAttn a) {
+  using C = Cfg<D, MT>;
+  constexpr int R = C::kRows, STAGES = C::kStages;
+  constexpr int COLS = D / 8, ON = COLS / 8;  // output columns of a warp
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~uintptr_t(1023));
+  uint8_t *qs = smem + STAGES * C::kStageBytes;
+  uint8_t *ps = qs + C::kQBytes;
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ __align__(16) int limits[STAGES][8];  // seen keys of each 16-key group
+  __shared__ __align__(16) float red[R][8];        // a value per row and warp
+  __shared__ uint32_t odd_keys[4];  // keys of the tile that hold an infinity or NaN
+  __shared__ int abort_flag;
+  __shared__ Cursor<R> share;
+  __shared__ int per;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 8);
+    }
+    fence_mbar_init();
+    abort_flag = 0;
+    if (a.jobs) a.jobs[blockIdx.x].parts = 0;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (threadIdx.x == 256) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
+  find_share<R, C::kThreads>(a, share, &per);
+  if (share.left <= 0) return;
+  Cursor<R> cur = share;
+
+  if (warp == 8) {
+    load_tiles<D, R, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits, &abort_flag);
+    if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
+  } else {
+    const int quad = lane >> 2, qc = (lane & 3) * 2;
+    Piece p;
+    int i = 0;      // tiles so far
+    int piece = 0;  // pieces so far
+    bool live = true;
+    while (live && cur.next(a, p)) {
+      // Queries to shared memory, 16 bytes a thread; rows of no token are 0.
+      // (The last reads of the old ones lie before the last tile's barriers.)
+      for (int x = threadIdx.x; x < R * D / 8; x += 256) {
+        const int r = x / (D / 8), c = (x % (D / 8)) * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < p.rows) {
+          const int y = p.row0 + r, tok = y / a.group;
+          v = *reinterpret_cast<const uint4 *>(
+              a.q + ((int64_t)p.seq.first + tok) * a.ld_q +
+              ((int64_t)p.head * a.group + (y - tok * a.group)) * D + c);
+        }
+        *reinterpret_cast<uint4 *>(qs + strip_offset<R>(r, c)) = v;
+      }
+      // Rows of this lane: quad and quad + 8 of each row tile.
+      int tok_row[MT][2];
+      float m[MT][2], l[MT][2], o[MT][ON][4];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int64_t at = row * D + lane * V + j;
-    if (a.out_f32)
-      static_cast<float *>(a.out)[at] = o[j] * inv;
-    else
-      static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(o[j] * inv);
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          tok_row[mt][hh] = (p.row0 + mt * 16 + quad + hh * 8) / a.group;
+          m[mt][hh] = -INFINITY;
+          l[mt][hh] = 0.0f;
+        }
+#pragma unroll
+        for (int n = 0; n < ON; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[mt][n][j] = 0.0f;
+      }
+      // Positions from here on are not seen by every row of the tile.
+      const int all_see =
+          p.list ? 0x7fffffff : (a.mask ? p.prefix : p.prefix + p.row0 / a.group + 1);
+      auto allowed = [&](int tok, int pos) {  // pos < keys
+        if (!a.mask) return pos <= p.prefix + tok;
+        return pos < p.prefix ||
+               (tok < p.seq.count && ((a.mask[p.seq.first + tok] >> (pos - p.prefix)) & 1) != 0);
+      };
+      compute_sync();  // the queries are there
+
+      for (int t = p.t0; t < p.t1; ++t, ++i) {
+        const int s = i % STAGES;
+        const bool got = mbar_wait(&full[s], (i / STAGES) & 1, &abort_flag);
+        if (compute_vote(!got)) {  // all warps leave together
+          live = false;
+          break;
+        }
+        uint8_t *kt = smem + s * C::kStageBytes, *vt = kt + C::kTileBytes;
+        const int4 la = *reinterpret_cast<const int4 *>(&limits[s][0]);
+        const int4 lb = *reinterpret_cast<const int4 *>(&limits[s][4]);
+        const bool tail = la.x + la.y + la.z + la.w + lb.x + lb.y + lb.z + lb.w < kTile;
+        const bool partial = !p.list && (t + 1) * kTile > all_see;
+        bool odd = false;
+        if (tail || partial) {
+          // Values that a row may not see are multiplied by a weight of 0, so
+          // what lies behind the last key becomes 0, and keys that only some
+          // rows see are searched for infinities and NaN (0 * inf is NaN).
+          if (threadIdx.x < 4) odd_keys[threadIdx.x] = 0;
+          compute_sync();
+          const int key = threadIdx.x >> 1, part = threadIdx.x & 1;  // half of its channels
+          const bool dead = (key & 15) >= limits[s][key >> 4];
+          const bool some = partial && !dead && t * kTile + key >= all_see;
+          bool found = false;
+          if (dead || some) {
+#pragma unroll 1
+            for (int ch = 0; ch < D / 16; ++ch) {
+              uint4 *x = reinterpret_cast<uint4 *>(
+                  vt + strip_offset<kTile>(key, part * (D / 2) + ch * 8));
+              if (dead) {
+                *x = make_uint4(0, 0, 0, 0);
+              } else {
+                const uint4 y = *x;
+                const uint32_t word[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  found |= (word[j] & 0x7f80u) == 0x7f80u ||
+                           (word[j] & 0x7f800000u) == 0x7f800000u;
+              }
+            }
+          }
+          if (found) atomicOr(&odd_keys[key >> 5], 1u << (key & 31));
+          if (dead) fence_proxy_async_smem();  // before the stage is loaded again
+          odd = compute_vote(found);
+        }
+
+        // Scores of the warp's 16 keys.
+        float sc[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[mt][n][j] = 0.0f;
+        const uint32_t kb = smem_u32(kt), vb = smem_u32(vt), qb = smem_u32(qs),
+                       pb = smem_u32(ps);
+        const int mtx = lane >> 3;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t b[4];
+          ldsm4(b, kb + strip_offset<kTile>(warp * 16 + (mtx >> 1) * 8 + (lane & 7),
+                                            k * 16 + (mtx & 1) * 8));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t q4[4];
+            ldsm4(q4, qb + strip_offset<R>(mt * 16 + (mtx & 1) * 8 + (lane & 7),
+                                           k * 16 + (mtx >> 1) * 8));
+            mma16816(sc[mt][0], q4, b[0], b[1]);
+            mma16816(sc[mt][1], q4, b[2], b[3]);
+          }
+        }
+        if (tail || partial) {
+          const int lim = limits[s][warp];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int key = n * 8 + qc + (j & 1);
+                bool ok = key < lim;
+                if (ok && partial) ok = allowed(tok_row[mt][j >> 1], t * kTile + warp * 16 + key);
+                if (!ok) sc[mt][n][j] = -INFINITY;
+              }
+        }
+        // A row's maximum over the warp's keys, then over the warps.
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            float mx = fmaxf(fmaxf(sc[mt][0][2 * hh], sc[mt][0][2 * hh + 1]),
+                             fmaxf(sc[mt][1][2 * hh], sc[mt][1][2 * hh + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if ((lane & 3) == 0) red[mt * 16 + quad + hh * 8][warp] = mx;
+          }
+        compute_sync();
+        float mu[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh) {
+            const float4 *x = reinterpret_cast<const float4 *>(red[mt * 16 + quad + hh * 8]);
+            const float4 x0 = x[0], x1 = x[1];
+            const float mx = fmaxf(fmaxf(fmaxf(x0.x, x0.y), fmaxf(x0.z, x0.w)),
+                                   fmaxf(fmaxf(x1.x, x1.y), fmaxf(x1.z, x1.w)));
+            const float mn = fmaxf(m[mt][hh], mx * a.scale_log2);
+            // No key so far: any finite shift will do, and keeps -inf - -inf out.
+            mu[mt][hh] = mn == -INFINITY ? 0.0f : mn;
+            const float corr = exp2_approx(m[mt][hh] - mu[mt][hh]);
+            m[mt][hh] = mn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const float w0 = exp2_approx(sc[mt][n][2 * hh] * a.scale_log2 - mu[mt][hh]);
+              const float w1 = exp2_approx(sc[mt][n][2 * hh + 1] * a.scale_log2 - mu[mt][hh]);
+              sum += w0 + w1;
+              *reinterpret_cast<uint32_t *>(
+                  ps + strip_offset<R>(mt * 16 + quad + hh * 8, warp * 16 + n * 8 + qc)) =
+                  pack_bf16(w0, w1);
+            }
+            l[mt][hh] = l[mt][hh] * corr + sum;
+#pragma unroll
+            for (int n = 0; n < ON; ++n) {
+              o[mt][n][2 * hh] *= corr;
+              o[mt][n][2 * hh + 1] *= corr;
+            }
+          }
+        if (odd) {
+          // Rare: an infinity or NaN in a key that some rows see.  Its terms
+          // are added by hand for the rows that see it (the weight is computed
+          // again: code that hardly ever runs should be small), then its
+          // values become 0.
+#pragma unroll 1
+          for (int key = 0; key < kTile; ++key) {
+            if (!((odd_keys[key >> 5] >> (key & 31)) & 1)) continue;
+            const int pos = t * kTile + key;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const int r = mt * 16 + quad + hh * 8;
+                if (r >= p.rows || !allowed(tok_row[mt][hh], pos)) continue;
+                float dot = 0.0f;
+#pragma unroll 1
+                for (int d = 0; d < D; ++d)
+                  dot += __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
+                             qs + strip_offset<R>(r, d))) *
+                         __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
+                             kt + strip_offset<kTile>(key, d)));
+                const float w = exp2_approx(dot * a.scale_log2 - mu[mt][hh]);
+#pragma unroll
+                for (int n = 0; n < ON; ++n)
+#pragma unroll
+                  for (int j = 0; j < 2; ++j)
+                    o[mt][n][2 * hh + j] +=
+                        w * __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
+                                vt + strip_offset<kTile>(key, warp * COLS + n * 8 + qc + j)));
+              }
+          }
+          compute_sync();
+          const int key = threadIdx.x >> 1, part = threadIdx.x & 1;
+          if ((odd_keys[key >> 5] >> (key & 31)) & 1) {
+#pragma unroll 1
+            for (int ch = 0; ch < D / 16; ++ch)
+              *reinterpret_cast<uint4 *>(
+                  vt + strip_offset<kTile>(key, part * (D / 2) + ch * 8)) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+        }
+        compute_sync();  // the weights are there
+
+        // O += P V for the warp's columns.
+        if (ON == 2) {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k) {
+            uint32_t b[4];
+            ldsm4_t(b, vb + strip_offset<kTile>(k * 16 + (mtx & 1) * 8 + (lane & 7),
+                                                warp * COLS + (mtx >> 1) * 8));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              uint32_t p4[4];
+              ldsm4(p4, pb + strip_offset<R>(mt * 16 + (mtx & 1) * 8 + (lane & 7),
+                                             k * 16 + (mtx >> 1) * 8));
+              mma16816(o[mt][0], p4, b[0], b[1]);
+              mma16816(o[mt][ON - 1], p4, b[2], b[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < kTile / 16; k += 2) {
+            uint32_t b[4];  // 32 keys x 8 columns
+            ldsm4_t(b, vb + strip_offset<kTile>(k * 16 + mtx * 8 + (lane & 7), warp * COLS));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                uint32_t p4[4];
+                ldsm4(p4, pb + strip_offset<R>(mt * 16 + (mtx & 1) * 8 + (lane & 7),
+                                               (k + u) * 16 + (mtx >> 1) * 8));
+                mma16816(o[mt][0], p4, b[2 * u], b[2 * u + 1]);
+              }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      if (!live) break;
+
+      // l over the quad's lanes, then over the warps, in their order.
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float x = l[mt][hh];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          if ((lane & 3) == 0) red[mt * 16 + quad + hh * 8][warp] = x;
+        }
+      compute_sync();
+      const int slot = 2 * (int)blockIdx.x + (piece > 0);
+      const bool whole = p.first && p.last;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int r = mt * 16 + quad + hh * 8;
+          if (r >= p.rows) continue;
+          float sum = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 8; ++w) sum += red[r][w];
+          if (whole) {
+            const int64_t at =
+                out_row(a, p.seq.first, p.head, p.row0 + r) * D + warp * COLS + qc;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int n = 0; n < ON; ++n)
+              store_out(a, at + n * 8, o[mt][n][2 * hh] * inv, o[mt][n][2 * hh + 1] * inv);
+          } else {
+            const int64_t at = (int64_t)slot * R + r;
+            if (warp == 0 && (lane & 3) == 0) a.part_ml[at] = make_float2(m[mt][hh], sum);
+#pragma unroll
+            for (int n = 0; n < ON; ++n)
+              *reinterpret_cast<float2 *>(a.part_o + at * D + warp * COLS + n * 8 + qc) =
+                  make_float2(o[mt][n][2 * hh], o[mt][n][2 * hh + 1]);
+          }
+        }
+      if (threadIdx.x == 0 && p.first && !p.last) {
+        MergeJob j{};
+        j.slot0 = slot;
+        j.parts = (p.unit_at + cur.tiles - 1) / per - (int)blockIdx.x + 1;
+        j.first_token = p.seq.first;
+        j.row0 = p.row0;
+        j.rows = p.rows;
+        j.head = p.head;
+        a.jobs[blockIdx.x] = j;
+      }
+      ++piece;
+      compute_sync();  // red is read before the next piece writes it
+    }
+  }
+  __syncthreads();
+  if (abort_flag && threadIdx.x == 0) report(a.err, NK_TIMEOUT);
+}
+
+// Joins the parts of the unit that begins in block blockIdx.x of the
+// attention, in their order: a warp per row, blockIdx.y over the rows.
+template <int D>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttn a, int R) {
+  // Launched while the attention runs: nothing is read before it has ended.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const MergeJob j = a.jobs[blockIdx.x];
+  const int lane = threadIdx.x & 31;
+  constexpr int V = D / 32;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); j.parts > 0 && r < j.rows;
+       r += gridDim.y * 4) {
+    // Part i > 0 is the first piece of block blockIdx.x + i.
+    auto row_of = [&](int i) {
+      return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : j.slot0) * R + r;
+    };
+    float mx = -INFINITY;
+    for (int i = lane; i < j.parts; i += 32) mx = fmaxf(mx, a.part_ml[row_of(i)].x);
+    for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
+    const float mu = mx == -INFINITY ? 0.0f : mx;
+    float l = 0.0f, o[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < j.parts; ++i) {
+      const float2 ml = a.part_ml[row_of(i)];
+      const float c = exp2_approx(ml.x - mu);
+      l += ml.y * c;
+      const float *p = a.part_o + row_of(i) * D + lane * V;
+#pragma unroll
+      for (int k = 0; k < V; k += 2) {
+        const float2 x = *reinterpret_cast<const float2 *>(p + k);
+        o[k] += x.x * c;
+        o[k + 1] += x.y * c;
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int64_t at = out_row(a, j.first_token, j.head, j.row0 + r) * D + lane * V;
+#pragma unroll
+    for (int k = 0; k < V; k += 2) store_out(a, at + k, o[k] * inv, o[k + 1] * inv);
   }
 }
 
 // ------------------------------------------------------------------- host
-// Row tile and key split of a call, from its bounds alone.
+// Row tile and blocks of a call, from its bounds alone.
 struct AttnPlan {
-  int row_warps;   // 16 * row_warps rows a block
-  int row_tiles;   // blocks over the rows of a sequence and head
-  int splits, split_tiles;
-  size_t bytes;
+  int row_tiles;  // 16 * row_tiles rows a unit
+  double tiles;   // the longest list
+  int blocks;
+  bool merge;     // a unit may be split over blocks
+  size_t o_bytes, ml_bytes, bytes;
 };
 
 static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
@@ -588,20 +810,21 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   AttnPlan p{};
   const int64_t group = a.q_heads / kv.kv_heads;
   const int64_t rows = a.blocks ? group : b.max_new * group;
-  p.row_warps = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
-  const int64_t r = 16 * p.row_warps;
-  p.row_tiles = (int)(a.blocks ? b.max_new * ceil_div(group, r) : ceil_div(rows, r));
-  const int64_t keys = a.blocks ? a.max_blocks * kv.page_size : b.max_kv;
-  const int64_t tiles = ceil_div(keys > 0 ? keys : 1, kTile);
-  const int64_t units = b.seqs * kv.kv_heads * p.row_tiles;
-  // Two blocks a SM; ragged lengths want a few blocks more to even out.
-  int64_t want = ceil_div(2 * 2 * 148, units > 0 ? units : 1);
-  int64_t per = ceil_div(tiles, want);
-  if (per < 2) per = 2;  // a range shorter than two tiles costs more to join than to read
-  p.split_tiles = (int)per;
-  p.splits = (int)ceil_div(tiles, per);
-  if (p.splits > 1)
-    p.bytes = (size_t)p.splits * b.tokens * a.q_heads * (kv.head_dim * 4 + 8);
+  p.row_tiles = rows <= 16 ? 1 : 2;
+  const int64_t r = 16 * p.row_tiles;
+  const int64_t units = a.blocks ? b.max_new * ceil_div(group, r) : ceil_div(rows, r);
+  int64_t keys = b.max_kv;
+  if (a.blocks && a.max_blocks < ceil_div(keys, kv.page_size)) keys = a.max_blocks * kv.page_size;
+  const int64_t tiles = ceil_div(ceil_div(keys, kv.page_size) * kv.page_size, kTile);
+  // One block an SM, or fewer when there are not as many tiles.
+  p.tiles = (double)b.seqs * kv.kv_heads * units * tiles;
+  p.blocks = p.tiles < num_sms() ? (p.tiles < 1 ? 1 : (int)p.tiles) : num_sms();
+  p.merge = tiles > 1;
+  if (p.merge) {
+    p.o_bytes = (size_t)2 * p.blocks * r * kv.head_dim * 4;
+    p.ml_bytes = (size_t)2 * p.blocks * r * 8;
+    p.bytes = p.o_bytes + p.ml_bytes + (size_t)p.blocks * sizeof(MergeJob);
+  }
   return p;
 }
 
@@ -631,13 +854,10 @@ static nk_status check_attention(const nk_kv_pages *kv, const nk_kv_batch *b,
     return fail(NK_UNSUPPORTED, "a tree holds at most 64 drafted tokens");
   if (a->blocks && (a->max_blocks <= 0 || a->max_blocks > (1 << 20)))
     return fail(NK_INVALID_PARAMS, "max_blocks must lie in 1 .. 2^20");
-  const int64_t group = a->q_heads / kv->kv_heads;
-  if (b->max_new * a->q_heads >= (1ll << 31) - 64 || b->tokens * a->q_heads >= (1ll << 40))
+  if (b->max_new * a->q_heads >= (1ll << 31) - 64)
     return fail(NK_UNSUPPORTED, "max_new * q_heads must be < 2^31 - 64");
-  const AttnPlan p = plan_attention(*kv, *b, *a);
-  if ((a->blocks ? b->max_new * ceil_div(group, 16 * p.row_warps) : (int64_t)p.row_tiles) *
-          kv->kv_heads > 65535)
-    return fail(NK_UNSUPPORTED, "too many query rows in one sequence: split the chunk");
+  if (plan_attention(*kv, *b, *a).tiles >= 2147000000.0)
+    return fail(NK_UNSUPPORTED, "too much work for one call: split the batch");
   return NK_OK;
 }
 
@@ -665,14 +885,28 @@ static nk_status page_map(const uint16_t *base, int64_t rows, int64_t d, int box
   return NK_OK;
 }
 
-template <int D, int RW, int STAGES>
+template <int D, int MT>
 static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
-                                  const PagedAttn &a, dim3 grid, cudaStream_t s) {
-  using C = Cfg<D, RW, STAGES>;
-  NK_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<D, RW, STAGES>,
+                                  const PagedAttn &a, const AttnPlan &p, cudaStream_t s) {
+  using C = Cfg<D, MT>;
+  NK_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<D, MT>,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
-  paged_attn_kernel<D, RW, STAGES><<<grid, 160, C::kSmem, s>>>(km, vm, a);
-  return check_launch("paged_attn_kernel");
+  paged_attn_kernel<D, MT><<<p.blocks, C::kThreads, C::kSmem, s>>>(km, vm, a);
+  nk_status st = check_launch("paged_attn_kernel");
+  if (st != NK_OK || !p.merge) return st;
+  // The merge is launched while the attention runs and waits on the device for
+  // its end, which hides the launch.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)p.blocks, 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_merge_kernel<D>, a, (int)C::kRows));
+  return ok();
 }
 
 }  // namespace nk
@@ -725,38 +959,26 @@ nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.scale_log2 = sc * 1.44269504088896340736f;
   a.out = args->out;
   a.out_f32 = args->out_dtype == NK_DTYPE_F32;
-  a.splits = p.splits;
-  a.split_tiles = p.split_tiles;
-  a.part_o = static_cast<float *>(workspace);
-  a.part_ml = reinterpret_cast<float2 *>(a.part_o + (int64_t)p.splits * batch->tokens *
-                                                        args->q_heads * kv->head_dim);
+  if (p.merge) {
+    uint8_t *w = static_cast<uint8_t *>(workspace);
+    a.part_o = reinterpret_cast<float *>(w);
+    a.part_ml = reinterpret_cast<float2 *>(w + p.o_bytes);
+    a.jobs = reinterpret_cast<MergeJob *>(w + p.o_bytes + p.ml_bytes);
+  }
   a.err = device_error_ptr();
   if (!a.err) return fail(NK_DEVICE_ERROR, "cannot resolve device error word");
   const int64_t rows = kv->layers * kv->pages * kv->kv_heads * kv->page_size;
-  const int box = kv->page_size < kTile ? (int)kv->page_size : kTile;
+  const int box = (int)kv->page_size;
   CUtensorMap km, vm;
   st = page_map(kv->k, rows, kv->head_dim, box, &km);
   if (st == NK_OK) st = page_map(kv->v, rows, kv->head_dim, box, &vm);
   if (st != NK_OK) return st;
   cudaStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.row_tiles * kv->kv_heads),
-                  (unsigned)batch->seqs);
-  if (kv->head_dim == 128) {
-    st = p.row_warps == 1   ? launch_attention<128, 1, 3>(km, vm, a, grid, s)
-         : p.row_warps == 2 ? launch_attention<128, 2, 3>(km, vm, a, grid, s)
-                            : launch_attention<128, 4, 3>(km, vm, a, grid, s);
-  } else {
-    st = p.row_warps == 1   ? launch_attention<64, 1, 6>(km, vm, a, grid, s)
-         : p.row_warps == 2 ? launch_attention<64, 2, 6>(km, vm, a, grid, s)
-                            : launch_attention<64, 4, 6>(km, vm, a, grid, s);
-  }
-  if (st != NK_OK || p.splits == 1) return st;
-  const dim3 mg((unsigned)ceil_div(batch->max_new * args->q_heads, 4), (unsigned)batch->seqs);
   if (kv->head_dim == 128)
-    paged_merge_kernel<128><<<mg, 128, 0, s>>>(a);
-  else
-    paged_merge_kernel<64><<<mg, 128, 0, s>>>(a);
-  return check_launch("paged_merge_kernel");
+    return p.row_tiles == 1 ? launch_attention<128, 1>(km, vm, a, p, s)
+                            : launch_attention<128, 2>(km, vm, a, p, s);
+  return p.row_tiles == 1 ? launch_attention<64, 1>(km, vm, a, p, s)
+                          : launch_attention<64, 2>(km, vm, a, p, s);
 }
 
 }  // extern "C"

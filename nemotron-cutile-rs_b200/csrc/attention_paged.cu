@@ -19,6 +19,8 @@
 // reads without bank conflicts.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+
 #include "gemm_tc.h"
 #include "paged.cuh"
 
@@ -889,10 +891,12 @@ template <int D, int MT>
 static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
                                   const PagedAttn &a, const AttnPlan &p, cudaStream_t s) {
   using C = Cfg<D, MT>;
-  NK_CUDA_TRY(cudaFuncSetAttribute(paged_attn_kernel<D, MT>,
-                                   cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  static std::atomic<uint64_t> prepared{0};  // a bit per device
+  nk_status st = allow_smem(reinterpret_cast<const void *>(paged_attn_kernel<D, MT>), C::kSmem,
+                            prepared);
+  if (st != NK_OK) return st;
   paged_attn_kernel<D, MT><<<p.blocks, C::kThreads, C::kSmem, s>>>(km, vm, a);
-  nk_status st = check_launch("paged_attn_kernel");
+  st = check_launch("paged_attn_kernel");
   if (st != NK_OK || !p.merge) return st;
   // The merge is launched while the attention runs and waits on the device for
   // its end, which hides the launch.

@@ -2,14 +2,21 @@
 // bound of the block's scores from the channel bounds of its keys, then the
 // largest top_k of them.
 //
-// The bound is sum_c q_c * (q_c >= 0 ? k_max_c : k_min_c), per query head;
-// the heads that share a KV head share a list, ranked by their largest bound.
-// Products of two bf16 values are exact in f64, and sums of head_dim of them
-// are exact or off by 2^-53 relative, so the ranking does not depend on the
-// order of the sum: a list is the same whatever split or layout computes it.
+// The score is sum_c q_c * (q_c >= 0 ? k_max_c : k_min_c), per query head; the
+// heads that share a KV head share a list, ranked by their largest score.  A
+// list must not depend on the order of a sum, so it is defined by 64-bit sums
+// (products of two bf16 values are exact in f64).  f64 arithmetic over every
+// block measured 42 us for 4 sequences of 131072 tokens, so the first pass is
+// f32 with a bound of its error: each block gets an interval that holds its
+// score, the intervals settle nearly every block, and only those that straddle
+// the border are summed again in 64 bits.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace nk {
+
+typedef unsigned long long u64;
 
 struct SelectArgs {
   PagePool pool;
@@ -20,21 +27,30 @@ struct SelectArgs {
   const uint16_t *k_min, *k_max;  // the layer's
   int top_k, sink, local;
   int64_t score_ld;
-  double *scores;  // [tokens, kv_heads, score_ld]
+  float2 *range;   // [tokens, kv_heads, score_ld]: the score lies in it
+  double *exact;   // the same shape: 64-bit scores of the blocks in doubt
   int32_t *blocks;
   int *err;
 };
 
-// Token t of the batch's buffers -> its sequence (start is ascending): -1 when
-// no sequence holds it.
+// Token t of the batch's buffers -> its sequence (start is ascending), -1 when
+// no sequence holds it.  A warp halves the range 32-fold a load; every lane
+// returns the result.
 __device__ __forceinline__ int sequence_of(const PageBatch &b, int64_t t) {
-  int lo = 0, hi = b.seqs;  // start[lo] <= t < start[hi]
-  if (t < b.start[0] || t >= b.start[b.seqs]) return -1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (b.start[mid] <= t) lo = mid; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = b.seqs + 1;  // the last start <= t lies in lo .. lo+n-1
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int at = lo + lane * step;
+    const bool le = lane * step < n && b.start[at] <= t;
+    const uint32_t hit = __ballot_sync(0xffffffffu, le);
+    if (!hit) return -1;
+    const int last = 31 - __clz(hit);
+    const int left = n - last * step;
+    lo += last * step;
+    n = left < step ? left : step;
   }
-  return lo;
+  return b.start[lo] <= t && lo < b.seqs ? lo : -1;
 }
 
 struct Query {
@@ -54,155 +70,453 @@ __device__ __forceinline__ bool find_query(const SelectArgs &a, int64_t token, Q
   return true;
 }
 
-// Block = (128 eligible blocks x, KV head y, token z): a thread per block, the
-// group's queries as f64 in shared memory.
+__device__ __forceinline__ float bf16_f32(uint16_t x) {
+  return __uint_as_float((uint32_t)x << 16);
+}
+
+// Two f32 FMAs in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<u64 *>(&d))
+      : "l"(*reinterpret_cast<const u64 *>(&a)), "l"(*reinterpret_cast<const u64 *>(&b)),
+        "l"(*reinterpret_cast<const u64 *>(&c)));
+  return d;
+}
+
+// Block = (64 eligible blocks x, KV head y, token z): a lane holds a block and a
+// warp a quarter of the channels of 32 blocks, so that a query value is one
+// broadcast read of shared memory for 32 blocks; HEADS query heads at a time.
+//   s_g = sum_c max(q, 0) * k_max + min(q, 0) * k_min   (f32 FMAs)
+//   A   = sum_c max_g|q| * max(|k_min|, |k_max|)        >= sum of any head's |terms|
+// A lane adds D/4 terms (the other product of a channel is 0) and the quarters
+// are joined in two more steps, each off by at most 2^-24 of a partial sum,
+// itself at most A: |s_g - score| <= (D/4 + 2) * 2^-24 A.  The interval takes
+// (D/4 + 6) * 2^-24 A: one more covers the roundings of its own ends, another
+// the relative error of A ((D/4 + 3) * 2^-24, times D/4 + 2), and 1e-38 results
+// that underflow.  Where a sum is not finite (0 * inf is NaN here, not in the
+// definition) the interval is everything.
+// The loop is not unrolled beyond a 16-byte word of bounds: a warp runs through
+// it a few times only, and straight-line code of this kernel spent its time on
+// instruction fetch.
 template <int D>
-__global__ void __launch_bounds__(128) block_scores_kernel(const SelectArgs a) {
-  extern __shared__ double qd[];  // [group][D]
+struct ScoreShared {
+  static constexpr int kRow = D * 2 + 16;  // bytes of a block's bounds: 16 apart in banks
+  static constexpr int kBounds = 2 * 64 * kRow;
+  static constexpr int kSums = 4 * 64 * 4;  // a pass's head: [quarter][block] f32
+  static size_t bytes(int64_t wide) {
+    return (size_t)kBounds + (size_t)wide * D * 8 + D * 4 + (size_t)wide * kSums + kSums;
+  }
+};
+
+template <int D, int HEADS>
+__global__ void __launch_bounds__(256) block_scores_kernel(const SelectArgs a) {
+  using S = ScoreShared<D>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int wide = (a.group + HEADS - 1) / HEADS * HEADS;
+  float4 *qs = reinterpret_cast<float4 *>(smem + S::kBounds);  // [D][wide/2]: q+ of two heads, q- of both
+  float *qm = reinterpret_cast<float *>(qs + D * wide / 2);    // [D]: max_g |q|
+  float *sums = qm + D;                                        // [wide + 1][quarter][block]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Query x;
   if (!find_query(a, blockIdx.z, x, threadIdx.x == 0)) return;
   if (x.blocks <= a.top_k) return;  // every block is taken
-  const int first = blockIdx.x * 128;
+  const int first = blockIdx.x * 64;
   // the forced blocks need no score
-  if (first >= x.blocks - a.local || first + 128 <= a.sink) return;
+  if (first >= x.blocks - a.local || first + 64 <= a.sink) return;
   const int h = blockIdx.y;
+  // Bounds: a warp copies 8 blocks' rows (whole 128- or 256-byte rows a load).
+  {
+    constexpr int C = D / 8;  // 16-byte words of a row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int mine = first + warp * 8 + (lane & 7);
+    int page = -1;
+    if (mine >= a.sink && mine < x.blocks - a.local) {
+      page = x.seq.table[mine];
+      if (!page_ok(a.pool, page)) {
+        if (lane < 8) report(a.err, NK_PAGE_OUT_OF_RANGE);
+        page = -1;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; r += 32 / C) {
+      const int row = r + lane / C;
+      const int pg = __shfl_sync(0xffffffffu, page, row);
+      const int64_t at = ((int64_t)(pg < 0 ? 0 : pg) * a.pool.heads + h) * C + lane % C;
+      uint8_t *to = smem + (warp * 8 + row) * S::kRow + (lane % C) * 16;
+      *reinterpret_cast<uint4 *>(to) = reinterpret_cast<const uint4 *>(a.k_min)[at];
+      *reinterpret_cast<uint4 *>(to + 64 * S::kRow) = reinterpret_cast<const uint4 *>(a.k_max)[at];
+    }
+  }
   const uint16_t *q = a.q + x.token * a.ld_q + (int64_t)h * a.group * D;
-  for (int i = threadIdx.x; i < a.group * D; i += 128)
-    qd[i] = (double)__uint_as_float((uint32_t)q[i] << 16);
+  bool odd = false;  // a NaN query is dropped by fmaxf and fminf
+#pragma unroll 4
+  for (int i = threadIdx.x; i < wide * D; i += 256) {
+    const int c = i / wide, g = i - c * wide;
+    const float v = g < a.group ? bf16_f32(q[g * D + c]) : 0.0f;
+    odd |= v != v;
+    float *to = reinterpret_cast<float *>(qs + c * (wide / 2) + g / 2) + (g & 1);
+    to[0] = fmaxf(v, 0.0f);
+    to[2] = fminf(v, 0.0f);
+  }
+  odd = __syncthreads_or(odd);
+  for (int c = threadIdx.x; c < D; c += 256) {
+    const float4 *row = qs + c * (wide / 2);
+    float mx = 0.0f;
+#pragma unroll 4
+    for (int g = 0; g < wide / 2; ++g)
+      mx = fmaxf(mx, fmaxf(fmaxf(row[g].x, row[g].y), fmaxf(-row[g].z, -row[g].w)));
+    qm[c] = mx;
+  }
   __syncthreads();
-  const int j = first + threadIdx.x;
-  if (j < a.sink || j >= x.blocks - a.local) return;
+  const int part = (threadIdx.x >> 5) & 3;
+  const int b = (threadIdx.x & 31) + (threadIdx.x >> 7) * 32;  // block of this lane
+  const uint8_t *low_row = smem + b * S::kRow + part * (D / 2);
+  const uint8_t *high_row = low_row + 64 * S::kRow;
+  float mag = 0.0f;
+#pragma unroll 1
+  for (int g0 = 0; g0 < wide; g0 += HEADS) {
+    float2 acc[HEADS / 2];
+#pragma unroll
+    for (int g = 0; g < HEADS / 2; ++g) acc[g] = make_float2(0.0f, 0.0f);
+    const float4 *qc = qs + part * (D / 4) * (wide / 2) + g0 / 2;
+    const float *qa = qm + part * (D / 4);
+#pragma unroll 1
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 lo = *reinterpret_cast<const uint4 *>(low_row + i * 16);
+      const uint4 hi = *reinterpret_cast<const uint4 *>(high_row + i * 16);
+      const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w};
+      const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e, qc += wide / 2) {
+        const float l = __uint_as_float((e & 1) ? lw[e >> 1] & 0xffff0000u : lw[e >> 1] << 16);
+        const float u = __uint_as_float((e & 1) ? hw[e >> 1] & 0xffff0000u : hw[e >> 1] << 16);
+#pragma unroll
+        for (int g = 0; g < HEADS / 2; ++g) {
+          const float4 v = qc[g];
+          acc[g] = fma2(make_float2(v.x, v.y), make_float2(u, u), acc[g]);
+          acc[g] = fma2(make_float2(v.z, v.w), make_float2(l, l), acc[g]);
+        }
+        if (g0 == 0) mag = fmaf(qa[i * 8 + e], fmaxf(fabsf(l), fabsf(u)), mag);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < HEADS / 2; ++g) {
+      sums[((g0 + 2 * g) * 4 + part) * 64 + b] = acc[g].x;
+      sums[((g0 + 2 * g + 1) * 4 + part) * 64 + b] = acc[g].y;
+    }
+  }
+  sums[(wide * 4 + part) * 64 + b] = mag;
+  __syncthreads();
+  // Join the quarters; 4 threads a block take its heads in turn.
+  const int jb = threadIdx.x >> 2, j = first + jb;
+  auto joined = [&](int g) {
+    const float *v = sums + g * 256 + jb;
+    return (v[0] + v[64]) + (v[128] + v[192]);
+  };
+  float best = -INFINITY;
+  for (int g = threadIdx.x & 3; g < a.group; g += 4) {
+    const float v = joined(g);
+    odd |= !(fabsf(v) < INFINITY);
+    best = fmaxf(best, v);
+  }
+  best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+  best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+  const uint32_t odds = __ballot_sync(0xffffffffu, odd);
+  if ((threadIdx.x & 3) == 0 && j >= a.sink && j < x.blocks - a.local) {
+    const float e = fmaf(joined(wide), (D / 4 + 6) * 0x1p-24f, 1e-38f);
+    float2 r = make_float2(best - e, best + e);
+    if (((odds >> (threadIdx.x & 31)) & 15) || !(e < INFINITY)) r = make_float2(-INFINITY, INFINITY);
+    if (!page_ok(a.pool, x.seq.table[j])) r = make_float2(-INFINITY, -INFINITY);
+    a.range[(x.token * a.pool.heads + h) * a.score_ld + j] = r;
+  }
+}
+
+// The score by its definition, by one warp (every lane returns it): a lane sums
+// D / 32 neighbouring channels.
+template <int D>
+__device__ __forceinline__ double exact_score(const SelectArgs &a, const Query &x, int h, int j) {
+  constexpr int V = D / 32;
+  struct alignas(2 * V) Chunk { uint16_t v[V]; };
+  const int c0 = (threadIdx.x & 31) * V;
   const int page = x.seq.table[j];
   double best = -INFINITY;
-  if (page_ok(a.pool, page)) {
-    const int64_t at = ((int64_t)page * a.pool.heads + h) * D;
-    constexpr int HEADS = 8;  // sums in flight
-    for (int g0 = 0; g0 < a.group; g0 += HEADS) {
-      double acc[HEADS];
+  if (!page_ok(a.pool, page)) return best;
+  const int64_t at = ((int64_t)page * a.pool.heads + h) * D + c0;
+  const Chunk lo = *reinterpret_cast<const Chunk *>(a.k_min + at);
+  const Chunk hi = *reinterpret_cast<const Chunk *>(a.k_max + at);
+  const uint16_t *q = a.q + x.token * a.ld_q + (int64_t)h * a.group * D + c0;
+#pragma unroll 4
+  for (int g = 0; g < a.group; ++g) {
+    double s = 0.0;
 #pragma unroll
-      for (int g = 0; g < HEADS; ++g) acc[g] = 0.0;
-      for (int c = 0; c < D; c += 8) {
-        const uint4 lo4 = *reinterpret_cast<const uint4 *>(a.k_min + at + c);
-        const uint4 hi4 = *reinterpret_cast<const uint4 *>(a.k_max + at + c);
-        const uint32_t lw[4] = {lo4.x, lo4.y, lo4.z, lo4.w};
-        const uint32_t hw[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t lb = (e & 1) ? lw[e >> 1] & 0xffff0000u : lw[e >> 1] << 16;
-          const uint32_t hb = (e & 1) ? hw[e >> 1] & 0xffff0000u : hw[e >> 1] << 16;
-          const double lo = (double)__uint_as_float(lb), hi = (double)__uint_as_float(hb);
-#pragma unroll
-          for (int g = 0; g < HEADS; ++g)
-            if (g0 + g < a.group) {
-              const double qv = qd[(g0 + g) * D + c + e];
-              acc[g] = fma(qv, qv >= 0.0 ? hi : lo, acc[g]);
-            }
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < HEADS; ++g)
-        if (g0 + g < a.group) best = fmax(best, acc[g]);  // NaN loses
+    for (int c = 0; c < V; ++c) {
+      const float v = bf16_f32(q[g * D + c]);
+      s = fma((double)v, (double)bf16_f32(v >= 0.0f ? hi.v[c] : lo.v[c]), s);
     }
-  } else {
-    report(a.err, NK_PAGE_OUT_OF_RANGE);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    best = fmax(best, s);  // NaN loses
   }
-  a.scores[(x.token * a.pool.heads + h) * a.score_ld + j] = best;
+  return best;
 }
 
-// f64 -> a whole number of the same order.
-__device__ __forceinline__ unsigned long long order_key(double v) {
-  v += 0.0;  // -0 ranks as 0
-  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+// A float or double -> a whole number of the same order (-0 ranks as 0), above 0.
+__device__ __forceinline__ u64 order_key(double v) {
+  v += 0.0;
+  const u64 b = (u64)__double_as_longlong(v);
   return b >> 63 ? ~b : b | (1ull << 63);
 }
+__device__ __forceinline__ uint32_t order_key(float v) {
+  v += 0.0f;
+  const uint32_t b = __float_as_uint(v);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
 
-// Block = (KV head x, token y): finds the need-th largest score digit by digit
-// (8 bits a pass, stopping once a digit's bin is taken whole), then writes the
-// chosen blocks in ascending order.
-__global__ void __launch_bounds__(256) block_topk_kernel(const SelectArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[8][2];
-  __shared__ int sh_digit, sh_need, sh_count;
+constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32;
+
+struct TopShared {
+  int hist[256];
+  u64 ends[2][kTopWarps];
+  int above[kTopWarps], equal[kTopWarps];
+  int digit, need, whole;
+};
+
+__device__ __forceinline__ uint32_t warp_min(uint32_t v) {
+  return __reduce_min_sync(0xffffffffu, v);
+}
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) {
+  return __reduce_max_sync(0xffffffffu, v);
+}
+__device__ __forceinline__ u64 warp_min(u64 v) {
+  for (int o = 16; o > 0; o >>= 1) {
+    const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = w < v ? w : v;
+  }
+  return v;
+}
+__device__ __forceinline__ u64 warp_max(u64 v) {
+  for (int o = 16; o > 0; o >>= 1) {
+    const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// Sum over the block; ends with a barrier behind which `sh` may be reused.
+__device__ __forceinline__ int block_sum(int v, int *sh) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kTopWarps; ++w) total += sh[w];
+  __syncthreads();
+  return total;
+}
+
+// The need-th largest of the keys at(j), j = j0, j0+32, .. < j1 of all threads
+// (0: no key; 1 <= need <= keys): a t that the need-th key reaches and the next
+// smaller one does not (`whole`), or, when keys tie there, their value.  A pass
+// spreads the keys that are left over 256 bins between the smallest and the
+// largest of them, so one or two passes end most searches among a few thousand.
+template <typename K, typename At>
+__device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopShared &sh,
+                                         bool &whole) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  K least = ~(K)0, most = 0;
+#pragma unroll 4
+  for (int j = j0; j < j1; j += 32) {
+    const K k = at(j);
+    if (k) {
+      least = k < least ? k : least;
+      most = k > most ? k : most;
+    }
+  }
+  least = warp_min(least);
+  most = warp_max(most);
+  if (lane == 0) {
+    sh.ends[0][warp] = least;
+    sh.ends[1][warp] = most;
+  }
+  if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kTopWarps; ++w) {
+    least = (K)sh.ends[0][w] < least ? (K)sh.ends[0][w] : least;
+    most = (K)sh.ends[1][w] > most ? (K)sh.ends[1][w] : most;
+  }
+  for (;;) {
+    const int bits = 64 - __clzll((long long)(u64)(most - least));
+    const int shift = bits > 8 ? bits - 8 : 0;
+#pragma unroll 4
+    for (int j = j0; j < j1; j += 32) {
+      const K k = at(j);
+      if (k >= least && k <= most) atomicAdd(&sh.hist[(int)((k - least) >> shift)], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {  // lane: bins 8*lane .. +7; higher bins hold larger keys
+      int c[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += c[i] = sh.hist[lane * 8 + i];
+      int up = sum;  // bins of this lane and the lanes above
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_down_sync(0xffffffffu, up, o);
+        if (lane + o < 32) up += v;
+      }
+      int before = up - sum;
+      if (before < need && up >= need) {  // one lane
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+          if (before < need) {
+            before += c[i];
+            if (before >= need) {
+              sh.digit = lane * 8 + i;
+              sh.need = need - (before - c[i]);
+              sh.whole = before == need;
+              before = need;  // found
+            }
+          }
+      }
+    }
+    __syncthreads();
+    least += (K)sh.digit << shift;
+    need = sh.need;
+    whole = sh.whole != 0;
+    if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+    __syncthreads();  // the shared words are read, the bins are empty
+    if (whole || shift == 0) return least;
+    most = least + (((K)1 << shift) - 1);
+  }
+}
+
+// Block = (KV head x, token y).  With L the need-th largest lower end of the
+// intervals: a block whose upper end is below L is out, and when exactly `need`
+// upper ends reach L they are the list.  If not, with H the (need+1)-th largest
+// upper end, a block whose lower end is above H is in and those in between are
+// scored in 64 bits.  Then the list is written in ascending order: a warp holds
+// a contiguous run of blocks, 32 neighbours at a time.
+template <int D>
+__global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const SelectArgs a) {
+  __shared__ TopShared sh;
   Query x;
   if (!find_query(a, blockIdx.y, x, threadIdx.x == 0)) return;
+  // Launched while the scores are computed: nothing of them is read before.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int h = blockIdx.x, n = x.blocks;
   int32_t *out = a.blocks + (x.token * a.pool.heads + h) * (int64_t)a.top_k;
   if (n <= a.top_k) {
-    for (int i = threadIdx.x; i < a.top_k; i += 256) out[i] = i < n ? i : -1;
+    for (int i = threadIdx.x; i < a.top_k; i += kTopThreads) out[i] = i < n ? i : -1;
     return;
   }
-  const double *sc = a.scores + (x.token * a.pool.heads + h) * a.score_ld;
+  const int64_t row = (x.token * a.pool.heads + h) * a.score_ld;
+  const float2 *range = a.range + row;
+  double *exact = a.exact + row;
   const int lo = a.sink, hi = n - a.local;  // free blocks
-  int need = a.top_k - a.sink - a.local;
-  unsigned long long prefix = 0, mask = 0;  // digits found so far
-  bool whole = need == 0;                   // all keys that match the prefix are taken
-  for (int shift = 56; shift >= 0 && !whole; shift -= 8) {
-    hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int j = lo + threadIdx.x; j < hi; j += 256) {
-      const unsigned long long key = order_key(sc[j]);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int left = need, d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      sh_digit = d;
-      sh_need = left;
-      sh_count = hist[d];
-    }
-    __syncthreads();
-    prefix |= (unsigned long long)sh_digit << shift;
-    mask |= 255ull << shift;
-    need = sh_need;
-    whole = sh_count == need;
-    __syncthreads();
-  }
-  // Above the prefix: taken.  Equal to it: the first `need` by index (all, when
-  // the bin is whole).  A contiguous run of blocks per thread keeps the order.
-  const int per = (n + 255) / 256;
-  const int a0 = threadIdx.x * per < n ? threadIdx.x * per : n;
-  const int a1 = a0 + per < n ? a0 + per : n;
-  const bool none = a.top_k == a.sink + a.local;
-  int above = 0, equal = 0;
-  for (int j = a0; j < a1; ++j) {
-    if (j < lo || j >= hi) {
-      ++above;
-    } else if (!none) {
-      const unsigned long long key = order_key(sc[j]) & mask;
-      above += key > prefix;
-      equal += key == prefix;
-    }
-  }
-  // Exclusive sums over the block of both counts.
-  int sa = above, se = equal;
+  const int need = a.top_k - a.sink - a.local;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int o = 1; o < 32; o <<= 1) {
-    const int va = __shfl_up_sync(0xffffffffu, sa, o), ve = __shfl_up_sync(0xffffffffu, se, o);
-    if (lane >= o) {
-      sa += va;
-      se += ve;
+  const int run = ((n + kTopThreads - 1) / kTopThreads) * 32;
+  const int j0 = warp * run + lane, j1 = (warp + 1) * run < n ? (warp + 1) * run : n;
+  auto is_free = [&](int j) { return j >= lo && j < hi; };
+  uint32_t low = 1, high = 0xffffffffu;
+  bool settled = true;  // no block is in doubt
+  if (need > 0) {
+    bool whole;
+    // A `whole` result may lie below L: the blocks it keeps in play are more.
+    low = nth_largest<uint32_t>(
+        j0, j1, [&](int j) { return is_free(j) ? order_key(range[j].x) : 0u; }, need, sh, whole);
+    int reach = 0;
+#pragma unroll 4
+    for (int j = j0; j < j1; j += 32) reach += is_free(j) && order_key(range[j].y) >= low;
+    settled = block_sum(reach, sh.above) == need;
+    if (!settled) {
+      auto upper = [&](int j) { return is_free(j) ? order_key(range[j].y) : 0u; };
+      high = nth_largest<uint32_t>(j0, j1, upper, need + 1, sh, whole);
+      // A whole result may lie below H, which is the smallest key that reaches it.
+      uint32_t least = 0xffffffffu;
+      for (int j = j0; j < j1; j += 32) {
+        const uint32_t k = upper(j);
+        if (k >= high && k < least) least = k;
+      }
+      least = warp_min(least);
+      if (lane == 0) sh.above[warp] = (int)least;
+      __syncthreads();
+      for (int w = 0; w < kTopWarps; ++w)
+        least = (uint32_t)sh.above[w] < least ? (uint32_t)sh.above[w] : least;
+      high = least;
+      __syncthreads();
     }
   }
-  if (lane == 31) {
-    warp_sum[warp][0] = sa;
-    warp_sum[warp][1] = se;
+  // 0: out, 1: in, 2: in doubt.
+  auto kind = [&](int j) {
+    if (!is_free(j)) return 1;
+    if (need == 0) return 0;
+    const float2 r = range[j];
+    if (order_key(r.y) < low) return 0;
+    return settled || order_key(r.x) > high ? 1 : 2;
+  };
+  u64 from = 0;       // blocks in doubt: taken above it,
+  bool ties = false;  // and the first by index of those equal to it
+  if (!settled) {
+    int in = 0;
+    for (int j = j0; j - lane < j1; j += 32) {
+      const int k = j < j1 ? kind(j) : 0;
+      in += k == 1 && is_free(j);
+      for (uint32_t doubt = __ballot_sync(0xffffffffu, k == 2); doubt; doubt &= doubt - 1) {
+        const int b = j - lane + __ffs(doubt) - 1;
+        const double v = exact_score<D>(a, x, h, b);
+        if (b == j) exact[b] = v;  // read again by this thread only
+      }
+    }
+    const int left = need - block_sum(in, sh.above);
+    bool whole = true;
+    from = ~0ull;  // no score is that large (it would be a NaN's)
+    if (left > 0)
+      from = nth_largest<u64>(
+          j0, j1, [&](int j) { return kind(j) == 2 ? order_key(exact[j]) : 0ull; }, left, sh,
+          whole);
+    ties = !whole;
+  }
+  // How a block counts: 0 out, 1 taken, 2 equal to the last score taken.
+  auto verdict = [&](int j) {
+    const int k = kind(j);
+    if (k != 2) return k;
+    const u64 e = order_key(exact[j]);
+    return e == from ? (ties ? 2 : 1) : (e > from ? 1 : 0);
+  };
+  int above = 0, equal = 0;
+  uint32_t kept = 0;  // the verdicts of the first 16 blocks of this thread
+  for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
+    const int v = j < j1 ? verdict(j) : 0;
+    if (i < 16) kept |= (uint32_t)v << (2 * i);
+    above += __popc(__ballot_sync(0xffffffffu, v == 1));
+    equal += __popc(__ballot_sync(0xffffffffu, v == 2));
+  }
+  if (lane == 0) {
+    sh.above[warp] = above;
+    sh.equal[warp] = equal;
   }
   __syncthreads();
-  for (int w = 0; w < warp; ++w) {
-    sa += warp_sum[w][0];
-    se += warp_sum[w][1];
-  }
-  int eq = se - equal;                       // equals before this run
-  int at = sa - above + (eq < need ? eq : need);
-  for (int j = a0; j < a1; ++j) {
-    bool take = j < lo || j >= hi;
-    if (!take && !none) {
-      const unsigned long long key = order_key(sc[j]) & mask;
-      if (key == prefix) take = eq++ < need;
-      else take = key > prefix;
+  int at = 0, eq = 0, all_above = 0;  // before this warp's run
+#pragma unroll
+  for (int w = 0; w < kTopWarps; ++w) {
+    all_above += sh.above[w];
+    if (w < warp) {
+      at += sh.above[w];
+      eq += sh.equal[w];
     }
-    if (take) out[at++] = j;
+  }
+  const int room = a.top_k - all_above;  // equals that are taken
+  at += eq < room ? eq : room;
+  const uint32_t below = (1u << lane) - 1;
+  for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
+    const int v = i < 16 ? (kept >> (2 * i)) & 3 : (j < j1 ? verdict(j) : 0);
+    const uint32_t same = __ballot_sync(0xffffffffu, v == 2);
+    const bool take = v == 1 || (v == 2 && eq + __popc(same & below) < room);
+    const uint32_t taken = __ballot_sync(0xffffffffu, take);
+    if (take) out[at + __popc(taken & below)] = j;
+    at += __popc(taken);
+    eq += __popc(same);
   }
 }
 
@@ -214,6 +528,30 @@ static nk_status check_select(const nk_kv_pages *kv, const nk_kv_batch *b) {
 
 static int64_t score_width(const nk_kv_pages *kv, const nk_kv_batch *b) {
   return ceil_div(b->max_kv > 0 ? b->max_kv : 1, kv->page_size);
+}
+
+template <int D, int HEADS>
+static nk_status launch_scores_heads(const SelectArgs &a, dim3 grid, cudaStream_t s) {
+  static std::atomic<uint64_t> prepared{0};  // a bit per device
+  nk_status st = allow_smem(reinterpret_cast<const void *>(block_scores_kernel<D, HEADS>),
+                            227 * 1024, prepared);
+  if (st != NK_OK) return st;
+  const int64_t wide = ceil_div(a.group, HEADS) * HEADS;
+  block_scores_kernel<D, HEADS><<<grid, 256, ScoreShared<D>::bytes(wide), s>>>(a);
+  return NK_OK;
+}
+
+// Heads of a pass: as many as a list has, up to 16.
+template <int D>
+static nk_status launch_scores(const SelectArgs &a, dim3 grid, cudaStream_t s) {
+  return a.group <= 2   ? launch_scores_heads<D, 2>(a, grid, s)
+         : a.group <= 4 ? launch_scores_heads<D, 4>(a, grid, s)
+         : a.group <= 8 ? launch_scores_heads<D, 8>(a, grid, s)
+                        : launch_scores_heads<D, 16>(a, grid, s);
+}
+
+static size_t select_bytes(const nk_kv_pages *kv, const nk_kv_batch *b) {
+  return (size_t)b->tokens * kv->kv_heads * score_width(kv, b) * (sizeof(float2) + sizeof(double));
 }
 
 }  // namespace nk
@@ -229,7 +567,7 @@ nk_status nk_kv_block_select_workspace_bytes(const nk_kv_pages *kv, const nk_kv_
   if (st == NK_OK) st = check_batch(kv, batch);
   if (st == NK_OK) st = check_select(kv, batch);
   if (st != NK_OK) return st;
-  *bytes = (size_t)batch->tokens * kv->kv_heads * score_width(kv, batch) * sizeof(double);
+  *bytes = select_bytes(kv, batch);
   return ok();
 }
 
@@ -249,8 +587,7 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
     return st;
   }
   const int64_t group = q_heads / kv->kv_heads;
-  if (group * kv->head_dim * 8 > 48 * 1024)
-    return fail(NK_UNSUPPORTED, "q_heads / kv_heads * head_dim must be <= 6144");
+  if (group > 64) return fail(NK_UNSUPPORTED, "q_heads / kv_heads must be <= 64");
   if (ld_q < q_heads * kv->head_dim)
     return fail(NK_INVALID_PARAMS, "ld_q must be >= q_heads * head_dim");
   if (sink < 0 || local < 1 || top_k < sink + local || top_k > (1 << 20))
@@ -258,7 +595,7 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0) return ok();
   if (!q || !blocks) return fail(NK_INVALID_PARAMS, "q and blocks are required");
   const int64_t width = score_width(kv, batch);
-  const size_t need = (size_t)batch->tokens * kv->kv_heads * width * sizeof(double);
+  const size_t need = select_bytes(kv, batch);
   if (workspace_bytes < need || !workspace) {
     st = fail(NK_WORKSPACE_TOO_SMALL, "block selection workspace too small");
     tls_error().expected = need;
@@ -279,24 +616,32 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.sink = (int)sink;
   a.local = (int)local;
   a.score_ld = width;
-  a.scores = static_cast<double *>(workspace);
+  a.exact = static_cast<double *>(workspace);
+  a.range = reinterpret_cast<float2 *>(a.exact + batch->tokens * kv->kv_heads * width);
   a.blocks = blocks;
   a.err = device_error_ptr();
   if (!a.err) return fail(NK_DEVICE_ERROR, "cannot resolve device error word");
   cudaStream_t s = as_stream(stream);
   if (width > top_k) {
-    const dim3 grid((unsigned)ceil_div(width, 128), (unsigned)kv->kv_heads,
+    const dim3 grid((unsigned)ceil_div(width, 64), (unsigned)kv->kv_heads,
                     (unsigned)batch->tokens);
-    const size_t smem = (size_t)(group * kv->head_dim * 8);
-    if (kv->head_dim == 128)
-      block_scores_kernel<128><<<grid, 128, smem, s>>>(a);
-    else
-      block_scores_kernel<64><<<grid, 128, smem, s>>>(a);
+    st = kv->head_dim == 128 ? launch_scores<128>(a, grid, s) : launch_scores<64>(a, grid, s);
+    if (st != NK_OK) return st;
     st = check_launch("block_scores_kernel");
     if (st != NK_OK) return st;
   }
-  block_topk_kernel<<<dim3((unsigned)kv->kv_heads, (unsigned)batch->tokens), 256, 0, s>>>(a);
-  return check_launch("block_topk_kernel");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)kv->kv_heads, (unsigned)batch->tokens);
+  cfg.blockDim = dim3(kTopThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = width > top_k ? 1 : 0;
+  NK_CUDA_TRY(kv->head_dim == 128 ? cudaLaunchKernelEx(&cfg, block_topk_kernel<128>, a)
+                                  : cudaLaunchKernelEx(&cfg, block_topk_kernel<64>, a));
+  return ok();
 }
 
 }  // extern "C"

@@ -2,6 +2,8 @@
 // ragged batch, and the checks every kernel makes of device arrays.
 #pragma once
 
+#include <atomic>
+
 #include "nk_common.cuh"
 
 namespace nk {
@@ -45,6 +47,17 @@ inline PageBatch page_batch(const nk_kv_batch &b) {
   p.max_new = (int)b.max_new;
   p.max_kv = (int)b.max_kv;
   return p;
+}
+
+// The kernel's dynamic shared memory, set once per device (`prepared`: a bit each).
+inline nk_status allow_smem(const void *kernel, int bytes, std::atomic<uint64_t> &prepared) {
+  int dev = 0;
+  NK_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (prepared.load(std::memory_order_acquire) & bit) return NK_OK;
+  NK_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  prepared.fetch_or(bit, std::memory_order_release);
+  return NK_OK;
 }
 
 // First error of a kernel stays in the device word.

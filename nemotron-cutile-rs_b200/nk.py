@@ -829,35 +829,38 @@ def _expect_ints(t, name, n, device):
         raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
 
 
-class _OnDevice:
-    """Runs libnk calls on the pages' device, whichever is current, and keeps
-    temporaries alive for an explicit stream."""
+def _on_pages_device(fn):
+    """Runs a wrapper with the device of its first tensor (or of the pages)
+    current: libnk launches on the current device."""
+    import functools
 
-    def __init__(self, device, stream):
+    @functools.wraps(fn)
+    def run(*args, **kw):
         import torch
 
-        self._guard = None
-        if torch.cuda.current_device() != device.index:
-            self._guard = torch.cuda.device(device)
-        self.stream = stream
+        index = (args[0] if args else next(iter(kw.values()))).device.index
+        if index is None or index == torch._C._cuda_getDevice():
+            return fn(*args, **kw)
+        with torch.cuda.device(index):
+            return fn(*args, **kw)
 
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-        self.ptr = stream_ptr(self.stream)
-        return self
+    return run
 
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
 
-    def hold(self, *tensors):
-        """Memory handed to this stream is not given out again before the
-        stream's queued work is done with it."""
-        if self.stream is not None:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(self.stream)
+def _stream_of(device, stream) -> int:
+    """The stream to launch on: the given one or the device's current one."""
+    import torch
+
+    return stream.cuda_stream if stream is not None else \
+        torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _hold(stream, *tensors):
+    """Memory handed to an explicit stream is not given out again before the
+    stream's queued work is done with it."""
+    if stream is not None:
+        for t in tensors:
+            t.record_stream(stream)
 
 
 class KvPages:
@@ -892,18 +895,31 @@ class KvPages:
                                  else table.shape[1])
         self._ref = ctypes.byref(self._struct)
 
-    def batch(self, start, kv_len, tokens, max_new, max_kv, rows=None) -> NkKvBatch:
+    def batch(self, start, kv_len, tokens, max_new, max_kv=None, rows=None) -> NkKvBatch:
         """The ragged batch of one step (nk_kv_batch): start int32 [n + 1],
-        kv_len int32 [n], rows int32 [n] or None on the pages' device."""
+        kv_len int32 [n], rows int32 [n] or None on the pages' device; max_kv
+        defaults to what the table can hold."""
         n = kv_len.numel()
         _expect_ints(start, "start", n + 1, self.device)
         _expect_ints(kv_len, "kv_len", n, self.device)
         if rows is not None:
             _expect_ints(rows, "rows", n, self.device)
-        return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(), ptr(rows), max_new,
-                         max_kv)
+        if max_kv is None:
+            max_kv = self.table.shape[1] * self.page_size
+        return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(),
+                         None if rows is None else rows.data_ptr(), max_new, max_kv)
+
+    def _queries(self, q, q_heads):
+        import torch
+
+        _expect(q, "q", torch.bfloat16, 2, self.device)
+        tokens, width = q.shape
+        if width != q_heads * self.head_dim:
+            raise ValueError(f"q must be [tokens, {q_heads * self.head_dim}]")
+        return tokens, (q.stride(0) if tokens > 1 else width)
 
 
+@_on_pages_device
 def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max_kv=None,
                     rows=None, layer: int = 0, stream=None) -> None:
     """Stores new keys and values (bf16 [tokens, kv_heads * head_dim], any row
@@ -917,23 +933,19 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
         if t.shape != (k_new.shape[0], width):
             raise ValueError(f"{name} must be [tokens, {width}]")
     tokens = k_new.shape[0]
-    b = pages.batch(start, kv_len, tokens, max_new, _max_kv(pages, max_kv), rows)
-    with _OnDevice(pages.device, stream) as on:
-        call("nk_kv_pages_append", pages._ref, layer, ctypes.byref(b), k_new.data_ptr(),
-             k_new.stride(0) if tokens > 1 else width, v_new.data_ptr(),
-             v_new.stride(0) if tokens > 1 else width, on.ptr)
-
-
-def _max_kv(pages: KvPages, max_kv):
-    return max_kv if max_kv is not None else pages.table.shape[1] * pages.page_size
+    b = pages.batch(start, kv_len, tokens, max_new, max_kv, rows)
+    ld_k, ld_v = (k_new.stride(0), v_new.stride(0)) if tokens > 1 else (width, width)
+    call("nk_kv_pages_append", pages._ref, layer, ctypes.byref(b), k_new.data_ptr(), ld_k,
+         v_new.data_ptr(), ld_v, _stream_of(pages.device, stream))
 
 
 def _host_ints(a, dtype):
     import numpy as np
 
-    return np.ascontiguousarray(np.asarray(a).reshape(-1), dtype=dtype)
+    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
 
 
+@_on_pages_device
 def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
     """Page dst[i] becomes a copy of page src[i] in every layer
     (nk_kv_pages_copy); src, dst are host sequences of page ids."""
@@ -942,10 +954,11 @@ def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
     s, d = _host_ints(src, np.int32), _host_ints(dst, np.int32)
     if s.size != d.size:
         raise ValueError("src and dst must have one length")
-    with _OnDevice(pages.device, stream) as on:
-        call("nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size, on.ptr)
+    call("nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size,
+         _stream_of(pages.device, stream))
 
 
+@_on_pages_device
 def kv_table_write(dst, values, offsets=None, stream=None) -> None:
     """dst.view(-1)[offsets[i]] = values[i] (nk_kv_table_write; offsets None:
     the first len(values) entries); dst is a contiguous int32 device tensor,
@@ -960,11 +973,11 @@ def kv_table_write(dst, values, offsets=None, stream=None) -> None:
     o = None if offsets is None else _host_ints(offsets, np.int64)
     if o is not None and o.size != v.size:
         raise ValueError("offsets and values must have one length")
-    with _OnDevice(dst.device, stream) as on:
-        call("nk_kv_table_write", ptr(dst), dst.numel(), None if o is None else o.ctypes.data,
-             v.ctypes.data, v.size, on.ptr)
+    call("nk_kv_table_write", ptr(dst), dst.numel(), None if o is None else o.ctypes.data,
+         v.ctypes.data, v.size, _stream_of(dst.device, stream))
 
 
+@_on_pages_device
 def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, dst_table=None,
                      new_len=None, stream=None):
     """Token base[b] + keep[b, i] of sequence b moves to position base[b] + i
@@ -981,25 +994,67 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
     _expect(keep, "keep", torch.int32, 2, dev)
     if keep.shape[0] != n:
         raise ValueError("keep must have a row for each sequence")
+    dst, dst_ld = None, 0
     if dst_table is not None:
         _expect(dst_table, "dst_table", torch.int32, 2, dev)
         if dst_table.shape[0] != n:
             raise ValueError("dst_table must have a row for each sequence")
-    if new_len is not None:
+        dst, dst_ld = dst_table.data_ptr(), dst_table.stride(0) if n > 1 else dst_table.shape[1]
+    if new_len is None:
+        new_len = torch.empty(n, dtype=torch.int32, device=dev)
+        _hold(stream, new_len)
+    else:
         _expect_ints(new_len, "new_len", n, dev)
-    with _OnDevice(dev, stream) as on:
-        if new_len is None:
-            new_len = torch.empty(n, dtype=torch.int32, device=dev)
-            on.hold(new_len)
-        width = keep.shape[1]
-        a = NkKvCompactArgs(n, ptr(rows), ptr(kv_len), ptr(base), ptr(keep),
-                            keep.stride(0) if n > 1 else width, ptr(n_keep), width,
-                            ptr(dst_table), 0 if dst_table is None else
-                            (dst_table.stride(0) if n > 1 else dst_table.shape[1]), ptr(new_len))
-        call("nk_kv_pages_compact", pages._ref, ctypes.byref(a), on.ptr)
+    width = keep.shape[1]
+    a = NkKvCompactArgs(n, ptr(rows), kv_len.data_ptr(), base.data_ptr(), keep.data_ptr(),
+                        keep.stride(0) if n > 1 else width, n_keep.data_ptr(), width, dst, dst_ld,
+                        new_len.data_ptr())
+    call("nk_kv_pages_compact", pages._ref, ctypes.byref(a), _stream_of(dev, stream))
     return new_len
 
 
+def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dtype, out,
+            workspace, stream):
+    """attention_paged behind its checks of q and the batch b."""
+    import torch
+
+    dev, tokens = pages.device, q.shape[0]
+    max_blocks = 0
+    if tree_mask is not None:
+        _expect(tree_mask, "tree_mask", torch.int64, 1, dev)
+        if tree_mask.numel() != tokens:
+            raise ValueError("tree_mask must hold a word for each token")
+    if blocks is not None:
+        _expect(blocks, "blocks", torch.int32, 3, dev)
+        if blocks.shape[:2] != (tokens, pages.kv_heads) or not blocks.is_contiguous():
+            raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
+        max_blocks = blocks.shape[2]
+    if out is None:
+        out = torch.empty(q.shape, device=dev,
+                          dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
+        _hold(stream, out)
+    elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be contiguous, of q's shape and on its device")
+    a = NkPagedAttentionArgs(q.data_ptr(), ld_q, q_heads, ptr(tree_mask), ptr(blocks), max_blocks,
+                             0 if scale is None else 1, 0.0 if scale is None else scale,
+                             out.data_ptr(), _dtype_code(out))
+    br, ar = ctypes.byref(b), ctypes.byref(a)
+    size = 0
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
+        size = need.value
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+            _hold(stream, workspace)
+    else:
+        size = workspace.numel()
+    call("nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace), size,
+         _stream_of(dev, stream))
+    return out
+
+
+@_on_pages_device
 def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=None, max_kv=None,
                     tree_mask=None, blocks=None, rows=None, layer: int = 0, scale=None,
                     out_dtype=BF16, out=None, workspace=None, stream=None):
@@ -1016,47 +1071,13 @@ def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=Non
     f32 with out_dtype=F32; rows that belong to no sequence stay as they were
     (a new `out` is not initialised).  workspace: optional uint8 device tensor
     of attention_paged_workspace_bytes."""
-    import torch
-
-    dev = pages.device
-    _expect(q, "q", torch.bfloat16, 2, dev)
-    tokens, width = q.shape
-    if width != q_heads * pages.head_dim:
-        raise ValueError(f"q must be [tokens, {q_heads * pages.head_dim}]")
-    if tree_mask is not None:
-        _expect(tree_mask, "tree_mask", torch.int64, 1, dev)
-        if tree_mask.numel() != tokens:
-            raise ValueError("tree_mask must hold a word for each token")
-    if blocks is not None:
-        _expect(blocks, "blocks", torch.int32, 3, dev)
-        if blocks.shape[:2] != (tokens, pages.kv_heads) or not blocks.is_contiguous():
-            raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
-    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q,
-                    _max_kv(pages, max_kv), rows)
-    with _OnDevice(dev, stream) as on:
-        if out is None:
-            out = torch.empty(tokens, width, device=dev,
-                              dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
-            on.hold(out)
-        elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
-            raise ValueError("out must be contiguous, of q's shape and on its device")
-        a = NkPagedAttentionArgs(q.data_ptr(), q.stride(0) if tokens > 1 else width, q_heads,
-                                 ptr(tree_mask), ptr(blocks),
-                                 0 if blocks is None else blocks.shape[2],
-                                 0 if scale is None else 1, 0.0 if scale is None else scale,
-                                 out.data_ptr(), _dtype_code(out))
-        br, ar = ctypes.byref(b), ctypes.byref(a)
-        if workspace is None:
-            need = ctypes.c_size_t(0)
-            call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
-            if need.value:
-                workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
-                on.hold(workspace)
-        call("nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace),
-             0 if workspace is None else workspace.numel(), on.ptr)
-    return out
+    tokens, ld_q = pages._queries(q, q_heads)
+    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    return _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dtype, out,
+                   workspace, stream)
 
 
+@_on_pages_device
 def attention_paged_workspace_bytes(pages: KvPages, tokens: int, seqs: int, q_heads: int, *,
                                     max_q: int, max_kv: int, max_blocks: int = 0) -> int:
     """Scratch bytes of attention_paged for these bounds (max_blocks > 0: the
@@ -1070,51 +1091,52 @@ def attention_paged_workspace_bytes(pages: KvPages, tokens: int, seqs: int, q_he
     return need.value
 
 
+def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspace, stream):
+    """kv_block_select behind its checks of q and the batch b."""
+    import torch
+
+    dev, tokens = pages.device, q.shape[0]
+    if out is None:
+        out = torch.empty(tokens, pages.kv_heads, max(top_k, 1), dtype=torch.int32, device=dev)
+        _hold(stream, out)
+    else:
+        _expect(out, "out", torch.int32, 3, dev)
+        if out.shape != (tokens, pages.kv_heads, top_k) or not out.is_contiguous():
+            raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
+    br = ctypes.byref(b)
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _hold(stream, workspace)
+    call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k, sink,
+         local, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(dev, stream))
+    return out
+
+
+@_on_pages_device
 def kv_block_select(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *, sink: int = 1,
                     local: int = 1, max_q=None, max_kv=None, rows=None, layer: int = 0, out=None,
                     workspace=None, stream=None):
     """The blocks each token's query reads (nk_kv_block_select): int32 [tokens,
     kv_heads, top_k], ascending, -1 behind the last; the first `sink` and last
     `local` blocks and those whose key bounds allow the largest scores."""
-    import torch
-
-    dev = pages.device
-    _expect(q, "q", torch.bfloat16, 2, dev)
-    tokens, width = q.shape
-    if width != q_heads * pages.head_dim:
-        raise ValueError(f"q must be [tokens, {q_heads * pages.head_dim}]")
-    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q,
-                    _max_kv(pages, max_kv), rows)
-    with _OnDevice(dev, stream) as on:
-        if out is None:
-            out = torch.empty(tokens, pages.kv_heads, max(top_k, 1), dtype=torch.int32, device=dev)
-            on.hold(out)
-        else:
-            _expect(out, "out", torch.int32, 3, dev)
-            if out.shape != (tokens, pages.kv_heads, top_k) or not out.is_contiguous():
-                raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
-        br = ctypes.byref(b)
-        if workspace is None:
-            need = ctypes.c_size_t(0)
-            call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            on.hold(workspace)
-        call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(),
-             q.stride(0) if tokens > 1 else width, q_heads, top_k, sink, local, ptr(out),
-             ptr(workspace), workspace.numel(), on.ptr)
-    return out
+    tokens, ld_q = pages._queries(q, q_heads)
+    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    return _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspace, stream)
 
 
+@_on_pages_device
 def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *,
                            sink: int = 1, local: int = 1, max_q=None, max_kv=None, rows=None,
                            layer: int = 0, scale=None, out_dtype=BF16, out=None, stream=None):
     """kv_block_select, then attention_paged over the chosen blocks; returns
     (out, blocks)."""
-    blocks = kv_block_select(q, pages, start, kv_len, q_heads, top_k, sink=sink, local=local,
-                             max_q=max_q, max_kv=max_kv, rows=rows, layer=layer, stream=stream)
-    return attention_paged(q, pages, start, kv_len, q_heads, max_q=max_q, max_kv=max_kv,
-                           blocks=blocks, rows=rows, layer=layer, scale=scale,
-                           out_dtype=out_dtype, out=out, stream=stream), blocks
+    tokens, ld_q = pages._queries(q, q_heads)
+    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    blocks = _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, None, None, stream)
+    return _attend(pages, q, ld_q, b, q_heads, None, blocks, layer, scale, out_dtype, out, None,
+                   stream), blocks
 
 
 # ------------------------------------------------- decoder steps around projections

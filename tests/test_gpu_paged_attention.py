@@ -431,3 +431,49 @@ def test_decoder_over_pages_matches_the_contiguous_cache(cuda):
     nk.device_status()
     out = model.generate(dev(toks[:, :T].copy()), steps, page_size=32)
     assert out.shape == (B, steps) and int(out.min()) >= 0 and int(out.max()) < 512
+
+
+@pytest.mark.parametrize("ps,d,group,n,top_k,step", [
+    (16, 64, 2, 700, 40, 0.0), (16, 128, 16, 5000, 64, 2.0**-16), (32, 64, 1, 300, 7, 2.0**-30),
+    (16, 128, 3, 4099, 1000, 2.0**-22), (16, 64, 17, 130, 64, 1.0)])
+def test_block_select_with_scores_that_nearly_tie(cuda, ps, d, group, n, top_k, step):
+    """Bounds that differ from block to block by a last place somewhere, so
+    that f32 sums cannot tell them apart, and many that are equal: the list is
+    the one of 64-bit sums, ties by index."""
+    c = Paged(n, [n * ps - 3], 1, ps, d)
+    r = c.rng
+    base = bf16(r.standard_normal(d))
+    c.lo[0], c.hi[0] = base, base
+    order = r.permutation(n)
+    for rank, j in enumerate(order):
+        ch = int(r.integers(0, d))
+        c.hi[0, c.table[0, j], 0, ch] = bf16(np.array([base[ch] + step * (rank // 3)]))[0]
+    q = bf16(r.standard_normal((1, group, d)))
+    want = chosen_blocks(q[0], c.lo[0, c.table[0, :n], 0], c.hi[0, c.table[0, :n], 0], n, top_k, 1,
+                         1)
+    got = nk.kv_block_select(dev(q.reshape(1, -1)).bfloat16(), c.device(), ints([0, 1]),
+                             ints([n * ps - 3]), group, top_k, max_q=1, max_kv=n * ps)
+    nk.device_status()
+    assert got.cpu().numpy()[0, 0].tolist() == want.tolist()
+
+
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_block_select_with_infinite_bounds_and_queries(cuda, value):
+    """What the definition makes of infinities and NaN, in a bound and in a
+    query: no f32 interval holds such a score."""
+    n, ps, d = 200, 16, 64
+    for where in ("hi", "lo", "q"):
+        c = Paged(5, [n * ps], 1, ps, d)
+        q = bf16(c.rng.standard_normal((1, 2, d)))
+        if where == "q":
+            q[0, 1, 9] = value
+        else:
+            for j in (3, 50, 51, 120):
+                getattr(c, where)[0, c.table[0, j], 0, 9] = value
+        q[0, 0, 9] = 0.0
+        want = chosen_blocks(q[0], c.lo[0, c.table[0, :n], 0], c.hi[0, c.table[0, :n], 0], n, 20,
+                             1, 1)
+        got = nk.kv_block_select(dev(q.reshape(1, -1)).bfloat16(), c.device(), ints([0, 1]),
+                                 ints([n * ps]), 2, 20, max_q=1, max_kv=n * ps)
+        nk.device_status()
+        assert got.cpu().numpy()[0, 0].tolist() == want.tolist(), where

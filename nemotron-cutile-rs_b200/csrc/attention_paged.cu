@@ -31,7 +31,7 @@ constexpr int kTile = 128;  // keys of a stage
 struct PagedAttn {
   PagePool pool;
   PageBatch batch;
-  const uint16_t *q;
+  const uint16_t *q, *v;  // v: the value pool, for poison()
   int64_t ld_q;
   int q_heads, group;
   int64_t layer_row;  // first token row of the layer in the pools
@@ -299,12 +299,14 @@ struct Cfg {
 // Producer warp of both attention kernels: streams the block's tiles into the
 // ring.  Lane = (page of the tile, channel strip, K or V): up to 32 boxes of 64
 // channels x one page.  Pages are looked up 32 at a time, a lane each, one
-// batch ahead of the loads.
-template <int D, int R, int STAGES>
+// batch ahead of the loads.  SPLIT: K and V of a tile are stages of their own
+// (2i and 2i+1), else they share one.  limits[i % LIMITS] gets the keys of tile
+// i that any row may see, by groups of 16.
+template <int D, int R, int STAGES, bool SPLIT, int LIMITS>
 __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
-                                          const CUtensorMap *kmap, const CUtensorMap *vmap,
-                                          uint8_t *ring, uint64_t *full, uint64_t *empty,
-                                          int (*limits)[8], int *abort_flag) {
+                                           const CUtensorMap *kmap, const CUtensorMap *vmap,
+                                           uint8_t *ring, uint64_t *full, uint64_t *empty,
+                                           int (*limits)[8], int *abort_flag) {
   constexpr int kTileBytes = kTile * D * 2;
   const int lane = threadIdx.x & 31;
   const int box_rows = a.pool.ps, npg = kTile >> a.pool.ps_log2;  // pages of a tile
@@ -330,7 +332,6 @@ __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
     lookup(base);
     base -= 32;
     for (int t = p.t0; t < p.t1; ++t, ++i) {
-      const int s = i % STAGES;
       const int e = t * npg + c;
       if (t * npg - base >= 32) {  // the same for all lanes
         base += 32;
@@ -340,35 +341,42 @@ __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
       }
       int page = __shfl_sync(0xffffffffu, page_now, (e - base) & 31);
       const int block = __shfl_sync(0xffffffffu, block_now, (e - base) & 31);
-      const bool room = i < STAGES || mbar_wait(&empty[s], ((i / STAGES) - 1) & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, room)) return;  // the lanes leave together
       if (block >= 0 && !page_ok(a.pool, page)) {
         report(a.err, NK_PAGE_OUT_OF_RANGE);
         page = -1;
       }
       const bool have = block >= 0 && page >= 0;
       const bool load = have && lane < boxes;
-      if (lane < npg) {
-        // Keys of the box that the rows may see: up to the last position.
-        int n = 0;
-        if (have) {
-          n = p.list ? p.pos + 1 - (block << a.pool.ps_log2) : p.keys - (e << a.pool.ps_log2);
-          n = n < 0 ? 0 : (n > box_rows ? box_rows : n);
+      const int64_t row =
+          a.layer_row + (((int64_t)page * a.pool.heads + p.head) << a.pool.ps_log2);
+#pragma unroll
+      for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
+        const int stage = SPLIT ? 2 * i + half : i, s = stage % STAGES;
+        const bool room = stage < STAGES ||
+                          mbar_wait(&empty[s], ((stage / STAGES) - 1) & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, room)) return;  // the lanes leave together
+        if (half == 0 && lane < npg) {
+          // Keys of the box that the rows may see: up to the last position.
+          int n = 0;
+          if (have) {
+            n = p.list ? p.pos + 1 - (block << a.pool.ps_log2) : p.keys - (e << a.pool.ps_log2);
+            n = n < 0 ? 0 : (n > box_rows ? box_rows : n);
+          }
+          for (int g = 0; g < box_rows / 16; ++g)
+            limits[i % LIMITS][c * (box_rows / 16) + g] =
+                n - 16 * g < 0 ? 0 : (n - 16 * g > 16 ? 16 : n - 16 * g);
         }
-        for (int g = 0; g < box_rows / 16; ++g)
-          limits[s][c * (box_rows / 16) + g] =
-              n - 16 * g < 0 ? 0 : (n - 16 * g > 16 ? 16 : n - 16 * g);
-      }
-      const uint32_t mine = __ballot_sync(0xffffffffu, load);
-      if (lane == 0)
-        mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(mine) * (uint32_t)box_rows * 128u);
-      __syncwarp();
-      if (load) {
-        uint8_t *dst = ring + s * 2 * kTileBytes + is_v * kTileBytes + strip * (kTile * 128) +
-                       c * box_rows * 128;
-        const int64_t row =
-            a.layer_row + (((int64_t)page * a.pool.heads + p.head) << a.pool.ps_log2);
-        tma_load_2d(dst, is_v ? vmap : kmap, &full[s], strip * 64, (int)row);
+        const bool now = load && (!SPLIT || is_v == half);
+        const uint32_t mine = __ballot_sync(0xffffffffu, now);
+        if (lane == 0)
+          mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(mine) * (uint32_t)box_rows * 128u);
+        __syncwarp();
+        if (now) {
+          uint8_t *dst = ring + s * (SPLIT ? 1 : 2) * kTileBytes +
+                         (SPLIT ? 0 : is_v * kTileBytes) + strip * (kTile * 128) +
+                         c * box_rows * 128;
+          tma_load_2d(dst, is_v ? vmap : kmap, &full[s], strip * 64, (int)row);
+        }
       }
     }
   }
@@ -383,6 +391,78 @@ __device__ __forceinline__ void drain_ring(uint64_t *full, int stages) {
       while (!mbar_try_wait(&full[s], ph) && nk_globaltimer() - start < 1000000ull) {
       }
     }
+}
+
+// Positions from here on are not seen by every row of the piece.
+__device__ __forceinline__ int seen_by_all(const PagedAttn &a, const Piece &p) {
+  return p.list ? 0x7fffffff : (a.mask ? p.prefix : p.prefix + p.row0 / a.group + 1);
+}
+// Whether the new token `tok` sees position pos < keys of its sequence.
+__device__ __forceinline__ bool sees(const PagedAttn &a, const Piece &p, int tok, int pos) {
+  if (!a.mask) return pos <= p.prefix + tok;
+  return pos < p.prefix ||
+         (tok < p.seq.count && ((a.mask[p.seq.first + tok] >> (pos - p.prefix)) & 1) != 0);
+}
+
+// A weight of 0 must leave no trace, and 0 * inf is NaN.  One of PARTS threads
+// of a key's row in the value tile: what lies behind the last key becomes 0, and
+// of the keys from `shared` on, which only some rows see, the infinities and
+// NaN become 0.  True when it found one: the piece's end puts them back for the
+// rows that see them (poison).  The weights are signalled behind this, so the
+// product reads the tile as it is then.
+template <int D>
+__device__ __forceinline__ bool clean_values(uint8_t *vt, int key, int part, int parts,
+                                             const int *limits, int shared) {
+  const bool dead = (key & 15) >= limits[key >> 4];
+  if (!dead && key < shared) return false;
+  bool found = false;
+#pragma unroll 1
+  for (int c = part * 8; c < D; c += parts * 8) {
+    uint4 *x = reinterpret_cast<uint4 *>(vt + strip_offset<kTile>(key, c));
+    if (dead) {
+      *x = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const uint4 y = *x;
+    uint32_t word[4] = {y.x, y.y, y.z, y.w};
+    bool hit = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((word[j] & 0x7f80u) == 0x7f80u) {
+        word[j] &= 0xffff0000u;
+        hit = true;
+      }
+      if ((word[j] & 0x7f800000u) == 0x7f800000u) {
+        word[j] &= 0x0000ffffu;
+        hit = true;
+      }
+    }
+    if (hit) *x = make_uint4(word[0], word[1], word[2], word[3]);
+    found |= hit;
+  }
+  fence_proxy_async_smem();  // before the stage is loaded again, or read by an MMA
+  return found;
+}
+
+// What a row's output channel gains from infinities and NaN that clean_values
+// took out: their sum over the keys of the piece that the row sees.
+__device__ __noinline__ float poison(const PagedAttn &a, const Piece &p, const uint16_t *v,
+                                     int head_dim, int tok, int chan) {
+  float sum = 0.0f;
+  int from = seen_by_all(a, p);
+  if (from < p.t0 * kTile) from = p.t0 * kTile;
+  const int to = p.keys < p.t1 * kTile ? p.keys : p.t1 * kTile;
+  for (int pos = from; pos < to; ++pos) {
+    if (!sees(a, p, tok, pos)) continue;
+    const int page = p.seq.table[pos >> a.pool.ps_log2];
+    if (!page_ok(a.pool, page)) continue;
+    const int64_t row = a.layer_row +
+                        (((int64_t)page * a.pool.heads + p.head) << a.pool.ps_log2) +
+                        (pos & (a.pool.ps - 1));
+    const float x = __uint_as_float((uint32_t)v[row * head_dim + chan] << 16);
+    if (!(fabsf(x) < INFINITY)) sum += x;
+  }
+  return sum;
 }
 
 // Barrier of the 256 compute threads that also ORs a flag.
@@ -418,7 +498,7 @@ __global__ void __launch_bounds__(288, 1)
   __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ __align__(16) int limits[STAGES][8];  // seen keys of each 16-key group
   __shared__ __align__(16) float red[R][8];        // a value per row and warp
-  __shared__ uint32_t odd_keys[4];  // keys of the tile that hold an infinity or NaN
+  __shared__ int odd;  // a value that only some rows see is no finite number
   __shared__ int abort_flag;
   __shared__ Cursor<R> share;
   __shared__ int per;
@@ -443,7 +523,7 @@ __global__ void __launch_bounds__(288, 1)
   Cursor<R> cur = share;
 
   if (warp == 8) {
-    load_tiles<D, R, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits, &abort_flag);
+    load_tiles<D, R, STAGES, false, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits, &abort_flag);
     if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
   } else {
     const int quad = lane >> 2, qc = (lane & 3) * 2;
@@ -481,14 +561,8 @@ __global__ void __launch_bounds__(288, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[mt][n][j] = 0.0f;
       }
-      // Positions from here on are not seen by every row of the tile.
-      const int all_see =
-          p.list ? 0x7fffffff : (a.mask ? p.prefix : p.prefix + p.row0 / a.group + 1);
-      auto allowed = [&](int tok, int pos) {  // pos < keys
-        if (!a.mask) return pos <= p.prefix + tok;
-        return pos < p.prefix ||
-               (tok < p.seq.count && ((a.mask[p.seq.first + tok] >> (pos - p.prefix)) & 1) != 0);
-      };
+      const int all_see = seen_by_all(a, p);
+      if (threadIdx.x == 0) odd = 0;
       compute_sync();  // the queries are there
 
       for (int t = p.t0; t < p.t1; ++t, ++i) {
@@ -503,37 +577,10 @@ __global__ void __launch_bounds__(288, 1)
         const int4 lb = *reinterpret_cast<const int4 *>(&limits[s][4]);
         const bool tail = la.x + la.y + la.z + la.w + lb.x + lb.y + lb.z + lb.w < kTile;
         const bool partial = !p.list && (t + 1) * kTile > all_see;
-        bool odd = false;
         if (tail || partial) {
-          // Values that a row may not see are multiplied by a weight of 0, so
-          // what lies behind the last key becomes 0, and keys that only some
-          // rows see are searched for infinities and NaN (0 * inf is NaN).
-          if (threadIdx.x < 4) odd_keys[threadIdx.x] = 0;
-          compute_sync();
-          const int key = threadIdx.x >> 1, part = threadIdx.x & 1;  // half of its channels
-          const bool dead = (key & 15) >= limits[s][key >> 4];
-          const bool some = partial && !dead && t * kTile + key >= all_see;
-          bool found = false;
-          if (dead || some) {
-#pragma unroll 1
-            for (int ch = 0; ch < D / 16; ++ch) {
-              uint4 *x = reinterpret_cast<uint4 *>(
-                  vt + strip_offset<kTile>(key, part * (D / 2) + ch * 8));
-              if (dead) {
-                *x = make_uint4(0, 0, 0, 0);
-              } else {
-                const uint4 y = *x;
-                const uint32_t word[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  found |= (word[j] & 0x7f80u) == 0x7f80u ||
-                           (word[j] & 0x7f800000u) == 0x7f800000u;
-              }
-            }
-          }
-          if (found) atomicOr(&odd_keys[key >> 5], 1u << (key & 31));
-          if (dead) fence_proxy_async_smem();  // before the stage is loaded again
-          odd = compute_vote(found);
+          if (clean_values<D>(vt, threadIdx.x >> 1, threadIdx.x & 1, 2, limits[s],
+                              partial ? all_see - t * kTile : kTile))
+            odd = 1;
         }
 
         // Scores of the warp's 16 keys.
@@ -571,7 +618,8 @@ __global__ void __launch_bounds__(288, 1)
               for (int j = 0; j < 4; ++j) {
                 const int key = n * 8 + qc + (j & 1);
                 bool ok = key < lim;
-                if (ok && partial) ok = allowed(tok_row[mt][j >> 1], t * kTile + warp * 16 + key);
+                if (ok && partial)
+                  ok = sees(a, p, tok_row[mt][j >> 1], t * kTile + warp * 16 + key);
                 if (!ok) sc[mt][n][j] = -INFINITY;
               }
         }
@@ -618,48 +666,6 @@ __global__ void __launch_bounds__(288, 1)
               o[mt][n][2 * hh + 1] *= corr;
             }
           }
-        if (odd) {
-          // Rare: an infinity or NaN in a key that some rows see.  Its terms
-          // are added by hand for the rows that see it (the weight is computed
-          // again: code that hardly ever runs should be small), then its
-          // values become 0.
-#pragma unroll 1
-          for (int key = 0; key < kTile; ++key) {
-            if (!((odd_keys[key >> 5] >> (key & 31)) & 1)) continue;
-            const int pos = t * kTile + key;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const int r = mt * 16 + quad + hh * 8;
-                if (r >= p.rows || !allowed(tok_row[mt][hh], pos)) continue;
-                float dot = 0.0f;
-#pragma unroll 1
-                for (int d = 0; d < D; ++d)
-                  dot += __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
-                             qs + strip_offset<R>(r, d))) *
-                         __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
-                             kt + strip_offset<kTile>(key, d)));
-                const float w = exp2_approx(dot * a.scale_log2 - mu[mt][hh]);
-#pragma unroll
-                for (int n = 0; n < ON; ++n)
-#pragma unroll
-                  for (int j = 0; j < 2; ++j)
-                    o[mt][n][2 * hh + j] +=
-                        w * __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(
-                                vt + strip_offset<kTile>(key, warp * COLS + n * 8 + qc + j)));
-              }
-          }
-          compute_sync();
-          const int key = threadIdx.x >> 1, part = threadIdx.x & 1;
-          if ((odd_keys[key >> 5] >> (key & 31)) & 1) {
-#pragma unroll 1
-            for (int ch = 0; ch < D / 16; ++ch)
-              *reinterpret_cast<uint4 *>(
-                  vt + strip_offset<kTile>(key, part * (D / 2) + ch * 8)) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-          }
-        }
         compute_sync();  // the weights are there
 
         // O += P V for the warp's columns.
@@ -712,6 +718,18 @@ __global__ void __launch_bounds__(288, 1)
       compute_sync();
       const int slot = 2 * (int)blockIdx.x + (piece > 0);
       const bool whole = p.first && p.last;
+      if (odd) {  // rare
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int n = 0; n < ON; ++n)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                o[mt][n][2 * hh + j] += poison(a, p, a.v, D, tok_row[mt][hh],
+                                               warp * COLS + n * 8 + qc + j);
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -748,10 +766,382 @@ __global__ void __launch_bounds__(288, 1)
         a.jobs[blockIdx.x] = j;
       }
       ++piece;
-      compute_sync();  // red is read before the next piece writes it
+      compute_sync();  // red and odd are read before the next piece writes them
     }
   }
   __syncthreads();
+  if (abort_flag && threadIdx.x == 0) report(a.err, NK_TIMEOUT);
+}
+
+// ------------------------------------------------------- more than 32 rows
+// tcgen05 products.  A unit is up to 256 rows: two tiles of 128 (A and B) that
+// share every K and V tile of 128 keys.  Per key tile and row tile
+//   S = Q K^T  128 x 128 x D, f32 in tensor memory,
+//   P          exp2 of the scaled scores, bf16, written over S,
+//   O += P V   P from tensor memory, V as it lies (MN-major), f32 in tensor memory.
+// Warps 0-3 turn A's scores into weights, a row a thread, warps 4-7 B's, warp 8
+// issues the products, warp 9 loads.  While one row tile's weights are computed
+// the tensor cores work for the other: with both tiles a key tile costs 2 x 1024
+// tensor cycles and 2 x 1024 cycles of exponentials side by side.
+// The running maximum moves only when it grows by more than 2^8 (weights stay
+// below 2^8, sums and bf16 lose nothing by that), so O is hardly ever rescaled.
+template <int D>
+struct TcCfg {
+  static constexpr int kRows = 256;
+  static constexpr int kStages = 5;  // K and V tiles of their own: K0 V0 K1 V1 ..
+  static constexpr int kLimits = 4;  // the loader is at most 3 tiles ahead
+  static constexpr int kTileBytes = kTile * D * 2;
+  static constexpr int kQBytes = 2 * 128 * D * 2;
+  static constexpr int kSmem = kStages * kTileBytes + kQBytes + 1024;
+  static constexpr int kThreads = 320;
+  static constexpr uint32_t kO = 256;  // tensor memory columns: S/P A, S/P B, O A, O B
+};
+
+// All lanes or none: a wait whose outcome the warp shares.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int *abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase, abort_flag));
+}
+
+template <int D>
+__global__ void __launch_bounds__(320, 1)
+    paged_attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
+                         const __grid_constant__ CUtensorMap vmap,
+                         const __grid_constant__ PagedAttn a) {
+  using C = TcCfg<D>;
+  constexpr int R = C::kRows, STAGES = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                              ~uintptr_t(1023));
+  uint8_t *qs = ring + STAGES * C::kTileBytes;  // [A, B][strips][128 rows][128 bytes]
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  __shared__ __align__(16) int limits[C::kLimits][8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ int odd[4];  // per piece: a value that only some rows see is no finite number
+  __shared__ Cursor<R> share;
+  __shared__ int per;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&q_full[g], 4);
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 4);
+      mbar_init(&o_full[g], 1);
+    }
+    mbar_init(&drain, 1);
+    fence_mbar_init();
+    abort_flag = 0;
+    if (a.jobs) a.jobs[blockIdx.x].parts = 0;
+  }
+  if (threadIdx.x == 288) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
+  find_share<R, C::kThreads>(a, share, &per);
+  if (share.left <= 0) return;
+  Cursor<R> cur = share;
+  if (warp == 8) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 9) {
+    load_tiles<D, R, STAGES, true, C::kLimits>(a, cur, &kmap, &vmap, ring, full, empty, limits,
+                                               &abort_flag);
+    if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
+  } else if (warp == 8) {
+    // --------------------------------------------------------------- products
+    const uint32_t idesc_s = idesc_bf16_f32(128, 128);
+    const uint32_t idesc_o = idesc_bf16_f32(128, D) | (1u << 16);  // B (the values) MN-major
+    int i = 0;           // tiles before this piece
+    int pieces[2] = {};  // pieces with rows in A / B
+    int tiles[2] = {};   // tiles of A / B so far
+    bool live = true;
+    Piece p;
+    auto scores = [&](int g, int tile) {  // lane 0
+      const uint32_t q = smem_u32(qs + g * (128 * D * 2));
+      const uint32_t k = smem_u32(ring + (2 * tile) % STAGES * C::kTileBytes);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const uint32_t off = (x >> 2) * (128 * 128) + (x & 3) * 32;
+        tc_mma_bf16(tmem + g * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s,
+                    x > 0);
+      }
+      tc_commit(&s_full[g]);
+    };
+    auto values = [&](int g, int tile, bool more) {  // lane 0
+      const uint32_t v = smem_u32(ring + (2 * tile + 1) % STAGES * C::kTileBytes);
+#pragma unroll
+      for (int x = 0; x < kTile / 16; ++x)
+        tc_mma_bf16_ta(tmem + C::kO + g * 128, tmem + g * 128 + x * 8,
+                       smem_desc_sw128_mn(v + x * 2048, kTile * 128), idesc_o, more || x > 0);
+    };
+    auto loaded = [&](int stage) {
+      return warp_wait(&full[stage % STAGES], (stage / STAGES) & 1, &abort_flag);
+    };
+    while (live && cur.next(a, p)) {
+      const int n = p.t1 - p.t0;
+      if (n <= 0) continue;
+      const int groups = p.rows > 128 ? 2 : 1;
+      for (int g = 0; live && g < groups; ++g)
+        live = warp_wait(&q_full[g], pieces[g] & 1, &abort_flag);
+      live = live && loaded(2 * i);
+      if (!live) break;
+      tc_fence_after();
+      if (lane == 0) {
+        for (int g = 0; g < groups; ++g) scores(g, i);
+        tc_commit(&empty[(2 * i) % STAGES]);
+      }
+      for (int x = 0; live && x < n; ++x) {
+        const int tile = i + x;
+        const bool again = x + 1 < n;
+        for (int g = 0; live && g < groups; ++g) {
+          // The weights of this row tile are in place; its next scores go over
+          // them, behind the product that reads them.
+          live = warp_wait(&p_full[g], tiles[g] & 1, &abort_flag) && loaded(2 * tile + 1);
+          if (live && again) live = loaded(2 * tile + 2);
+          if (!live) break;
+          ++tiles[g];
+          tc_fence_after();
+          if (lane == 0) {
+            values(g, tile, x > 0);
+            if (g == groups - 1) tc_commit(&empty[(2 * tile + 1) % STAGES]);
+            if (again) scores(g, tile + 1);
+            else tc_commit(&o_full[g]);
+            if (again && g == groups - 1) tc_commit(&empty[(2 * tile + 2) % STAGES]);
+          }
+          __syncwarp();
+        }
+      }
+      for (int g = 0; g < groups; ++g) ++pieces[g];
+      i += n;
+    }
+    if (*(volatile int *)&abort_flag) {  // products in flight end before the memory goes
+      if (lane == 0) tc_commit(&drain);
+      __syncwarp();
+      const uint64_t start = nk_globaltimer();
+      while (!mbar_try_wait(&drain, 0) && nk_globaltimer() - start < 10000000ull) {
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- weights
+    const int g = warp >> 2;
+    const int r = threadIdx.x;  // row of the unit
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + g * 128 + lanes, to = tmem + C::kO + g * 128 + lanes;
+    int i = 0, pieces_g = 0, tiles_g = 0, piece = 0;
+    bool live = true;
+    Piece p;
+    while (live && cur.next(a, p)) {
+      const int n = p.t1 - p.t0;
+      const bool mine = g == 0 || p.rows > 128;  // the row tile holds rows
+      const bool ok_row = r < p.rows;
+      const int tok = (p.row0 + r) / a.group;
+      const int all_see = seen_by_all(a, p);
+      float m = -INFINITY, l = 0.0f;
+      if (mine && n > 0) {
+        // A is at most two pieces ahead of B, so four flags are enough.
+        if (threadIdx.x == 0) odd[piece & 3] = 0;
+        // Queries: neighbouring threads load neighbouring 16 bytes of a row.
+        uint8_t *qt = qs + g * (128 * D * 2);
+#pragma unroll 4
+        for (int x = threadIdx.x & 127; x < 128 * D / 8; x += 128) {
+          const int qr = x / (D / 8), c = (x % (D / 8)) * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (g * 128 + qr < p.rows) {
+            const int y = p.row0 + g * 128 + qr, t = y / a.group;
+            v = *reinterpret_cast<const uint4 *>(
+                a.q + ((int64_t)p.seq.first + t) * a.ld_q +
+                ((int64_t)p.head * a.group + (y - t * a.group)) * D + c);
+          }
+          *reinterpret_cast<uint4 *>(qt + strip_offset<128>(qr, c)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[g]);
+        const uint64_t tree =
+            a.mask && ok_row && tok < p.seq.count ? a.mask[p.seq.first + tok] : 0;
+
+        for (int t = p.t0; t < p.t1; ++t) {
+          const int tile = i + t - p.t0;
+          live = warp_wait(&s_full[g], tiles_g & 1, &abort_flag);
+          if (!live) break;
+          ++tiles_g;
+          tc_fence_after();
+          const int *lim = limits[tile % C::kLimits];
+          const int4 la = *reinterpret_cast<const int4 *>(lim);
+          const int4 lb = *reinterpret_cast<const int4 *>(lim + 4);
+          const bool tail = la.x + la.y + la.z + la.w + lb.x + lb.y + lb.z + lb.w < kTile;
+          const bool partial = !p.list && (t + 1) * kTile > all_see;
+          if (g == 0 && (tail || partial)) {
+            const int stage = 2 * tile + 1;
+            live = warp_wait(&full[stage % STAGES], (stage / STAGES) & 1, &abort_flag);
+            if (!live) break;
+            if (clean_values<D>(ring + stage % STAGES * C::kTileBytes, r, 0, 1, lim,
+                                partial ? all_see - t * kTile : kTile))
+              odd[piece & 3] = 1;
+            __syncwarp();
+          }
+          // Keys of a chunk of 32 that this row sees, a bit each.
+          auto seen = [&](int c) -> uint32_t {
+            const int l0 = lim[2 * c], l1 = lim[2 * c + 1];
+            uint32_t bits = ((1u << l0) - 1) | ((1u << l1) - 1) << 16;
+            if (partial) {
+              const int k0 = t * kTile + c * 32;
+              if (a.mask) {
+                // positions below the prefix, then the tree's bits
+                const int d = k0 - p.prefix;  // draft of the chunk's first key
+                uint32_t see;
+                if (d >= 0) see = d < 64 ? (uint32_t)(tree >> d) : 0u;
+                else if (d > -32) see = (uint32_t)(tree << -d) | ((1u << -d) - 1);
+                else see = 0xffffffffu;
+                bits &= see;
+              } else {
+                const int last = p.prefix + tok - k0;  // last key seen
+                bits &= last >= 31 ? 0xffffffffu : (last < 0 ? 0u : (2u << last) - 1);
+              }
+            }
+            return bits;
+          };
+          const bool masked = tail || partial;
+          float mx = -INFINITY;
+          __syncwarp();
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            tmem_ld32(ts + c * 32, v);
+            if (masked) {
+              const uint32_t bits = seen(c);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((bits >> j) & 1)) v[j] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+          }
+          const float mn = mx * a.scale_log2;
+          // First keys of the row, or a maximum that has outgrown the old one.
+          const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m);
+          const float corr = grow ? exp2_approx(m - mn) : 1.0f;  // 0 for the first keys
+          if (grow) {
+            m = mn;
+            l *= corr;
+          }
+          if (t > p.t0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float v[32];
+              tmem_ld32(to + c * 32, v);
+              uint32_t w[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[j] * corr);
+              tmem_st16(to + c * 32, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
+              tmem_st16(to + c * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+            }
+          }
+          const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            tmem_ld32(ts + c * 32, v);
+            if (masked) {
+              const uint32_t bits = seen(c);
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((bits >> j) & 1)) v[j] = -INFINITY;
+            }
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float w0 = exp2_approx(v[j] * a.scale_log2 - mu);
+              const float w1 = exp2_approx(v[j + 1] * a.scale_log2 - mu);
+              l += w0 + w1;
+              w[j / 2] = pack_bf16(w0, w1);
+            }
+            tmem_st16(ts + c * 16, w);  // over scores that have been read
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[g]);
+        }
+        live = live && warp_wait(&o_full[g], pieces_g & 1, &abort_flag);
+        if (!live) break;
+        ++pieces_g;
+        tc_fence_after();
+      }
+      const int slot = 2 * (int)blockIdx.x + (piece > 0);
+      const bool whole = p.first && p.last;
+      if (mine) {
+        const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+        const int64_t at = whole ? out_row(a, p.seq.first, p.head, p.row0 + r) * D
+                                 : ((int64_t)slot * R + r) * D;
+        if (!whole && ok_row) a.part_ml[(int64_t)slot * R + r] = make_float2(m, l);
+        const bool bad = n > 0 && odd[piece & 3];
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          __syncwarp();
+          if (n > 0) {
+            tmem_ld32(to + c * 32, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          }
+          if (!ok_row) continue;
+          if (bad) {  // rare
+#pragma unroll 1
+            for (int j = 0; j < 32; ++j) {
+              const float x = poison(a, p, a.v, D, tok, c * 32 + j);
+#pragma unroll
+              for (int y = 0; y < 32; ++y)
+                if (y == j) v[y] += x;
+            }
+          }
+          // A row that sees nothing has l = 0; what the product left is 0 * value.
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 x = make_float4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
+            if (!whole)
+              *reinterpret_cast<float4 *>(a.part_o + at + c * 32 + j) = x;
+            else if (a.out_f32)
+              *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at + c * 32 + j) = x;
+            else
+              *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at + c * 32 + j) =
+                  make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+          }
+        }
+        __syncwarp();
+        tc_fence_before();  // O is read before the next piece's weights are signalled
+      }
+      if (threadIdx.x == 0 && p.first && !p.last) {
+        MergeJob j{};
+        j.slot0 = slot;
+        j.parts = (p.unit_at + cur.tiles - 1) / per - (int)blockIdx.x + 1;
+        j.first_token = p.seq.first;
+        j.row0 = p.row0;
+        j.rows = p.rows;
+        j.head = p.head;
+        a.jobs[blockIdx.x] = j;
+      }
+      ++piece;
+      i += n > 0 ? n : 0;
+    }
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
   if (abort_flag && threadIdx.x == 0) report(a.err, NK_TIMEOUT);
 }
 
@@ -800,7 +1190,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
 // ------------------------------------------------------------------- host
 // Row tile and blocks of a call, from its bounds alone.
 struct AttnPlan {
-  int row_tiles;  // 16 * row_tiles rows a unit
+  int row_tiles;  // 16 * row_tiles rows a unit (1, 2, or 16: tensor memory)
   double tiles;   // the longest list
   int blocks;
   bool merge;     // a unit may be split over blocks
@@ -812,7 +1202,7 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   AttnPlan p{};
   const int64_t group = a.q_heads / kv.kv_heads;
   const int64_t rows = a.blocks ? group : b.max_new * group;
-  p.row_tiles = rows <= 16 ? 1 : 2;
+  p.row_tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : 16);
   const int64_t r = 16 * p.row_tiles;
   const int64_t units = a.blocks ? b.max_new * ceil_div(group, r) : ceil_div(rows, r);
   int64_t keys = b.max_kv;
@@ -887,16 +1277,28 @@ static nk_status page_map(const uint16_t *base, int64_t rows, int64_t d, int box
   return NK_OK;
 }
 
-template <int D, int MT>
+template <typename Kernel>
+static nk_status launch_attention(Kernel kernel, int smem, int threads,
+                                  std::atomic<uint64_t> &prepared, const CUtensorMap &km,
+                                  const CUtensorMap &vm, const PagedAttn &a, const AttnPlan &p,
+                                  cudaStream_t s) {
+  nk_status st = allow_smem(reinterpret_cast<const void *>(kernel), smem, prepared);
+  if (st != NK_OK) return st;
+  kernel<<<p.blocks, threads, smem, s>>>(km, vm, a);
+  return check_launch("paged attention");
+}
+
+template <int D>
 static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
                                   const PagedAttn &a, const AttnPlan &p, cudaStream_t s) {
-  using C = Cfg<D, MT>;
-  static std::atomic<uint64_t> prepared{0};  // a bit per device
-  nk_status st = allow_smem(reinterpret_cast<const void *>(paged_attn_kernel<D, MT>), C::kSmem,
-                            prepared);
-  if (st != NK_OK) return st;
-  paged_attn_kernel<D, MT><<<p.blocks, C::kThreads, C::kSmem, s>>>(km, vm, a);
-  st = check_launch("paged_attn_kernel");
+  static std::atomic<uint64_t> prepared[3];  // a bit per device
+  nk_status st =
+      p.row_tiles == 1 ? launch_attention(paged_attn_kernel<D, 1>, Cfg<D, 1>::kSmem,
+                                          Cfg<D, 1>::kThreads, prepared[0], km, vm, a, p, s)
+      : p.row_tiles == 2 ? launch_attention(paged_attn_kernel<D, 2>, Cfg<D, 2>::kSmem,
+                                            Cfg<D, 2>::kThreads, prepared[1], km, vm, a, p, s)
+                         : launch_attention(paged_attn_tc_kernel<D>, TcCfg<D>::kSmem,
+                                            TcCfg<D>::kThreads, prepared[2], km, vm, a, p, s);
   if (st != NK_OK || !p.merge) return st;
   // The merge is launched while the attention runs and waits on the device for
   // its end, which hides the launch.
@@ -909,7 +1311,7 @@ static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_merge_kernel<D>, a, (int)C::kRows));
+  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_merge_kernel<D>, a, 16 * p.row_tiles));
   return ok();
 }
 
@@ -952,6 +1354,7 @@ nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.pool = page_pool(*kv);
   a.batch = page_batch(*batch);
   a.q = args->q;
+  a.v = kv->v;
   a.ld_q = args->ld_q;
   a.q_heads = (int)args->q_heads;
   a.group = (int)(args->q_heads / kv->kv_heads);
@@ -978,11 +1381,8 @@ nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   if (st == NK_OK) st = page_map(kv->v, rows, kv->head_dim, box, &vm);
   if (st != NK_OK) return st;
   cudaStream_t s = as_stream(stream);
-  if (kv->head_dim == 128)
-    return p.row_tiles == 1 ? launch_attention<128, 1>(km, vm, a, p, s)
-                            : launch_attention<128, 2>(km, vm, a, p, s);
-  return p.row_tiles == 1 ? launch_attention<64, 1>(km, vm, a, p, s)
-                          : launch_attention<64, 2>(km, vm, a, p, s);
+  return kv->head_dim == 128 ? launch_attention<128>(km, vm, a, p, s)
+                             : launch_attention<64>(km, vm, a, p, s);
 }
 
 }  // extern "C"

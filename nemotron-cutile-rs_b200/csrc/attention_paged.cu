@@ -73,6 +73,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<unsigned long long *>(&d))
+      : "l"(*reinterpret_cast<const unsigned long long *>(&a)),
+        "l"(*reinterpret_cast<const unsigned long long *>(&b)),
+        "l"(*reinterpret_cast<const unsigned long long *>(&c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<unsigned long long *>(&d))
+      : "l"(*reinterpret_cast<const unsigned long long *>(&a)),
+        "l"(*reinterpret_cast<const unsigned long long *>(&b)));
+  return d;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&v);
@@ -814,7 +832,7 @@ __global__ void __launch_bounds__(320, 1)
                                               ~uintptr_t(1023));
   uint8_t *qs = ring + STAGES * C::kTileBytes;  // [A, B][strips][128 rows][128 bytes]
   __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+  __shared__ uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], e_done[2], drain;
   __shared__ __align__(16) int limits[C::kLimits][8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -832,8 +850,10 @@ __global__ void __launch_bounds__(320, 1)
     for (int g = 0; g < 2; ++g) {
       mbar_init(&q_full[g], 4);
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 4);
+      mbar_init(&p_full[g][0], 4);  // the weights of keys 0-63
+      mbar_init(&p_full[g][1], 4);  // and of keys 64-127
       mbar_init(&o_full[g], 1);
+      mbar_init(&e_done[g], 4);
     }
     mbar_init(&drain, 1);
     fence_mbar_init();
@@ -880,10 +900,10 @@ __global__ void __launch_bounds__(320, 1)
       }
       tc_commit(&s_full[g]);
     };
-    auto values = [&](int g, int tile, bool more) {  // lane 0
+    auto values = [&](int g, int half, int tile, bool more) {  // lane 0
       const uint32_t v = smem_u32(ring + (2 * tile + 1) % STAGES * C::kTileBytes);
 #pragma unroll
-      for (int x = 0; x < kTile / 16; ++x)
+      for (int x = half * (kTile / 32); x < (half + 1) * (kTile / 32); ++x)
         tc_mma_bf16_ta(tmem + C::kO + g * 128, tmem + g * 128 + x * 8,
                        smem_desc_sw128_mn(v + x * 2048, kTile * 128), idesc_o, more || x > 0);
     };
@@ -907,15 +927,20 @@ __global__ void __launch_bounds__(320, 1)
         const int tile = i + x;
         const bool again = x + 1 < n;
         for (int g = 0; live && g < groups; ++g) {
-          // The weights of this row tile are in place; its next scores go over
-          // them, behind the product that reads them.
-          live = warp_wait(&p_full[g], tiles[g] & 1, &abort_flag) && loaded(2 * tile + 1);
+          // The weights of this row tile come in halves; its next scores go
+          // over them, behind the products that read them.
+          live = warp_wait(&p_full[g][0], tiles[g] & 1, &abort_flag) && loaded(2 * tile + 1);
+          if (!live) break;
+          tc_fence_after();
+          if (lane == 0) values(g, 0, tile, x > 0);
+          __syncwarp();
+          live = warp_wait(&p_full[g][1], tiles[g] & 1, &abort_flag);
           if (live && again) live = loaded(2 * tile + 2);
           if (!live) break;
           ++tiles[g];
           tc_fence_after();
           if (lane == 0) {
-            values(g, tile, x > 0);
+            values(g, 1, tile, true);
             if (g == groups - 1) tc_commit(&empty[(2 * tile + 1) % STAGES]);
             if (again) scores(g, tile + 1);
             else tc_commit(&o_full[g]);
@@ -940,32 +965,47 @@ __global__ void __launch_bounds__(320, 1)
     const int r = threadIdx.x;  // row of the unit
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + g * 128 + lanes, to = tmem + C::kO + g * 128 + lanes;
-    int i = 0, pieces_g = 0, tiles_g = 0, piece = 0;
+    int i = 0, pieces_g = 0, tiles_g = 0, ends_g = 0, piece = 0;
     bool live = true;
     Piece p;
     while (live && cur.next(a, p)) {
       const int n = p.t1 - p.t0;
       const bool mine = g == 0 || p.rows > 128;  // the row tile holds rows
       const bool ok_row = r < p.rows;
-      const int tok = (p.row0 + r) / a.group;
+      const int tok0 = p.row0 / a.group, tok = (p.row0 + r) / a.group;
       const int all_see = seen_by_all(a, p);
       float m = -INFINITY, l = 0.0f;
+      // The warps of a row tile leave the shared memory of its last results
+      // together.
+      if (mine && ends_g > 0 && !warp_wait(&e_done[g], (ends_g - 1) & 1, &abort_flag)) break;
       if (mine && n > 0) {
         // A is at most two pieces ahead of B, so four flags are enough.
         if (threadIdx.x == 0) odd[piece & 3] = 0;
-        // Queries: neighbouring threads load neighbouring 16 bytes of a row.
+        // Queries: neighbouring threads load neighbouring 16 bytes of a row, 8
+        // rows' loads in flight.
         uint8_t *qt = qs + g * (128 * D * 2);
-#pragma unroll 4
-        for (int x = threadIdx.x & 127; x < 128 * D / 8; x += 128) {
-          const int qr = x / (D / 8), c = (x % (D / 8)) * 8;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (g * 128 + qr < p.rows) {
-            const int y = p.row0 + g * 128 + qr, t = y / a.group;
-            v = *reinterpret_cast<const uint4 *>(
-                a.q + ((int64_t)p.seq.first + t) * a.ld_q +
-                ((int64_t)p.head * a.group + (y - t * a.group)) * D + c);
+        constexpr int RP = 128 / (D / 8);  // rows of a pass over the threads
+        const int q0 = (threadIdx.x & 127) / (D / 8), qc = (threadIdx.x % (D / 8)) * 8;
+        const int over = p.row0 - tok0 * a.group;  // row0 = tok0 * group + over
+        const float inv_group = 1.0f / (float)a.group;
+#pragma unroll 1
+        for (int x0 = 0; x0 < 128; x0 += 8 * RP) {
+          uint4 v[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int y = g * 128 + x0 + x * RP + q0;  // row of the unit
+            v[x] = make_uint4(0, 0, 0, 0);
+            if (y < p.rows) {
+              // (over + y) / group: the half keeps the product off whole numbers
+              const int t = (int)(((float)(over + y) + 0.5f) * inv_group);
+              v[x] = *reinterpret_cast<const uint4 *>(
+                  a.q + ((int64_t)p.seq.first + tok0 + t) * a.ld_q +
+                  ((int64_t)p.head * a.group + (over + y - t * a.group)) * D + qc);
+            }
           }
-          *reinterpret_cast<uint4 *>(qt + strip_offset<128>(qr, c)) = v;
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            *reinterpret_cast<uint4 *>(qt + strip_offset<128>(x0 + x * RP + q0, qc)) = v[x];
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -1015,22 +1055,28 @@ __global__ void __launch_bounds__(320, 1)
             return bits;
           };
           const bool masked = tail || partial;
-          float mx = -INFINITY;
+          // The row's 128 scores stay in registers from here to the weights.
+          uint32_t sv[128];
           __syncwarp();
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float v[32];
-            tmem_ld32(ts + c * 32, v);
-            if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_issue(ts + c * 32, sv + c * 32);
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
               const uint32_t bits = seen(c);
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (!((bits >> j) & 1)) v[j] = -INFINITY;
+                if (!((bits >> j) & 1)) sv[c * 32 + j] = 0xff800000u;
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
           }
-          const float mn = mx * a.scale_log2;
+          float mx = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 128; j += 4) {
+            mx = fmaxf(mx, fmaxf(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])));
+            mx1 = fmaxf(mx1, fmaxf(__uint_as_float(sv[j + 2]), __uint_as_float(sv[j + 3])));
+          }
+          const float mn = fmaxf(mx, mx1) * a.scale_log2;
           // First keys of the row, or a maximum that has outgrown the old one.
           const bool grow = mn > m + 8.0f || (m == -INFINITY && mn > m);
           const float corr = grow ? exp2_approx(m - mn) : 1.0f;  // 0 for the first keys
@@ -1040,41 +1086,42 @@ __global__ void __launch_bounds__(320, 1)
           }
           if (t > p.t0 && __any_sync(0xffffffffu, grow)) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float v[32];
-              tmem_ld32(to + c * 32, v);
-              uint32_t w[32];
+            for (int c = 0; c < D / 16; ++c) {
+              float v[16];
+              tmem_ld16(to + c * 16, v);
+              uint32_t w[16];
 #pragma unroll
-              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[j] * corr);
-              tmem_st16(to + c * 32, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
-              tmem_st16(to + c * 32 + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j] * corr);
+              tmem_st16(to + c * 16, w);
             }
           }
           const float mu = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            float v[32];
-            tmem_ld32(ts + c * 32, v);
-            if (masked) {
-              const uint32_t bits = seen(c);
+          const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
+          const float2 mu2 = make_float2(-mu, -mu);
+          float2 sum2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (!((bits >> j) & 1)) v[j] = -INFINITY;
-            }
-            uint32_t w[16];
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float w0 = exp2_approx(v[j] * a.scale_log2 - mu);
-              const float w1 = exp2_approx(v[j + 1] * a.scale_log2 - mu);
-              l += w0 + w1;
-              w[j / 2] = pack_bf16(w0, w1);
+            for (int c = 2 * half; c < 2 * half + 2; ++c) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                float2 x = make_float2(__uint_as_float(sv[c * 32 + j]),
+                                       __uint_as_float(sv[c * 32 + j + 1]));
+                x = fma2(x, scale2, mu2);
+                x.x = exp2_approx(x.x);
+                x.y = exp2_approx(x.y);
+                sum2 = add2(sum2, x);
+                w[j / 2] = pack_bf16(x.x, x.y);
+              }
+              tmem_st16(ts + c * 16, w);  // over scores that have been read
             }
-            tmem_st16(ts + c * 16, w);  // over scores that have been read
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[g][half]);
           }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[g]);
+          l += sum2.x + sum2.y;
         }
         live = live && warp_wait(&o_full[g], pieces_g & 1, &abort_flag);
         if (!live) break;
@@ -1085,10 +1132,15 @@ __global__ void __launch_bounds__(320, 1)
       const bool whole = p.first && p.last;
       if (mine) {
         const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        const int64_t at = whole ? out_row(a, p.seq.first, p.head, p.row0 + r) * D
-                                 : ((int64_t)slot * R + r) * D;
         if (!whole && ok_row) a.part_ml[(int64_t)slot * R + r] = make_float2(m, l);
         const bool bad = n > 0 && odd[piece & 3];
+        // Through shared memory (the queries' tile is free): a thread holds a
+        // row, a store instruction writes 4 rows of 32 columns.
+        float4 *stage = reinterpret_cast<float4 *>(qs + g * (128 * D * 2) + (warp & 3) * 4096);
+        const int er = lane >> 3, ec = lane & 7;
+        const int first_row = r - lane;
+        const int over = p.row0 - tok0 * a.group;
+        const float inv_group = 1.0f / (float)a.group;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
@@ -1099,8 +1151,7 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.0f;
           }
-          if (!ok_row) continue;
-          if (bad) {  // rare
+          if (bad && ok_row) {  // rare
 #pragma unroll 1
             for (int j = 0; j < 32; ++j) {
               const float x = poison(a, p, a.v, D, tok, c * 32 + j);
@@ -1109,21 +1160,35 @@ __global__ void __launch_bounds__(320, 1)
                 if (y == j) v[y] += x;
             }
           }
-          // A row that sees nothing has l = 0; what the product left is 0 * value.
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 x = make_float4(v[j] * f, v[j + 1] * f, v[j + 2] * f, v[j + 3] * f);
-            if (!whole)
-              *reinterpret_cast<float4 *>(a.part_o + at + c * 32 + j) = x;
-            else if (a.out_f32)
-              *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at + c * 32 + j) = x;
+          for (int j = 0; j < 8; ++j)
+            stage[lane * 8 + (j ^ (lane & 7))] =
+                make_float4(v[4 * j] * f, v[4 * j + 1] * f, v[4 * j + 2] * f, v[4 * j + 3] * f);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int lr = k * 4 + er, y = first_row + lr;  // row of the unit
+            const float4 x = stage[lr * 8 + (ec ^ (lr & 7))];
+            if (y >= p.rows) continue;
+            if (!whole) {
+              *reinterpret_cast<float4 *>(a.part_o + ((int64_t)slot * R + y) * D + c * 32 +
+                                          ec * 4) = x;
+              continue;
+            }
+            const int t = (int)(((float)(over + y) + 0.5f) * inv_group);
+            const int64_t at = (((int64_t)p.seq.first + tok0 + t) * a.q_heads +
+                                p.head * a.group + (over + y - t * a.group)) * D + c * 32 + ec * 4;
+            if (a.out_f32)
+              *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = x;
             else
-              *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at + c * 32 + j) =
+              *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) =
                   make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
           }
         }
         __syncwarp();
         tc_fence_before();  // O is read before the next piece's weights are signalled
+        if (lane == 0) mbar_arrive(&e_done[g]);
+        ++ends_g;
       }
       if (threadIdx.x == 0 && p.first && !p.last) {
         MergeJob j{};
@@ -1146,29 +1211,33 @@ __global__ void __launch_bounds__(320, 1)
 }
 
 // Joins the parts of the unit that begins in block blockIdx.x of the
-// attention, in their order: a warp per row, blockIdx.y over the rows.
+// attention, in their order.  A block takes 4 rows; the 4 warps of a row sum
+// every fourth part and meet in shared memory.
 template <int D>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedAttn a, int R) {
+__global__ void __launch_bounds__(512)
+    paged_merge_kernel(const __grid_constant__ PagedAttn a, int R) {
+  constexpr int V = D / 32;
+  __shared__ float sum[3][4][32][V + 1];
   // Launched while the attention runs: nothing is read before it has ended.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const MergeJob j = a.jobs[blockIdx.x];
-  const int lane = threadIdx.x & 31;
-  constexpr int V = D / 32;
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); j.parts > 0 && r < j.rows;
-       r += gridDim.y * 4) {
-    // Part i > 0 is the first piece of block blockIdx.x + i.
-    auto row_of = [&](int i) {
-      return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : j.slot0) * R + r;
-    };
-    float mx = -INFINITY;
+  const int lane = threadIdx.x & 31, row = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7;
+  const int r = blockIdx.y * 4 + row;
+  if (j.parts <= 0 || (int)blockIdx.y * 4 >= j.rows) return;  // the whole block
+  const bool live = r < j.rows;
+  // Part i > 0 is the first piece of block blockIdx.x + i.
+  auto row_of = [&](int i) {
+    return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : j.slot0) * R + r;
+  };
+  float mx = -INFINITY, l = 0.0f, o[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) o[k] = 0.0f;
+  if (live) {
     for (int i = lane; i < j.parts; i += 32) mx = fmaxf(mx, a.part_ml[row_of(i)].x);
     for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
     const float mu = mx == -INFINITY ? 0.0f : mx;
-    float l = 0.0f, o[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) o[k] = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < j.parts; ++i) {
+#pragma unroll 4
+    for (int i = part; i < j.parts; i += 4) {
       const float2 ml = a.part_ml[row_of(i)];
       const float c = exp2_approx(ml.x - mu);
       l += ml.y * c;
@@ -1180,11 +1249,24 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
         o[k + 1] += x.y * c;
       }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t at = out_row(a, j.first_token, j.head, j.row0 + r) * D + lane * V;
-#pragma unroll
-    for (int k = 0; k < V; k += 2) store_out(a, at + k, o[k] * inv, o[k + 1] * inv);
   }
+  if (part > 0) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[part - 1][row][lane][k] = o[k];
+    sum[part - 1][row][lane][V] = l;
+  }
+  __syncthreads();
+  if (part > 0 || !live) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] += sum[w][row][lane][k];
+    l += sum[w][row][lane][V];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = out_row(a, j.first_token, j.head, j.row0 + r) * D + lane * V;
+#pragma unroll
+  for (int k = 0; k < V; k += 2) store_out(a, at + k, o[k] * inv, o[k + 1] * inv);
 }
 
 // ------------------------------------------------------------------- host
@@ -1192,6 +1274,7 @@ __global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant_
 struct AttnPlan {
   int row_tiles;  // 16 * row_tiles rows a unit (1, 2, or 16: tensor memory)
   double tiles;   // the longest list
+  int unit_rows;  // rows that a unit holds at most
   int blocks;
   bool merge;     // a unit may be split over blocks
   size_t o_bytes, ml_bytes, bytes;
@@ -1204,6 +1287,7 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   const int64_t rows = a.blocks ? group : b.max_new * group;
   p.row_tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : 16);
   const int64_t r = 16 * p.row_tiles;
+  p.unit_rows = (int)(rows < r ? rows : r);
   const int64_t units = a.blocks ? b.max_new * ceil_div(group, r) : ceil_div(rows, r);
   int64_t keys = b.max_kv;
   if (a.blocks && a.max_blocks < ceil_div(keys, kv.page_size)) keys = a.max_blocks * kv.page_size;
@@ -1303,8 +1387,8 @@ static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
   // The merge is launched while the attention runs and waits on the device for
   // its end, which hides the launch.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)p.blocks, 4);
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)p.blocks, (unsigned)ceil_div(p.unit_rows, 4));
+  cfg.blockDim = dim3(512);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

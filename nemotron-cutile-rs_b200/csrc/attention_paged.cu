@@ -152,6 +152,7 @@ template <int R>
 struct Cursor {
   int b, unit, units, tiles, t;
   int left, at;  // tiles left to the block; list index of the next tile
+  int parts;     // blocks a unit is split over when it is known beforehand, else 0
   SeqView seq;
 
   // The next piece; false at the end of the block's share.  Every lane of a
@@ -274,8 +275,95 @@ __device__ __forceinline__ void find_share(const PagedAttn &a, Cursor<R> &share,
     const int off = (int)begin - at;
     c.unit = (int)((unsigned)off / (unsigned)c.tiles);
     c.t = off - c.unit * c.tiles;
+    c.parts = 0;
     share = c;
     *sh_per = per;
+  }
+  __syncthreads();
+}
+
+// A share of one piece: units split evenly over whole blocks, as many blocks
+// each as the shortest share allows that fits the grid.  Wide units (256 rows)
+// pay for every piece with a load of their queries and a pass of results
+// through memory, which weighs more than a perfect balance.  Falls back to
+// find_share when there are more units than blocks.  scratch: 2 * THREADS words
+// of shared memory.
+template <int R, int THREADS>
+__device__ __forceinline__ void find_piece(const PagedAttn &a, Cursor<R> &share, int *sh_per,
+                                           int *scratch) {
+  __shared__ int warp_total[THREADS / 32], best;
+  int *sh_units = scratch, *sh_tiles = scratch + THREADS;
+  const int n = a.batch.seqs;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (n > THREADS) {
+    find_share<R, THREADS>(a, share, sh_per);
+    return;
+  }
+  Cursor<R> c;
+  c.units = c.tiles = 0;
+  if ((int)threadIdx.x < n) seq_units<R>(a, threadIdx.x, c.seq, c.units, c.tiles, blockIdx.x == 0);
+  sh_units[threadIdx.x] = c.units;
+  sh_tiles[threadIdx.x] = c.tiles;
+  if (threadIdx.x == 0) {
+    best = 0x7fffffff;
+    share.left = 0;
+  }
+  __syncthreads();
+  // A warp tries a share length: blocks that it takes.
+  int total = 0, longest = 0, units = 0;
+  for (int b = lane; b < n; b += 32) {
+    total += sh_units[b] * sh_tiles[b];
+    units += sh_units[b];
+    longest = sh_tiles[b] > longest ? sh_tiles[b] : longest;
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  units = __reduce_add_sync(0xffffffffu, units);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (units > (int)gridDim.x) {  // the same in every warp
+    find_share<R, THREADS>(a, share, sh_per);
+    return;
+  }
+  const int least = (int)(((unsigned)total + gridDim.x - 1) / gridDim.x);
+  for (int x = least + warp; x < longest + THREADS / 32; x += THREADS / 32) {
+    int blocks = 0;
+    for (int b = lane; b < n; b += 32)
+      blocks += sh_units[b] * (int)(((unsigned)sh_tiles[b] + x - 1) / (unsigned)x);
+    blocks = __reduce_add_sync(0xffffffffu, blocks);
+    const bool fits = blocks <= (int)gridDim.x;
+    if (fits && lane == 0) atomicMin(&best, x);
+    __syncthreads();  // all warps make the same number of rounds
+    if (best != 0x7fffffff) break;
+    __syncthreads();
+  }
+  __syncthreads();
+  const int len = best;
+  int parts = 0, each = 0;
+  if (c.tiles > 0) {
+    parts = (c.tiles + len - 1) / len;
+    each = (c.tiles + parts - 1) / parts;
+    parts = (c.tiles + each - 1) / each;
+  }
+  const int sum = c.units * parts;
+  int scan = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) warp_total[warp] = scan;
+  __syncthreads();
+  int before = scan - sum;
+  for (int w = 0; w < warp; ++w) before += warp_total[w];
+  const int off = (int)blockIdx.x - before;
+  if (off >= 0 && off < sum) {
+    c.b = threadIdx.x;
+    c.unit = off / parts;
+    c.t = (off - c.unit * parts) * each;
+    c.left = c.tiles - c.t < each ? c.tiles - c.t : each;
+    c.at = 0;
+    c.parts = parts;
+    share = c;
+    *sh_per = each;
   }
   __syncthreads();
 }
@@ -324,7 +412,8 @@ template <int D, int R, int STAGES, bool SPLIT, int LIMITS>
 __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
                                            const CUtensorMap *kmap, const CUtensorMap *vmap,
                                            uint8_t *ring, uint64_t *full, uint64_t *empty,
-                                           int (*limits)[8], int *abort_flag) {
+                                           int (*limits)[8], int *abort_flag,
+                                           uint64_t *queries = nullptr) {
   constexpr int kTileBytes = kTile * D * 2;
   const int lane = threadIdx.x & 31;
   const int box_rows = a.pool.ps, npg = kTile >> a.pool.ps_log2;  // pages of a tile
@@ -370,6 +459,12 @@ __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
 #pragma unroll
       for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
         const int stage = SPLIT ? 2 * i + half : i, s = stage % STAGES;
+        // The ring's first fill would go ahead of the queries in the memory
+        // system, and nothing starts without them.  (No second phase of this
+        // barrier can begin before the first values are loaded.)
+        if (SPLIT && stage == 1 &&
+            !__all_sync(0xffffffffu, mbar_wait(queries, 0, abort_flag)))
+          return;
         const bool room = stage < STAGES ||
                           mbar_wait(&empty[s], ((stage / STAGES) - 1) & 1, abort_flag);
         if (!__all_sync(0xffffffffu, room)) return;  // the lanes leave together
@@ -798,7 +893,7 @@ __global__ void __launch_bounds__(288, 1)
 //   P          exp2 of the scaled scores, bf16, written over S,
 //   O += P V   P from tensor memory, V as it lies (MN-major), f32 in tensor memory.
 // Warps 0-3 turn A's scores into weights, a row a thread, warps 4-7 B's, warp 8
-// issues the products, warp 9 loads.  While one row tile's weights are computed
+// issues the products, warp 9 loads (10 and 11 fill the warp group).  While one row tile's weights are computed
 // the tensor cores work for the other: with both tiles a key tile costs 2 x 1024
 // tensor cycles and 2 x 1024 cycles of exponentials side by side.
 // The running maximum moves only when it grows by more than 2^8 (weights stay
@@ -811,7 +906,11 @@ struct TcCfg {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQBytes = 2 * 128 * D * 2;
   static constexpr int kSmem = kStages * kTileBytes + kQBytes + 1024;
-  static constexpr int kThreads = 320;
+  static constexpr int kThreads = 384;
+  // Registers a thread, launched with 65536 / 384 -> 168: the two weight groups
+  // take 216, the group of the other warps gives up all but 72 (2 * 216 + 72 =
+  // 3 * 168), so a row's 128 scores stay in registers.
+  static constexpr int kWeightRegs = 216, kOtherRegs = 72;
   static constexpr uint32_t kO = 256;  // tensor memory columns: S/P A, S/P B, O A, O B
 };
 
@@ -821,7 +920,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int *ab
 }
 
 template <int D>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(384, 1)
     paged_attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap,
                          const __grid_constant__ PagedAttn a) {
@@ -864,21 +963,25 @@ __global__ void __launch_bounds__(320, 1)
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  find_share<R, C::kThreads>(a, share, &per);
-  if (share.left <= 0) return;
-  Cursor<R> cur = share;
   if (warp == 8) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  find_piece<R, C::kThreads>(a, share, &per, reinterpret_cast<int *>(qs));
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  if (share.left <= 0) {
+    if (warp == 8) tmem_dealloc(tmem_slot, 512);
+    return;
+  }
+  Cursor<R> cur = share;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
-  if (warp == 9) {
+  if (warp >= 8) {
+   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+   if (warp == 9) {
     load_tiles<D, R, STAGES, true, C::kLimits>(a, cur, &kmap, &vmap, ring, full, empty, limits,
-                                               &abort_flag);
+                                               &abort_flag, &q_full[0]);
     if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
   } else if (warp == 8) {
     // --------------------------------------------------------------- products
@@ -889,23 +992,31 @@ __global__ void __launch_bounds__(320, 1)
     int tiles[2] = {};   // tiles of A / B so far
     bool live = true;
     Piece p;
-    auto scores = [&](int g, int tile) {  // lane 0
-      const uint32_t q = smem_u32(qs + g * (128 * D * 2));
-      const uint32_t k = smem_u32(ring + (2 * tile) % STAGES * C::kTileBytes);
+    // The whole warp walks through the products (one lane is elected to issue
+    // each), so that descriptors stay in uniform registers: under a branch on
+    // the lane a product cost 90 to 180 cycles to issue, more than it takes.
+    const uint64_t dk = smem_desc_sw128(smem_u32(ring));
+    const uint64_t dv = smem_desc_sw128_mn(smem_u32(ring), kTile * 128);
+    const uint64_t dq = smem_desc_sw128(smem_u32(qs));
+    auto scores = [&](int g, int tile) {
+      const uint32_t q = (uint32_t)dq + g * (128 * D * 2 >> 4);
+      const uint32_t k = (uint32_t)dk + (2 * tile) % STAGES * (C::kTileBytes >> 4);
 #pragma unroll
       for (int x = 0; x < D / 16; ++x) {
-        const uint32_t off = (x >> 2) * (128 * 128) + (x & 3) * 32;
-        tc_mma_bf16(tmem + g * 128, smem_desc_sw128(q + off), smem_desc_sw128(k + off), idesc_s,
-                    x > 0);
+        const uint32_t off = ((x >> 2) * (128 * 128) + (x & 3) * 32) >> 4;
+        tc_mma_bf16_warp(tmem + g * 128, q + off, (uint32_t)(dq >> 32), k + off,
+                         (uint32_t)(dk >> 32), idesc_s, x > 0);
       }
-      tc_commit(&s_full[g]);
+      tc_commit_warp(&s_full[g]);
     };
-    auto values = [&](int g, int half, int tile, bool more) {  // lane 0
-      const uint32_t v = smem_u32(ring + (2 * tile + 1) % STAGES * C::kTileBytes);
+    auto values = [&](int g, int half, int tile, bool more) {
+      const uint32_t v = (uint32_t)dv + (2 * tile + 1) % STAGES * (C::kTileBytes >> 4) +
+                         half * (kTile / 2 * 128 >> 4);
+      const uint32_t o = tmem + C::kO + g * 128, w = tmem + g * 128 + half * 32;
 #pragma unroll
-      for (int x = half * (kTile / 32); x < (half + 1) * (kTile / 32); ++x)
-        tc_mma_bf16_ta(tmem + C::kO + g * 128, tmem + g * 128 + x * 8,
-                       smem_desc_sw128_mn(v + x * 2048, kTile * 128), idesc_o, more || x > 0);
+      for (int x = 0; x < kTile / 32; ++x)
+        tc_mma_bf16_ta_warp(o, w + x * 8, v + x * (2048 >> 4), (uint32_t)(dv >> 32), idesc_o,
+                            (uint32_t)more + x);
     };
     auto loaded = [&](int stage) {
       return warp_wait(&full[stage % STAGES], (stage / STAGES) & 1, &abort_flag);
@@ -919,10 +1030,8 @@ __global__ void __launch_bounds__(320, 1)
       live = live && loaded(2 * i);
       if (!live) break;
       tc_fence_after();
-      if (lane == 0) {
-        for (int g = 0; g < groups; ++g) scores(g, i);
-        tc_commit(&empty[(2 * i) % STAGES]);
-      }
+      for (int g = 0; g < groups; ++g) scores(g, i);
+      tc_commit_warp(&empty[(2 * i) % STAGES]);
       for (int x = 0; live && x < n; ++x) {
         const int tile = i + x;
         const bool again = x + 1 < n;
@@ -932,35 +1041,33 @@ __global__ void __launch_bounds__(320, 1)
           live = warp_wait(&p_full[g][0], tiles[g] & 1, &abort_flag) && loaded(2 * tile + 1);
           if (!live) break;
           tc_fence_after();
-          if (lane == 0) values(g, 0, tile, x > 0);
-          __syncwarp();
+          values(g, 0, tile, x > 0);
           live = warp_wait(&p_full[g][1], tiles[g] & 1, &abort_flag);
           if (live && again) live = loaded(2 * tile + 2);
           if (!live) break;
           ++tiles[g];
           tc_fence_after();
-          if (lane == 0) {
-            values(g, 1, tile, true);
-            if (g == groups - 1) tc_commit(&empty[(2 * tile + 1) % STAGES]);
-            if (again) scores(g, tile + 1);
-            else tc_commit(&o_full[g]);
-            if (again && g == groups - 1) tc_commit(&empty[(2 * tile + 2) % STAGES]);
-          }
-          __syncwarp();
+          values(g, 1, tile, true);
+          if (g == groups - 1) tc_commit_warp(&empty[(2 * tile + 1) % STAGES]);
+          if (again) scores(g, tile + 1);
+          else tc_commit_warp(&o_full[g]);
+          if (again && g == groups - 1) tc_commit_warp(&empty[(2 * tile + 2) % STAGES]);
         }
       }
       for (int g = 0; g < groups; ++g) ++pieces[g];
       i += n;
     }
     if (*(volatile int *)&abort_flag) {  // products in flight end before the memory goes
-      if (lane == 0) tc_commit(&drain);
       __syncwarp();
+      tc_commit_warp(&drain);
       const uint64_t start = nk_globaltimer();
       while (!mbar_try_wait(&drain, 0) && nk_globaltimer() - start < 10000000ull) {
       }
     }
+   }
   } else {
     // ---------------------------------------------------------------- weights
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kWeightRegs));
     const int g = warp >> 2;
     const int r = threadIdx.x;  // row of the unit
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -1084,17 +1191,7 @@ __global__ void __launch_bounds__(320, 1)
             m = mn;
             l *= corr;
           }
-          if (t > p.t0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              float v[16];
-              tmem_ld16(to + c * 16, v);
-              uint32_t w[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j] * corr);
-              tmem_st16(to + c * 16, w);
-            }
-          }
+          const bool rescale = t > p.t0 && __any_sync(0xffffffffu, grow);
           const float mu = m == -INFINITY ? 0.0f : m;
           const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
           const float2 mu2 = make_float2(-mu, -mu);
@@ -1115,6 +1212,18 @@ __global__ void __launch_bounds__(320, 1)
                 w[j / 2] = pack_bf16(x.x, x.y);
               }
               tmem_st16(ts + c * 16, w);  // over scores that have been read
+            }
+            // O follows the maximum; here the first half's registers are free.
+            if (half == 0 && rescale) {
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                float v[16];
+                tmem_ld16(to + c * 16, v);
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[j] * corr);
+                tmem_st16(to + c * 16, w);
+              }
             }
             tmem_wait_st();
             tc_fence_before();
@@ -1193,7 +1302,8 @@ __global__ void __launch_bounds__(320, 1)
       if (threadIdx.x == 0 && p.first && !p.last) {
         MergeJob j{};
         j.slot0 = slot;
-        j.parts = (p.unit_at + cur.tiles - 1) / per - (int)blockIdx.x + 1;
+        j.parts = cur.parts ? cur.parts
+                            : (p.unit_at + cur.tiles - 1) / per - (int)blockIdx.x + 1;
         j.first_token = p.seq.first;
         j.row0 = p.row0;
         j.rows = p.rows;
@@ -1211,19 +1321,21 @@ __global__ void __launch_bounds__(320, 1)
 }
 
 // Joins the parts of the unit that begins in block blockIdx.x of the
-// attention, in their order.  A block takes 4 rows; the 4 warps of a row sum
-// every fourth part and meet in shared memory.
-template <int D>
+// attention, in their order.  SPLIT warps a row sum every SPLIT-th part and
+// meet in shared memory: 4 for units of few rows, whose parts are many, 1 for
+// wide units.
+template <int D, int SPLIT>
 __global__ void __launch_bounds__(512)
     paged_merge_kernel(const __grid_constant__ PagedAttn a, int R) {
-  constexpr int V = D / 32;
-  __shared__ float sum[3][4][32][V + 1];
+  constexpr int V = D / 32, ROWS = 16 / SPLIT;
+  __shared__ float sum[SPLIT > 1 ? SPLIT - 1 : 1][ROWS][32][V + 1];
   // Launched while the attention runs: nothing is read before it has ended.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const MergeJob j = a.jobs[blockIdx.x];
-  const int lane = threadIdx.x & 31, row = (threadIdx.x >> 5) & 3, part = threadIdx.x >> 7;
-  const int r = blockIdx.y * 4 + row;
-  if (j.parts <= 0 || (int)blockIdx.y * 4 >= j.rows) return;  // the whole block
+  const int lane = threadIdx.x & 31, row = (threadIdx.x >> 5) % ROWS;
+  const int part = threadIdx.x / (32 * ROWS);
+  const int r = blockIdx.y * ROWS + row;
+  if (j.parts <= 0 || (int)blockIdx.y * ROWS >= j.rows) return;  // the whole block
   const bool live = r < j.rows;
   // Part i > 0 is the first piece of block blockIdx.x + i.
   auto row_of = [&](int i) {
@@ -1237,7 +1349,7 @@ __global__ void __launch_bounds__(512)
     for (int k = 16; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, k));
     const float mu = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll 4
-    for (int i = part; i < j.parts; i += 4) {
+    for (int i = part; i < j.parts; i += SPLIT) {
       const float2 ml = a.part_ml[row_of(i)];
       const float c = exp2_approx(ml.x - mu);
       l += ml.y * c;
@@ -1250,19 +1362,22 @@ __global__ void __launch_bounds__(512)
       }
     }
   }
-  if (part > 0) {
+  if (SPLIT > 1) {
+    if (part > 0) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) sum[part - 1][row][lane][k] = o[k];
-    sum[part - 1][row][lane][V] = l;
+      for (int k = 0; k < V; ++k) sum[part - 1][row][lane][k] = o[k];
+      sum[part - 1][row][lane][V] = l;
+    }
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int w = 0; w < SPLIT - 1; ++w) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[k] += sum[w][row][lane][k];
+      l += sum[w][row][lane][V];
+    }
   }
-  __syncthreads();
-  if (part > 0 || !live) return;
-#pragma unroll
-  for (int w = 0; w < 3; ++w) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) o[k] += sum[w][row][lane][k];
-    l += sum[w][row][lane][V];
-  }
+  if (!live) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t at = out_row(a, j.first_token, j.head, j.row0 + r) * D + lane * V;
 #pragma unroll
@@ -1387,7 +1502,7 @@ static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
   // The merge is launched while the attention runs and waits on the device for
   // its end, which hides the launch.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)p.blocks, (unsigned)ceil_div(p.unit_rows, 4));
+  cfg.gridDim = dim3((unsigned)p.blocks, (unsigned)ceil_div(p.unit_rows, p.row_tiles > 2 ? 16 : 4));
   cfg.blockDim = dim3(512);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -1395,7 +1510,9 @@ static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_merge_kernel<D>, a, 16 * p.row_tiles));
+  NK_CUDA_TRY(p.row_tiles > 2
+                  ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, 1>, a, 16 * p.row_tiles)
+                  : cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, 4>, a, 16 * p.row_tiles));
   return ok();
 }
 

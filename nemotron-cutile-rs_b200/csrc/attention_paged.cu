@@ -388,12 +388,16 @@ __device__ __forceinline__ void store_out(const PagedAttn &a, int64_t at, float 
 //   values   warp w takes columns w*D/8 .. of the output over all 128 keys,
 // so an output lives in one place (D/8 columns a warp: 8 or 4 registers a row
 // tile), K, V and P are read from shared memory by whole tiles, and there is
-// nothing to join over the warps at the end but l.  A ninth warp loads.  One
-// block an SM with a ring of 192 KB, which covers HBM's latency several times.
+// nothing to join over the warps at the end but l.  A ninth warp loads.  Rings
+// of 192 KB an SM cover HBM's latency several times: one block with heads of
+// 128 (64 KB a tile, whose chain of three barriers is shorter than its load),
+// two with heads of 64, where a tile is half the bytes but the same chain (one
+// block: 46 us for 157 MB of block lists, two: see below).
 template <int D, int MT>
 struct Cfg {
   static constexpr int kRows = 16 * MT;
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kBlocks = D == 128 ? 1 : 2;  // of an SM
+  static constexpr int kStages = 3;
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kQBytes = kRows * D * 2;
@@ -596,7 +600,7 @@ __device__ __forceinline__ void compute_sync() {
 }
 
 template <int D, int MT>
-__global__ void __launch_bounds__(288, 1)
+__global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap,
                       const __grid_constant__ PagedAttn a) {
@@ -1407,9 +1411,10 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   int64_t keys = b.max_kv;
   if (a.blocks && a.max_blocks < ceil_div(keys, kv.page_size)) keys = a.max_blocks * kv.page_size;
   const int64_t tiles = ceil_div(ceil_div(keys, kv.page_size) * kv.page_size, kTile);
-  // One block an SM, or fewer when there are not as many tiles.
+  // As many blocks as are resident, or fewer when there are not as many tiles.
   p.tiles = (double)b.seqs * kv.kv_heads * units * tiles;
-  p.blocks = p.tiles < num_sms() ? (p.tiles < 1 ? 1 : (int)p.tiles) : num_sms();
+  const int most = num_sms() * (kv.head_dim == 64 && p.row_tiles <= 2 ? Cfg<64, 1>::kBlocks : 1);
+  p.blocks = p.tiles < most ? (p.tiles < 1 ? 1 : (int)p.tiles) : most;
   p.merge = tiles > 1;
   if (p.merge) {
     p.o_bytes = (size_t)2 * p.blocks * r * kv.head_dim * 4;

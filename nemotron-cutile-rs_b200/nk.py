@@ -284,7 +284,9 @@ def check(status: int) -> None:
 
 def call(name: str, *args) -> None:
     """Calls an nk_* entry point and raises NkError on a non-OK status."""
-    check(getattr(lib(), name)(*args))
+    status = getattr(_lib or lib(), name)(*args)
+    if status != OK:
+        raise NkError(last_error())
 
 
 # ----------------------------------------------------------------- torch glue
@@ -808,6 +810,13 @@ def attention_check(workspace, stream=None) -> int:
 
 
 # ------------------------------------------------------------- paged KV cache
+# The wrappers below are called several times a decode step, where the GPU work
+# of a call is a few microseconds: they look at each property of a tensor once
+# and leave the wording of refusals to the slow path.
+def _is(t, dtype, dim, device) -> bool:
+    return t.dtype is dtype and t.dim() == dim and t.device == device and t.stride(-1) == 1
+
+
 def _expect(t, name, dtype, dim, device=None):
     """A device tensor of the given type and rank whose last dimension is dense."""
     if t.dtype != dtype or t.dim() != dim:
@@ -824,7 +833,8 @@ def _expect(t, name, dtype, dim, device=None):
 def _expect_ints(t, name, n, device):
     import torch
 
-    _expect(t, name, torch.int32, 1, device)
+    if not _is(t, torch.int32, 1, device):
+        _expect(t, name, torch.int32, 1, device)
     if t.numel() != n:
         raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
 
@@ -894,6 +904,7 @@ class KvPages:
                                  table.shape[0], table.stride(0) if table.shape[0] > 1
                                  else table.shape[1])
         self._ref = ctypes.byref(self._struct)
+        self._bytes = {}  # bounds of an attention call -> its workspace bytes
 
     def batch(self, start, kv_len, tokens, max_new, max_kv=None, rows=None) -> NkKvBatch:
         """The ragged batch of one step (nk_kv_batch): start int32 [n + 1],
@@ -912,7 +923,8 @@ class KvPages:
     def _queries(self, q, q_heads):
         import torch
 
-        _expect(q, "q", torch.bfloat16, 2, self.device)
+        if not _is(q, torch.bfloat16, 2, self.device):
+            _expect(q, "q", torch.bfloat16, 2, self.device)
         tokens, width = q.shape
         if width != q_heads * self.head_dim:
             raise ValueError(f"q must be [tokens, {q_heads * self.head_dim}]")
@@ -928,11 +940,12 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
     import torch
 
     width = pages.kv_heads * pages.head_dim
-    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
-        _expect(t, name, torch.bfloat16, 2, pages.device)
-        if t.shape != (k_new.shape[0], width):
-            raise ValueError(f"{name} must be [tokens, {width}]")
     tokens = k_new.shape[0]
+    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
+        if not _is(t, torch.bfloat16, 2, pages.device):
+            _expect(t, name, torch.bfloat16, 2, pages.device)
+        if t.shape != (tokens, width):
+            raise ValueError(f"{name} must be [tokens, {width}]")
     b = pages.batch(start, kv_len, tokens, max_new, max_kv, rows)
     ld_k, ld_v = (k_new.stride(0), v_new.stride(0)) if tokens > 1 else (width, width)
     call("nk_kv_pages_append", pages._ref, layer, ctypes.byref(b), k_new.data_ptr(), ld_k,
@@ -1032,18 +1045,26 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
     if out is None:
         out = torch.empty(q.shape, device=dev,
                           dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
+        code = out_dtype
         _hold(stream, out)
     elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
+    else:
+        code = _dtype_code(out)
     a = NkPagedAttentionArgs(q.data_ptr(), ld_q, q_heads, ptr(tree_mask), ptr(blocks), max_blocks,
                              0 if scale is None else 1, 0.0 if scale is None else scale,
-                             out.data_ptr(), _dtype_code(out))
+                             out.data_ptr(), code)
     br, ar = ctypes.byref(b), ctypes.byref(a)
     size = 0
     if workspace is None:
-        need = ctypes.c_size_t(0)
-        call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
-        size = need.value
+        key = (tokens, b.seqs, q_heads, b.max_new, b.max_kv, max_blocks)
+        size = pages._bytes.get(key)
+        if size is None:
+            need = ctypes.c_size_t(0)
+            call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
+            if len(pages._bytes) > 4096:
+                pages._bytes.clear()
+            size = pages._bytes[key] = need.value
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=dev)
             _hold(stream, workspace)
@@ -1105,9 +1126,13 @@ def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspac
             raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
     br = ctypes.byref(b)
     if workspace is None:
-        need = ctypes.c_size_t(0)
-        call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        key = (tokens, b.max_kv)
+        size = pages._bytes.get(key)
+        if size is None:
+            need = ctypes.c_size_t(0)
+            call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
+            size = pages._bytes[key] = need.value
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
         _hold(stream, workspace)
     call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k, sink,
          local, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(dev, stream))

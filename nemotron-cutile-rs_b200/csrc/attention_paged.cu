@@ -44,6 +44,8 @@ struct PagedAttn {
   float *part_o;          // [2 * blocks][row tile][head_dim], unnormalised
   float2 *part_ml;        // [2 * blocks][row tile]: m (in log2 units), l
   struct MergeJob *jobs;  // [blocks]
+  int cluster, units_most;  // clusters of blocks share a unit (see below): their
+                            // size, and the units a sequence has at most
   int *err;
 };
 
@@ -90,6 +92,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "l"(*reinterpret_cast<const unsigned long long *>(&a)),
         "l"(*reinterpret_cast<const unsigned long long *>(&b)));
   return d;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -599,7 +606,11 @@ __device__ __forceinline__ void compute_sync() {
   asm volatile("bar.sync 1, 256;" ::: "memory");
 }
 
-template <int D, int MT>
+// CLUSTER: few units of few tiles (a short context, a small batch) run without a
+// list, a workspace and a merge launch: a cluster of blocks takes a unit, a
+// block each an even run of its tiles, and the blocks join through distributed
+// shared memory.
+template <int D, int MT, bool CLUSTER>
 __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap,
                       const __grid_constant__ CUtensorMap vmap,
@@ -635,9 +646,27 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  find_share<R, C::kThreads>(a, share, &per);
-  if (share.left <= 0) return;
-  Cursor<R> cur = share;
+  Cursor<R> cur;
+  if (CLUSTER) {
+    cur.b = blockIdx.x / (a.cluster * a.units_most);
+    cur.unit = blockIdx.x / a.cluster - cur.b * a.units_most;
+    seq_units<R>(a, cur.b, cur.seq, cur.units, cur.tiles,
+                 cur.unit == 0 && blockIdx.x % a.cluster == 0 && threadIdx.x == 0);
+    if (cur.unit >= cur.units) return;  // the whole cluster
+    const int each = (cur.tiles + a.cluster - 1) / a.cluster;
+    cur.t = (int)(blockIdx.x % a.cluster) * each;
+    cur.left = cur.tiles - cur.t < each ? cur.tiles - cur.t : each;
+    cur.at = cur.parts = 0;
+    __syncthreads();
+  } else {
+    find_share<R, C::kThreads>(a, share, &per);
+    if (share.left <= 0) return;
+    cur = share;
+  }
+  const Cursor<R> start = cur;
+  // CLUSTER: this block's part, over the ring once its tiles are used.
+  float *part_o = reinterpret_cast<float *>(smem);
+  float2 *part_ml = reinterpret_cast<float2 *>(smem + R * D * 4);
 
   if (warp == 8) {
     load_tiles<D, R, STAGES, false, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits, &abort_flag);
@@ -856,7 +885,13 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
           float sum = 0.0f;
 #pragma unroll
           for (int w = 0; w < 8; ++w) sum += red[r][w];
-          if (whole) {
+          if (CLUSTER) {
+            if (warp == 0 && (lane & 3) == 0) part_ml[r] = make_float2(m[mt][hh], sum);
+#pragma unroll
+            for (int n = 0; n < ON; ++n)
+              *reinterpret_cast<float2 *>(part_o + r * D + warp * COLS + n * 8 + qc) =
+                  make_float2(o[mt][n][2 * hh], o[mt][n][2 * hh + 1]);
+          } else if (whole) {
             const int64_t at =
                 out_row(a, p.seq.first, p.head, p.row0 + r) * D + warp * COLS + qc;
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -872,7 +907,7 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
                   make_float2(o[mt][n][2 * hh], o[mt][n][2 * hh + 1]);
           }
         }
-      if (threadIdx.x == 0 && p.first && !p.last) {
+      if (!CLUSTER && threadIdx.x == 0 && p.first && !p.last) {
         MergeJob j{};
         j.slot0 = slot;
         j.parts = (p.unit_at + cur.tiles - 1) / per - (int)blockIdx.x + 1;
@@ -885,8 +920,50 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
       ++piece;
       compute_sync();  // red and odd are read before the next piece writes them
     }
+    if (CLUSTER && start.left <= 0 && threadIdx.x < R)
+      part_ml[threadIdx.x] = make_float2(-INFINITY, 0.0f);
   }
-  __syncthreads();
+  if (CLUSTER) {
+    // Rows rank, rank + cluster, .. are joined here, a column a thread, from the
+    // parts of all blocks in their order.
+    Cursor<R> any = start;  // the unit's rows, whatever this block's tiles
+    any.t = 0;
+    any.left = 1;
+    Piece p;
+    any.next(a, p);
+    const int rank = (int)(blockIdx.x % a.cluster);
+    cluster_sync();
+    if (threadIdx.x < 256 && !abort_flag) {
+      const uint32_t mine_o = smem_u32(part_o), mine_ml = smem_u32(part_ml);
+      const int col = threadIdx.x % D;
+      for (int r = rank + a.cluster * (int)(threadIdx.x / D); r < p.rows;
+           r += a.cluster * (256 / D)) {
+        float mx = -INFINITY, sum = 0.0f, x = 0.0f;
+        for (int k = 0; k < a.cluster; ++k)
+          mx = fmaxf(mx, ld_cluster(mapa_cta(mine_ml + r * 8, k)));
+        const float mu = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll 4
+        for (int k = 0; k < a.cluster; ++k) {
+          const uint32_t ml = mapa_cta(mine_ml + r * 8, k);
+          const float lk = ld_cluster(ml + 4), c = exp2_approx(ld_cluster(ml) - mu);
+          const float ok = ld_cluster(mapa_cta(mine_o + (r * D + col) * 4, k));
+          if (lk != 0.0f) {  // else the block had no key: nothing is written there
+            sum += lk * c;
+            x += ok * c;
+          }
+        }
+        x *= sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t at = out_row(a, p.seq.first, p.head, p.row0 + r) * D + col;
+        if (a.out_f32)
+          static_cast<float *>(a.out)[at] = x;
+        else
+          static_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(x);
+      }
+    }
+    cluster_sync();  // the other blocks have read this one's part
+  } else {
+    __syncthreads();
+  }
   if (abort_flag && threadIdx.x == 0) report(a.err, NK_TIMEOUT);
 }
 
@@ -1396,6 +1473,8 @@ struct AttnPlan {
   int unit_rows;  // rows that a unit holds at most
   int blocks;
   bool merge;     // a unit may be split over blocks
+  int cluster;    // blocks that share a unit and join it among them, 0: a tile list
+  int units_most; // units of a sequence at most
   size_t o_bytes, ml_bytes, bytes;
 };
 
@@ -1415,6 +1494,19 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   p.tiles = (double)b.seqs * kv.kv_heads * units * tiles;
   const int most = num_sms() * (kv.head_dim == 64 && p.row_tiles <= 2 ? Cfg<64, 1>::kBlocks : 1);
   p.blocks = p.tiles < most ? (p.tiles < 1 ? 1 : (int)p.tiles) : most;
+  p.units_most = (int)(kv.kv_heads * units < (1 << 30) ? kv.kv_heads * units : 1 << 30);
+  // Clusters: when every unit gets a block for two of its tiles or fewer and all
+  // of them are resident at once.  (Clusters of 16 found no room side by side:
+  // 8 units of 32 tiles took 22 us, as a list 11 us and 4 for the merge.)
+  if (p.row_tiles <= 2 && tiles <= 16) {
+    int c = 1;
+    while (c < 8 && c < tiles) c *= 2;
+    if ((double)b.seqs * p.units_most * c <= most) {
+      p.cluster = c;
+      p.blocks = (int)b.seqs * p.units_most * c;
+      return p;
+    }
+  }
   p.merge = tiles > 1;
   if (p.merge) {
     p.o_bytes = (size_t)2 * p.blocks * r * kv.head_dim * 4;
@@ -1488,21 +1580,46 @@ static nk_status launch_attention(Kernel kernel, int smem, int threads,
                                   cudaStream_t s) {
   nk_status st = allow_smem(reinterpret_cast<const void *>(kernel), smem, prepared);
   if (st != NK_OK) return st;
-  kernel<<<p.blocks, threads, smem, s>>>(km, vm, a);
-  return check_launch("paged attention");
+  if (!p.cluster) {
+    kernel<<<p.blocks, threads, smem, s>>>(km, vm, a);
+    return check_launch("paged attention");
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)p.blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)p.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, km, vm, a));
+  return ok();
+}
+
+template <int D, int MT>
+static nk_status launch_rows(const CUtensorMap &km, const CUtensorMap &vm, const PagedAttn &a,
+                             const AttnPlan &p, cudaStream_t s) {
+  using C = Cfg<D, MT>;
+  static std::atomic<uint64_t> list{0}, clusters{0};  // a bit per device
+  if (!p.cluster)
+    return launch_attention(paged_attn_kernel<D, MT, false>, C::kSmem, C::kThreads, list, km, vm,
+                            a, p, s);
+  return launch_attention(paged_attn_kernel<D, MT, true>, C::kSmem, C::kThreads,
+                          clusters, km, vm, a, p, s);
 }
 
 template <int D>
 static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
                                   const PagedAttn &a, const AttnPlan &p, cudaStream_t s) {
-  static std::atomic<uint64_t> prepared[3];  // a bit per device
-  nk_status st =
-      p.row_tiles == 1 ? launch_attention(paged_attn_kernel<D, 1>, Cfg<D, 1>::kSmem,
-                                          Cfg<D, 1>::kThreads, prepared[0], km, vm, a, p, s)
-      : p.row_tiles == 2 ? launch_attention(paged_attn_kernel<D, 2>, Cfg<D, 2>::kSmem,
-                                            Cfg<D, 2>::kThreads, prepared[1], km, vm, a, p, s)
+  static std::atomic<uint64_t> prepared{0};
+  const nk_status st =
+      p.row_tiles == 1   ? launch_rows<D, 1>(km, vm, a, p, s)
+      : p.row_tiles == 2 ? launch_rows<D, 2>(km, vm, a, p, s)
                          : launch_attention(paged_attn_tc_kernel<D>, TcCfg<D>::kSmem,
-                                            TcCfg<D>::kThreads, prepared[2], km, vm, a, p, s);
+                                            TcCfg<D>::kThreads, prepared, km, vm, a, p, s);
   if (st != NK_OK || !p.merge) return st;
   // The merge is launched while the attention runs and waits on the device for
   // its end, which hides the launch.
@@ -1572,6 +1689,8 @@ nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.scale_log2 = sc * 1.44269504088896340736f;
   a.out = args->out;
   a.out_f32 = args->out_dtype == NK_DTYPE_F32;
+  a.cluster = p.cluster;
+  a.units_most = p.units_most;
   if (p.merge) {
     uint8_t *w = static_cast<uint8_t *>(workspace);
     a.part_o = reinterpret_cast<float *>(w);

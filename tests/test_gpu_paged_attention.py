@@ -79,9 +79,12 @@ def test_matches_the_formula(cuda, ps, d, kv, group, lens, counts, kind):
         words.append(w)
     tree = torch.from_numpy(np.concatenate(words)).cuda() if kind == "tree" else None
     want, mag = _reference(c, q, counts, H, kind, masks)
-    for dt in (nk.BF16, nk.F32):
+    # close bounds (short contexts: a cluster of blocks a unit) and loose ones (a
+    # list of tiles that is split anywhere)
+    for dt, max_kv in ((nk.BF16, max(lens)), (nk.F32, max(lens)), (nk.BF16, 20000),
+                       (nk.F32, 20000)):
         got = nk.attention_paged(dev(q.reshape(T, H * d)).bfloat16(), pages, ints(starts(counts)),
-                                 ints(lens), H, max_q=max(counts), max_kv=max(lens),
+                                 ints(lens), H, max_q=max(counts), max_kv=max_kv,
                                  tree_mask=tree, out_dtype=dt)
         nk.device_status()
         _close(got, want, mag, dt == nk.F32)
@@ -263,15 +266,15 @@ def test_captured_and_on_another_stream(cuda, lens, T, H, kv):
 def test_explicit_workspace(cuda):
     c = Paged(4, [3000], 2, 64, 64)
     pages, q = c.device(), torch.randn(1, 256, device="cuda").bfloat16()
-    need = nk.attention_paged_workspace_bytes(pages, 1, 1, 4, max_q=1, max_kv=3000)
+    need = nk.attention_paged_workspace_bytes(pages, 1, 1, 4, max_q=1, max_kv=9000)
     assert need > 0
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
     args = (q, pages, ints([0, 1]), ints([3000]), 4)
-    a = nk.attention_paged(*args, max_q=1, max_kv=3000, workspace=ws)
-    b = nk.attention_paged(*args, max_q=1, max_kv=3000)
+    a = nk.attention_paged(*args, max_q=1, max_kv=9000, workspace=ws)
+    b = nk.attention_paged(*args, max_q=1, max_kv=9000)
     assert torch.equal(a, b)
     with pytest.raises(nk.NkError) as e:
-        nk.attention_paged(*args, max_q=1, max_kv=3000, workspace=ws[:need - 16])
+        nk.attention_paged(*args, max_q=1, max_kv=9000, workspace=ws[:need - 16])
     assert e.value.code == nk.WORKSPACE_TOO_SMALL
 
 

@@ -84,83 +84,103 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// Block = (64 eligible blocks x, KV head y, token z): a lane holds a block and a
-// warp a quarter of the channels of 32 blocks, so that a query value is one
-// broadcast read of shared memory for 32 blocks; HEADS query heads at a time.
+// Block = (128 eligible blocks x, KV head y, token z): each of 8 warps takes an
+// eighth of the channels, a lane 4 blocks, so that a query value is one
+// broadcast read of shared memory for 128 blocks (a broadcast moves 4 bytes a
+// cycle: with a block a lane those reads took 12000 cycles, 6 us); HEADS query
+// heads at a time.
 //   s_g = sum_c max(q, 0) * k_max + min(q, 0) * k_min   (f32 FMAs)
 //   A   = sum_c max_g|q| * max(|k_min|, |k_max|)        >= sum of any head's |terms|
-// A lane adds D/4 terms (the other product of a channel is 0) and the quarters
-// are joined in two more steps, each off by at most 2^-24 of a partial sum,
-// itself at most A: |s_g - score| <= (D/4 + 2) * 2^-24 A.  The interval takes
-// (D/4 + 6) * 2^-24 A: one more covers the roundings of its own ends, another
-// the relative error of A ((D/4 + 3) * 2^-24, times D/4 + 2), and 1e-38 results
+// A lane adds D/8 terms (the other product of a channel is 0) and the eighths
+// are joined in three more steps, each off by at most 2^-24 of a partial sum,
+// itself at most A: |s_g - score| <= (D/8 + 3) * 2^-24 A.  The interval takes
+// (D/8 + 7) * 2^-24 A: one more covers the roundings of its own ends, another
+// the relative error of A ((D/8 + 4) * 2^-24, times D/8 + 3), and 1e-38 results
 // that underflow.  Where a sum is not finite (0 * inf is NaN here, not in the
 // definition) the interval is everything.
-// The loop is not unrolled beyond a 16-byte word of bounds: a warp runs through
-// it a few times only, and straight-line code of this kernel spent its time on
+// The loop is not unrolled beyond two channels: a warp runs through it a few
+// times only, and straight-line code of this kernel spent its time on
 // instruction fetch.
+constexpr int kScoreBlocks = 128, kScoreWarps = 8;
+
 template <int D>
 struct ScoreShared {
-  static constexpr int kRow = D * 2 + 16;  // bytes of a block's bounds: 16 apart in banks
-  static constexpr int kBounds = 2 * 64 * kRow;
-  static constexpr int kSums = 4 * 64 * 4;  // a pass's head: [quarter][block] f32
-  static size_t bytes(int64_t wide) {
-    return (size_t)kBounds + (size_t)wide * D * 8 + D * 4 + (size_t)wide * kSums + kSums;
+  static constexpr int kRow = D * 2 + 4;  // bytes of a block's bounds: 4 apart in banks
+  static constexpr int kBounds = 2 * kScoreBlocks * kRow;
+  static constexpr int kSums = kScoreWarps * kScoreBlocks * 4;  // of a head: [warp][block] f32
+  static size_t bytes(int64_t wide, int heads) {
+    return (size_t)kBounds + (size_t)wide * D * 8 + D * 4 + (size_t)(heads + 1) * kSums;
   }
 };
 
 template <int D, int HEADS>
-__global__ void __launch_bounds__(256) block_scores_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const SelectArgs a) {
   using S = ScoreShared<D>;
+  constexpr int NB = kScoreBlocks / 32;  // blocks of a lane
+  constexpr int C = D / 8;               // 16-byte words of a row
+  constexpr int T = 32 * kScoreWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   const int wide = (a.group + HEADS - 1) / HEADS * HEADS;
   float4 *qs = reinterpret_cast<float4 *>(smem + S::kBounds);  // [D][wide/2]: q+ of two heads, q- of both
   float *qm = reinterpret_cast<float *>(qs + D * wide / 2);    // [D]: max_g |q|
-  float *sums = qm + D;                                        // [wide + 1][quarter][block]
+  float *sums = qm + D;                                        // [HEADS + 1][warp][block]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // The first 8 channels of this thread's queries are on their way while the
+  // sequence is found.
+  const uint4 *q =
+      reinterpret_cast<const uint4 *>(a.q + blockIdx.z * a.ld_q + (int64_t)h * a.group * D);
+  uint4 qw = make_uint4(0, 0, 0, 0);
+  if ((int)threadIdx.x < a.group * C) qw = q[threadIdx.x];
   Query x;
   if (!find_query(a, blockIdx.z, x, threadIdx.x == 0)) return;
   if (x.blocks <= a.top_k) return;  // every block is taken
-  const int first = blockIdx.x * 64;
+  const int first = blockIdx.x * kScoreBlocks;
   // the forced blocks need no score
-  if (first >= x.blocks - a.local || first + 64 <= a.sink) return;
-  const int h = blockIdx.y;
-  // Bounds: a warp copies 8 blocks' rows (whole 128- or 256-byte rows a load).
+  if (first >= x.blocks - a.local || first + kScoreBlocks <= a.sink) return;
+  // Bounds: a warp copies the rows of 16 blocks, whole 128- or 256-byte rows a
+  // load.  (Rows lie 4 bytes past a multiple of 128: words go in by fours.)
   {
-    constexpr int C = D / 8;  // 16-byte words of a row
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int mine = first + warp * 8 + (lane & 7);
+    constexpr int ROWS = kScoreBlocks / kScoreWarps;
+    const int mine = first + warp * ROWS + lane % ROWS;
     int page = -1;
     if (mine >= a.sink && mine < x.blocks - a.local) {
       page = x.seq.table[mine];
       if (!page_ok(a.pool, page)) {
-        if (lane < 8) report(a.err, NK_PAGE_OUT_OF_RANGE);
+        report(a.err, NK_PAGE_OUT_OF_RANGE);
         page = -1;
       }
     }
 #pragma unroll
-    for (int r = 0; r < 8; r += 32 / C) {
+    for (int r = 0; r < ROWS; r += 32 / C) {
       const int row = r + lane / C;
       const int pg = __shfl_sync(0xffffffffu, page, row);
       const int64_t at = ((int64_t)(pg < 0 ? 0 : pg) * a.pool.heads + h) * C + lane % C;
-      uint8_t *to = smem + (warp * 8 + row) * S::kRow + (lane % C) * 16;
-      *reinterpret_cast<uint4 *>(to) = reinterpret_cast<const uint4 *>(a.k_min)[at];
-      *reinterpret_cast<uint4 *>(to + 64 * S::kRow) = reinterpret_cast<const uint4 *>(a.k_max)[at];
+      const uint4 lo = reinterpret_cast<const uint4 *>(a.k_min)[at];
+      const uint4 hi = reinterpret_cast<const uint4 *>(a.k_max)[at];
+      uint32_t *to = reinterpret_cast<uint32_t *>(smem + (warp * ROWS + row) * S::kRow) +
+                     (lane % C) * 4;
+      to[0] = lo.x, to[1] = lo.y, to[2] = lo.z, to[3] = lo.w;
+      to += kScoreBlocks * S::kRow / 4;
+      to[0] = hi.x, to[1] = hi.y, to[2] = hi.z, to[3] = hi.w;
     }
   }
-  const uint16_t *q = a.q + x.token * a.ld_q + (int64_t)h * a.group * D;
   bool odd = false;  // a NaN query is dropped by fmaxf and fminf
-#pragma unroll 4
-  for (int i = threadIdx.x; i < wide * D; i += 256) {
-    const int c = i / wide, g = i - c * wide;
-    const float v = g < a.group ? bf16_f32(q[g * D + c]) : 0.0f;
-    odd |= v != v;
-    float *to = reinterpret_cast<float *>(qs + c * (wide / 2) + g / 2) + (g & 1);
-    to[0] = fmaxf(v, 0.0f);
-    to[2] = fminf(v, 0.0f);
+  for (int i = threadIdx.x; i < wide * C; i += T) {
+    const int g = i / C, c = (i % C) * 8;
+    if (i >= T) qw = i < a.group * C ? q[i] : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {qw.x, qw.y, qw.z, qw.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float v = __uint_as_float((e & 1) ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+      odd |= v != v;
+      float *to = reinterpret_cast<float *>(qs + (c + e) * (wide / 2) + g / 2) + (g & 1);
+      to[0] = fmaxf(v, 0.0f);
+      to[2] = fminf(v, 0.0f);
+    }
   }
   odd = __syncthreads_or(odd);
-  for (int c = threadIdx.x; c < D; c += 256) {
+  for (int c = threadIdx.x; c < D; c += T) {
     const float4 *row = qs + c * (wide / 2);
     float mx = 0.0f;
 #pragma unroll 4
@@ -169,64 +189,87 @@ __global__ void __launch_bounds__(256) block_scores_kernel(const SelectArgs a) {
     qm[c] = mx;
   }
   __syncthreads();
-  const int part = (threadIdx.x >> 5) & 3;
-  const int b = (threadIdx.x & 31) + (threadIdx.x >> 7) * 32;  // block of this lane
-  const uint8_t *low_row = smem + b * S::kRow + part * (D / 2);
-  const uint8_t *high_row = low_row + 64 * S::kRow;
-  float mag = 0.0f;
+  const uint8_t *low_row = smem + lane * S::kRow + warp * (D / kScoreWarps * 2);
+  const int jb = threadIdx.x >> 1, j = first + jb;  // block of this thread's join
+  auto joined = [&](int g) {
+    const float *v = sums + g * kScoreWarps * kScoreBlocks + jb;
+    float s[kScoreWarps];
+#pragma unroll
+    for (int w = 0; w < kScoreWarps; ++w) s[w] = v[w * kScoreBlocks];
+    return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  };
+  float mag[NB], best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) mag[i] = 0.0f;
 #pragma unroll 1
   for (int g0 = 0; g0 < wide; g0 += HEADS) {
-    float2 acc[HEADS / 2];
+    float2 acc[NB][HEADS / 2];
 #pragma unroll
-    for (int g = 0; g < HEADS / 2; ++g) acc[g] = make_float2(0.0f, 0.0f);
-    const float4 *qc = qs + part * (D / 4) * (wide / 2) + g0 / 2;
-    const float *qa = qm + part * (D / 4);
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int g = 0; g < HEADS / 2; ++g) acc[i][g] = make_float2(0.0f, 0.0f);
+    const float4 *qc = qs + warp * (D / kScoreWarps) * (wide / 2) + g0 / 2;
+    const float *qa = qm + warp * (D / kScoreWarps);
 #pragma unroll 1
-    for (int i = 0; i < D / 32; ++i) {
-      const uint4 lo = *reinterpret_cast<const uint4 *>(low_row + i * 16);
-      const uint4 hi = *reinterpret_cast<const uint4 *>(high_row + i * 16);
-      const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w};
-      const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w};
+    for (int c = 0; c < D / kScoreWarps; c += 2) {
+      uint32_t lw[NB], hw[NB];
 #pragma unroll
-      for (int e = 0; e < 8; ++e, qc += wide / 2) {
-        const float l = __uint_as_float((e & 1) ? lw[e >> 1] & 0xffff0000u : lw[e >> 1] << 16);
-        const float u = __uint_as_float((e & 1) ? hw[e >> 1] & 0xffff0000u : hw[e >> 1] << 16);
+      for (int i = 0; i < NB; ++i) {
+        const uint8_t *at = low_row + i * 32 * S::kRow + c * 2;
+        lw[i] = *reinterpret_cast<const uint32_t *>(at);
+        hw[i] = *reinterpret_cast<const uint32_t *>(at + kScoreBlocks * S::kRow);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e, qc += wide / 2) {
+        float l[NB], u[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          l[i] = __uint_as_float(e ? lw[i] & 0xffff0000u : lw[i] << 16);
+          u[i] = __uint_as_float(e ? hw[i] & 0xffff0000u : hw[i] << 16);
+        }
 #pragma unroll
         for (int g = 0; g < HEADS / 2; ++g) {
           const float4 v = qc[g];
-          acc[g] = fma2(make_float2(v.x, v.y), make_float2(u, u), acc[g]);
-          acc[g] = fma2(make_float2(v.z, v.w), make_float2(l, l), acc[g]);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            acc[i][g] = fma2(make_float2(v.x, v.y), make_float2(u[i], u[i]), acc[i][g]);
+            acc[i][g] = fma2(make_float2(v.z, v.w), make_float2(l[i], l[i]), acc[i][g]);
+          }
         }
-        if (g0 == 0) mag = fmaf(qa[i * 8 + e], fmaxf(fabsf(l), fabsf(u)), mag);
+        if (g0 == 0) {
+          const float m = qa[c + e];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) mag[i] = fmaf(m, fmaxf(fabsf(l[i]), fabsf(u[i])), mag[i]);
+        }
       }
     }
 #pragma unroll
-    for (int g = 0; g < HEADS / 2; ++g) {
-      sums[((g0 + 2 * g) * 4 + part) * 64 + b] = acc[g].x;
-      sums[((g0 + 2 * g + 1) * 4 + part) * 64 + b] = acc[g].y;
+    for (int g = 0; g < HEADS / 2; ++g)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        float *to = sums + (2 * g * kScoreWarps + warp) * kScoreBlocks + i * 32 + lane;
+        to[0] = acc[i][g].x;
+        to[kScoreWarps * kScoreBlocks] = acc[i][g].y;
+      }
+    if (g0 == 0)
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+        sums[(HEADS * kScoreWarps + warp) * kScoreBlocks + i * 32 + lane] = mag[i];
+    __syncthreads();
+    // Join the eighths: two neighbouring threads a block, every other head each.
+    for (int g = threadIdx.x & 1; g < HEADS && g0 + g < a.group; g += 2) {
+      const float v = joined(g);
+      odd |= !(fabsf(v) < INFINITY);
+      best = fmaxf(best, v);
     }
-  }
-  sums[(wide * 4 + part) * 64 + b] = mag;
-  __syncthreads();
-  // Join the quarters; 4 threads a block take its heads in turn.
-  const int jb = threadIdx.x >> 2, j = first + jb;
-  auto joined = [&](int g) {
-    const float *v = sums + g * 256 + jb;
-    return (v[0] + v[64]) + (v[128] + v[192]);
-  };
-  float best = -INFINITY;
-  for (int g = threadIdx.x & 3; g < a.group; g += 4) {
-    const float v = joined(g);
-    odd |= !(fabsf(v) < INFINITY);
-    best = fmaxf(best, v);
+    if (g0 + HEADS < wide) __syncthreads();  // before the next pass writes its sums
   }
   best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-  best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-  const uint32_t odds = __ballot_sync(0xffffffffu, odd);
-  if ((threadIdx.x & 3) == 0 && j >= a.sink && j < x.blocks - a.local) {
-    const float e = fmaf(joined(wide), (D / 4 + 6) * 0x1p-24f, 1e-38f);
+  odd |= __shfl_xor_sync(0xffffffffu, (int)odd, 1) != 0;
+  if ((threadIdx.x & 1) == 0 && j >= a.sink && j < x.blocks - a.local) {
+    const float e = fmaf(joined(HEADS), (D / 8 + 7) * 0x1p-24f, 1e-38f);
     float2 r = make_float2(best - e, best + e);
-    if (((odds >> (threadIdx.x & 31)) & 15) || !(e < INFINITY)) r = make_float2(-INFINITY, INFINITY);
+    if (odd || !(e < INFINITY)) r = make_float2(-INFINITY, INFINITY);
     if (!page_ok(a.pool, x.seq.table[j])) r = make_float2(-INFINITY, -INFINITY);
     a.range[(x.token * a.pool.heads + h) * a.score_ld + j] = r;
   }
@@ -537,7 +580,7 @@ static nk_status launch_scores_heads(const SelectArgs &a, dim3 grid, cudaStream_
                             227 * 1024, prepared);
   if (st != NK_OK) return st;
   const int64_t wide = ceil_div(a.group, HEADS) * HEADS;
-  block_scores_kernel<D, HEADS><<<grid, 256, ScoreShared<D>::bytes(wide), s>>>(a);
+  block_scores_kernel<D, HEADS><<<grid, 32 * kScoreWarps, ScoreShared<D>::bytes(wide, HEADS), s>>>(a);
   return NK_OK;
 }
 
@@ -588,12 +631,13 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   }
   const int64_t group = q_heads / kv->kv_heads;
   if (group > 64) return fail(NK_UNSUPPORTED, "q_heads / kv_heads must be <= 64");
-  if (ld_q < q_heads * kv->head_dim)
-    return fail(NK_INVALID_PARAMS, "ld_q must be >= q_heads * head_dim");
+  if (ld_q < q_heads * kv->head_dim || ld_q % 8)
+    return fail(NK_INVALID_PARAMS, "ld_q must be a multiple of 8 and >= q_heads * head_dim");
   if (sink < 0 || local < 1 || top_k < sink + local || top_k > (1 << 20))
     return fail(NK_INVALID_PARAMS, "sink >= 0, local >= 1, sink + local <= top_k <= 2^20");
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0) return ok();
   if (!q || !blocks) return fail(NK_INVALID_PARAMS, "q and blocks are required");
+  if ((uintptr_t)q & 15) return fail(NK_INVALID_PARAMS, "q must be 16-byte aligned");
   const int64_t width = score_width(kv, batch);
   const size_t need = select_bytes(kv, batch);
   if (workspace_bytes < need || !workspace) {
@@ -623,7 +667,7 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   if (!a.err) return fail(NK_DEVICE_ERROR, "cannot resolve device error word");
   cudaStream_t s = as_stream(stream);
   if (width > top_k) {
-    const dim3 grid((unsigned)ceil_div(width, 64), (unsigned)kv->kv_heads,
+    const dim3 grid((unsigned)ceil_div(width, kScoreBlocks), (unsigned)kv->kv_heads,
                     (unsigned)batch->tokens);
     st = kv->head_dim == 128 ? launch_scores<128>(a, grid, s) : launch_scores<64>(a, grid, s);
     if (st != NK_OK) return st;

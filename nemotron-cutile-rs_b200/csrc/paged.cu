@@ -231,8 +231,9 @@ __device__ __forceinline__ int kept_position(const CompactSeq &c, int i, int *er
 }
 
 // Into other pages: block = (destination page x, head and layer y, sequence
-// z).  Tokens are independent, so a block's 128 threads gather a page's
-// tokens with all their loads in flight.
+// z).  Where each token comes from is looked up first, a thread a token (keep,
+// then the page table: two latencies for the page, not two for every few
+// tokens); the 128 threads then gather with all their loads in flight.
 template <int D>
 __global__ void __launch_bounds__(128)
     pages_compact_kernel(PagePool pool, CompactArgs args, uint4 *__restrict__ k,
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(128)
   constexpr int C = D / 8, LANES = 128 / C;
   __shared__ uint4 sh_lo[128], sh_hi[128];
   __shared__ int sh_any[128];
+  __shared__ int64_t sh_src[128];  // 16-byte word of the token's first channels, -1: none
   CompactSeq s;
   if (!load_compact(pool, args, blockIdx.z, s, err, threadIdx.x == 0)) return;
   const int end = s.base + s.n;
@@ -258,32 +260,53 @@ __global__ void __launch_bounds__(128)
   const int64_t lp = (int64_t)layer * pool.pages;
   const int c = threadIdx.x % C, lane = threadIdx.x / C;
   const int64_t unit = (lp + page) * pool.heads + h;
-  const int e = end - page0 < pool.ps ? end : page0 + pool.ps;
+  const int n = end - page0 < pool.ps ? end - page0 : pool.ps;  // tokens of the page
+  if ((int)threadIdx.x < n) {
+    const int t = page0 + (int)threadIdx.x;
+    int64_t src = -1;
+    if (t < s.base) {
+      src = -2;  // a token below base stays; it belongs to the page's bounds
+    } else {
+      const int from = kept_position(s, t - s.base, err);
+      if (from >= 0) {
+        const int fp = s.src[from >> pool.ps_log2];
+        if (page_ok(pool, fp))
+          src = (((lp + fp) * pool.heads + h) * pool.ps + (from & (pool.ps - 1))) * C;
+        else
+          report(err, NK_PAGE_OUT_OF_RANGE);
+      }
+    }
+    sh_src[threadIdx.x] = src;
+  }
+  __syncthreads();
   Bounds8 b;
   bool any = false;
-#pragma unroll 4
-  for (int t = page0 + lane; t < e; t += LANES) {
-    const int64_t dst = (unit * pool.ps + (t - page0)) * C + c;
-    uint4 kx;
-    if (t >= s.base) {
-      const int from = kept_position(s, t - s.base, err);
-      if (from < 0) continue;
-      const int fp = s.src[from >> pool.ps_log2];
-      if (!page_ok(pool, fp)) {
-        report(err, NK_PAGE_OUT_OF_RANGE);
-        continue;
+#pragma unroll 1
+  for (int t0 = lane; t0 < n; t0 += 4 * LANES) {
+    uint4 kx[4], vx[4];
+    int64_t src[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = t0 + u * LANES;
+      src[u] = t < n ? sh_src[t] : -1;
+      if (src[u] >= 0) {
+        kx[u] = k[src[u] + c];
+        vx[u] = v[src[u] + c];
+      } else if (src[u] == -2) {
+        kx[u] = k[(unit * pool.ps + t) * C + c];
       }
-      const int64_t src =
-          (((lp + fp) * pool.heads + h) * pool.ps + (from & (pool.ps - 1))) * C + c;
-      kx = k[src];
-      const uint4 vx = v[src];
-      k[dst] = kx;
-      v[dst] = vx;
-    } else {
-      kx = k[dst];  // a token below base stays; it belongs to the page's bounds
     }
-    if (any) b.add(kx); else b.set(kx);
-    any = true;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (src[u] == -1) continue;
+      const int64_t dst = (unit * pool.ps + t0 + u * LANES) * C + c;
+      if (src[u] >= 0) {
+        k[dst] = kx[u];
+        v[dst] = vx[u];
+      }
+      if (any) b.add(kx[u]); else b.set(kx[u]);
+      any = true;
+    }
   }
   if (k_min) write_bounds<D, 128>(b, any, k_min + unit * C, k_max + unit * C, sh_lo, sh_hi, sh_any);
 }

@@ -920,6 +920,33 @@ class KvPages:
         return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(),
                          None if rows is None else rows.data_ptr(), max_new, max_kv)
 
+    def _attend_bytes(self, b, q_heads, max_blocks):
+        """Workspace bytes of an attention call: its bounds alone decide."""
+        key = (b.tokens, b.seqs, q_heads, b.max_new, b.max_kv, max_blocks)
+        size = self._bytes.get(key)
+        if size is None:
+            # of the pointers only whether they are there is read
+            a = NkPagedAttentionArgs(None, q_heads * self.head_dim, q_heads, None,
+                                     16 if max_blocks else None, max_blocks, 0, 0.0, None, BF16)
+            need = ctypes.c_size_t(0)
+            call("nk_attention_paged_workspace_bytes", self._ref, ctypes.byref(b),
+                 ctypes.byref(a), ctypes.byref(need))
+            if len(self._bytes) > 4096:
+                self._bytes.clear()
+            size = self._bytes[key] = need.value
+        return size
+
+    def _select_bytes(self, b):
+        """Workspace bytes of kv_block_select."""
+        key = (b.tokens, b.seqs, b.max_new, b.max_kv)
+        size = self._bytes.get(key)
+        if size is None:
+            need = ctypes.c_size_t(0)
+            call("nk_kv_block_select_workspace_bytes", self._ref, ctypes.byref(b),
+                 ctypes.byref(need))
+            size = self._bytes[key] = need.value
+        return size
+
     def _queries(self, q, q_heads):
         import torch
 
@@ -1055,16 +1082,8 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
                              0 if scale is None else 1, 0.0 if scale is None else scale,
                              out.data_ptr(), code)
     br, ar = ctypes.byref(b), ctypes.byref(a)
-    size = 0
     if workspace is None:
-        key = (tokens, b.seqs, q_heads, b.max_new, b.max_kv, max_blocks)
-        size = pages._bytes.get(key)
-        if size is None:
-            need = ctypes.c_size_t(0)
-            call("nk_attention_paged_workspace_bytes", pages._ref, br, ar, ctypes.byref(need))
-            if len(pages._bytes) > 4096:
-                pages._bytes.clear()
-            size = pages._bytes[key] = need.value
+        size = pages._attend_bytes(b, q_heads, max_blocks)
         if size:
             workspace = torch.empty(size, dtype=torch.uint8, device=dev)
             _hold(stream, workspace)
@@ -1103,13 +1122,8 @@ def attention_paged_workspace_bytes(pages: KvPages, tokens: int, seqs: int, q_he
                                     max_q: int, max_kv: int, max_blocks: int = 0) -> int:
     """Scratch bytes of attention_paged for these bounds (max_blocks > 0: the
     form with block lists of that width)."""
-    b = NkKvBatch(seqs, tokens, 16, 16, 16, max_q, max_kv)  # only the bounds are read
-    a = NkPagedAttentionArgs(None, q_heads * pages.head_dim, q_heads, None,
-                             16 if max_blocks else None, max_blocks, 0, 0.0, None, BF16)
-    need = ctypes.c_size_t(0)
-    call("nk_attention_paged_workspace_bytes", pages._ref, ctypes.byref(b), ctypes.byref(a),
-         ctypes.byref(need))
-    return need.value
+    return pages._attend_bytes(NkKvBatch(seqs, tokens, 16, 16, 16, max_q, max_kv), q_heads,
+                               max_blocks)
 
 
 def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspace, stream):
@@ -1126,13 +1140,7 @@ def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspac
             raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
     br = ctypes.byref(b)
     if workspace is None:
-        key = (tokens, b.max_kv)
-        size = pages._bytes.get(key)
-        if size is None:
-            need = ctypes.c_size_t(0)
-            call("nk_kv_block_select_workspace_bytes", pages._ref, br, ctypes.byref(need))
-            size = pages._bytes[key] = need.value
-        workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+        workspace = torch.empty(pages._select_bytes(b), dtype=torch.uint8, device=dev)
         _hold(stream, workspace)
     call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k, sink,
          local, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(dev, stream))
@@ -1157,11 +1165,18 @@ def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k
                            layer: int = 0, scale=None, out_dtype=BF16, out=None, stream=None):
     """kv_block_select, then attention_paged over the chosen blocks; returns
     (out, blocks)."""
+    import torch
+
     tokens, ld_q = pages._queries(q, q_heads)
     b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
-    blocks = _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, None, None, stream)
-    return _attend(pages, q, ld_q, b, q_heads, None, blocks, layer, scale, out_dtype, out, None,
-                   stream), blocks
+    # One workspace for both: the selection is done with it when the attention starts.
+    size = max(pages._select_bytes(b), pages._attend_bytes(b, q_heads, top_k))
+    workspace = torch.empty(size, dtype=torch.uint8, device=pages.device)
+    _hold(stream, workspace)
+    blocks = _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, None, workspace,
+                     stream)
+    return _attend(pages, q, ld_q, b, q_heads, None, blocks, layer, scale, out_dtype, out,
+                   workspace, stream), blocks
 
 
 # ------------------------------------------------- decoder steps around projections

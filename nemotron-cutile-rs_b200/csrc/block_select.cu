@@ -108,8 +108,11 @@ struct ScoreShared {
   static constexpr int kRow = D * 2 + 4;  // bytes of a block's bounds: 4 apart in banks
   static constexpr int kBounds = 2 * kScoreBlocks * kRow;
   static constexpr int kSums = kScoreWarps * kScoreBlocks * 4;  // of a head: [warp][block] f32
+  // The sums of a pass lie over the bounds when it is the only one.
   static size_t bytes(int64_t wide, int heads) {
-    return (size_t)kBounds + (size_t)wide * D * 8 + D * 4 + (size_t)(heads + 1) * kSums;
+    const size_t sums = (size_t)(heads + 1) * kSums, queries = (size_t)wide * D * 8 + D * 4;
+    if (wide > heads) return kBounds + queries + sums;
+    return queries + (sums > (size_t)kBounds ? sums : (size_t)kBounds);
   }
 };
 
@@ -121,9 +124,12 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
   constexpr int T = 32 * kScoreWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   const int wide = (a.group + HEADS - 1) / HEADS * HEADS;
-  float4 *qs = reinterpret_cast<float4 *>(smem + S::kBounds);  // [D][wide/2]: q+ of two heads, q- of both
-  float *qm = reinterpret_cast<float *>(qs + D * wide / 2);    // [D]: max_g |q|
-  float *sums = qm + D;                                        // [HEADS + 1][warp][block]
+  float4 *qs = reinterpret_cast<float4 *>(smem);             // [D][wide/2]: q+ of two heads, q- of both
+  float *qm = reinterpret_cast<float *>(qs + D * wide / 2);  // [D]: max_g |q|
+  uint8_t *bounds = reinterpret_cast<uint8_t *>(qm + D);     // [low, high][block][kRow]
+  const bool once = wide == HEADS;                           // one pass
+  float *sums = reinterpret_cast<float *>(bounds + (once ? 0 : S::kBounds));
+                                                             // [HEADS + 1][warp][block]
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The first 8 channels of this thread's queries are on their way while the
@@ -158,7 +164,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
       const int64_t at = ((int64_t)(pg < 0 ? 0 : pg) * a.pool.heads + h) * C + lane % C;
       const uint4 lo = reinterpret_cast<const uint4 *>(a.k_min)[at];
       const uint4 hi = reinterpret_cast<const uint4 *>(a.k_max)[at];
-      uint32_t *to = reinterpret_cast<uint32_t *>(smem + (warp * ROWS + row) * S::kRow) +
+      uint32_t *to = reinterpret_cast<uint32_t *>(bounds + (warp * ROWS + row) * S::kRow) +
                      (lane % C) * 4;
       to[0] = lo.x, to[1] = lo.y, to[2] = lo.z, to[3] = lo.w;
       to += kScoreBlocks * S::kRow / 4;
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
     qm[c] = mx;
   }
   __syncthreads();
-  const uint8_t *low_row = smem + lane * S::kRow + warp * (D / kScoreWarps * 2);
+  const uint8_t *low_row = bounds + lane * S::kRow + warp * (D / kScoreWarps * 2);
   const int jb = threadIdx.x >> 1, j = first + jb;  // block of this thread's join
   auto joined = [&](int g) {
     const float *v = sums + g * kScoreWarps * kScoreBlocks + jb;
@@ -243,6 +249,7 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
         }
       }
     }
+    if (once) __syncthreads();  // the bounds are read
 #pragma unroll
     for (int g = 0; g < HEADS / 2; ++g)
 #pragma unroll
@@ -315,12 +322,12 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-constexpr int kTopThreads = 512, kTopWarps = kTopThreads / 32;
-
+template <int T>
 struct TopShared {
+  static constexpr int kWarps = T / 32;
   int hist[256];
-  u64 ends[2][kTopWarps];
-  int above[kTopWarps], equal[kTopWarps];
+  u64 ends[2][kWarps];
+  int above[kWarps], equal[kWarps];
   int digit, need, whole;
 };
 
@@ -346,13 +353,14 @@ __device__ __forceinline__ u64 warp_max(u64 v) {
 }
 
 // Sum over the block; ends with a barrier behind which `sh` may be reused.
+template <int T>
 __device__ __forceinline__ int block_sum(int v, int *sh) {
   v = __reduce_add_sync(0xffffffffu, v);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < kTopWarps; ++w) total += sh[w];
+  for (int w = 0; w < T / 32; ++w) total += sh[w];
   __syncthreads();
   return total;
 }
@@ -362,8 +370,8 @@ __device__ __forceinline__ int block_sum(int v, int *sh) {
 // smaller one does not (`whole`), or, when keys tie there, their value.  A pass
 // spreads the keys that are left over 256 bins between the smallest and the
 // largest of them, so one or two passes end most searches among a few thousand.
-template <typename K, typename At>
-__device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopShared &sh,
+template <typename K, int T, typename At>
+__device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopShared<T> &sh,
                                          bool &whole) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   K least = ~(K)0, most = 0;
@@ -381,10 +389,10 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
     sh.ends[0][warp] = least;
     sh.ends[1][warp] = most;
   }
-  if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < 256; i += T) sh.hist[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kTopWarps; ++w) {
+  for (int w = 0; w < T / 32; ++w) {
     least = (K)sh.ends[0][w] < least ? (K)sh.ends[0][w] : least;
     most = (K)sh.ends[1][w] > most ? (K)sh.ends[1][w] : most;
   }
@@ -426,7 +434,7 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
     least += (K)sh.digit << shift;
     need = sh.need;
     whole = sh.whole != 0;
-    if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < 256; i += T) sh.hist[i] = 0;
     __syncthreads();  // the shared words are read, the bins are empty
     if (whole || shift == 0) return least;
     most = least + (((K)1 << shift) - 1);
@@ -438,10 +446,11 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
 // upper ends reach L they are the list.  If not, with H the (need+1)-th largest
 // upper end, a block whose lower end is above H is in and those in between are
 // scored in 64 bits.  Then the list is written in ascending order: a warp holds
-// a contiguous run of blocks, 32 neighbours at a time.
-template <int D>
-__global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const SelectArgs a) {
-  __shared__ TopShared sh;
+// a contiguous run of blocks, 32 neighbours at a time.  T threads: 128 up to 1024
+// blocks (400 lists of 190: 16 us with 512, most of them idle), 512 beyond.
+template <int D, int T>
+__global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {
+  __shared__ TopShared<T> sh;
   Query x;
   if (!find_query(a, blockIdx.y, x, threadIdx.x == 0)) return;
   // Launched while the scores are computed: nothing of them is read before.
@@ -449,7 +458,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
   const int h = blockIdx.x, n = x.blocks;
   int32_t *out = a.blocks + (x.token * a.pool.heads + h) * (int64_t)a.top_k;
   if (n <= a.top_k) {
-    for (int i = threadIdx.x; i < a.top_k; i += kTopThreads) out[i] = i < n ? i : -1;
+    for (int i = threadIdx.x; i < a.top_k; i += T) out[i] = i < n ? i : -1;
     return;
   }
   const int64_t row = (x.token * a.pool.heads + h) * a.score_ld;
@@ -458,7 +467,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
   const int lo = a.sink, hi = n - a.local;  // free blocks
   const int need = a.top_k - a.sink - a.local;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int run = ((n + kTopThreads - 1) / kTopThreads) * 32;
+  const int run = ((n + T - 1) / T) * 32;
   const int j0 = warp * run + lane, j1 = (warp + 1) * run < n ? (warp + 1) * run : n;
   auto is_free = [&](int j) { return j >= lo && j < hi; };
   uint32_t low = 1, high = 0xffffffffu;
@@ -466,15 +475,15 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
   if (need > 0) {
     bool whole;
     // A `whole` result may lie below L: the blocks it keeps in play are more.
-    low = nth_largest<uint32_t>(
+    low = nth_largest<uint32_t, T>(
         j0, j1, [&](int j) { return is_free(j) ? order_key(range[j].x) : 0u; }, need, sh, whole);
     int reach = 0;
 #pragma unroll 4
     for (int j = j0; j < j1; j += 32) reach += is_free(j) && order_key(range[j].y) >= low;
-    settled = block_sum(reach, sh.above) == need;
+    settled = block_sum<T>(reach, sh.above) == need;
     if (!settled) {
       auto upper = [&](int j) { return is_free(j) ? order_key(range[j].y) : 0u; };
-      high = nth_largest<uint32_t>(j0, j1, upper, need + 1, sh, whole);
+      high = nth_largest<uint32_t, T>(j0, j1, upper, need + 1, sh, whole);
       // A whole result may lie below H, which is the smallest key that reaches it.
       uint32_t least = 0xffffffffu;
       for (int j = j0; j < j1; j += 32) {
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
       least = warp_min(least);
       if (lane == 0) sh.above[warp] = (int)least;
       __syncthreads();
-      for (int w = 0; w < kTopWarps; ++w)
+      for (int w = 0; w < T / 32; ++w)
         least = (uint32_t)sh.above[w] < least ? (uint32_t)sh.above[w] : least;
       high = least;
       __syncthreads();
@@ -511,11 +520,11 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
         if (b == j) exact[b] = v;  // read again by this thread only
       }
     }
-    const int left = need - block_sum(in, sh.above);
+    const int left = need - block_sum<T>(in, sh.above);
     bool whole = true;
     from = ~0ull;  // no score is that large (it would be a NaN's)
     if (left > 0)
-      from = nth_largest<u64>(
+      from = nth_largest<u64, T>(
           j0, j1, [&](int j) { return kind(j) == 2 ? order_key(exact[j]) : 0ull; }, left, sh,
           whole);
     ties = !whole;
@@ -542,7 +551,7 @@ __global__ void __launch_bounds__(kTopThreads, 2) block_topk_kernel(const Select
   __syncthreads();
   int at = 0, eq = 0, all_above = 0;  // before this warp's run
 #pragma unroll
-  for (int w = 0; w < kTopWarps; ++w) {
+  for (int w = 0; w < T / 32; ++w) {
     all_above += sh.above[w];
     if (w < warp) {
       at += sh.above[w];
@@ -676,15 +685,20 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)kv->kv_heads, (unsigned)batch->tokens);
-  cfg.blockDim = dim3(kTopThreads);
+  const bool small = width <= 1024;
+  cfg.blockDim = dim3(small ? 128 : 512);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = width > top_k ? 1 : 0;
-  NK_CUDA_TRY(kv->head_dim == 128 ? cudaLaunchKernelEx(&cfg, block_topk_kernel<128>, a)
-                                  : cudaLaunchKernelEx(&cfg, block_topk_kernel<64>, a));
+  if (kv->head_dim == 128)
+    NK_CUDA_TRY(small ? cudaLaunchKernelEx(&cfg, block_topk_kernel<128, 128>, a)
+                      : cudaLaunchKernelEx(&cfg, block_topk_kernel<128, 512>, a));
+  else
+    NK_CUDA_TRY(small ? cudaLaunchKernelEx(&cfg, block_topk_kernel<64, 128>, a)
+                      : cudaLaunchKernelEx(&cfg, block_topk_kernel<64, 512>, a));
   return ok();
 }
 

@@ -748,7 +748,7 @@ nk_status nk_kv_pages_append(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
 /* Copies page src_host[i] to page dst_host[i] in every layer: keys, values
  * and bounds (the copy before a write into a shared page; the partial page of
  * a fork).  Refused: ids outside the pool, a destination that appears twice
- * or is a source too. */
+ * or is a source too (index: the pair). */
 nk_status nk_kv_pages_copy(const nk_kv_pages *kv, const int32_t *src_host,
                            const int32_t *dst_host, int64_t count, void *stream);
 
@@ -769,7 +769,8 @@ nk_status nk_kv_table_write(int32_t *dst, int64_t dst_len, const int64_t *offset
  * dst_table NULL: in place (the accepted path of a draft tree closes up).
  * Otherwise the tokens go to the pages of dst_table [seqs, dst_ld] (a context
  * thinned into fresh pages); a page written must not be read as a source.
- * Refused entries (not ascending, past kv_len) leave their slot unwritten. */
+ * Refused entries (not ascending, past kv_len) leave their slot unwritten.
+ * A page that is written must belong to one sequence of the call only. */
 typedef struct nk_kv_compact_args {
   int64_t seqs;             /* <= 65535 */
   const int32_t *rows;      /* [seqs] table row of each sequence; NULL: row b */
@@ -825,7 +826,8 @@ nk_status nk_attention_paged(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
  *   k_max[c] : k_min[c]),
  * the largest q.k that the block's bounds allow, summed in 64 bits; equal
  * scores go to the lower block, NaN ranks last.  sink >= 0, local >= 1,
- * sink + local <= top_k.  Needs k_min and k_max. */
+ * sink + local <= top_k.  Needs k_min and k_max, at most 65535 tokens and 64
+ * query heads to a KV head; q 16-byte aligned, ld_q a multiple of 8. */
 nk_status nk_kv_block_select_workspace_bytes(const nk_kv_pages *kv, const nk_kv_batch *batch,
                                              size_t *bytes);
 nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_batch *batch,

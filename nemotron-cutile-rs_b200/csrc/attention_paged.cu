@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
   float2 *part_ml = reinterpret_cast<float2 *>(smem + R * D * 4);
 
   if (warp == 8) {
-    load_tiles<D, R, STAGES, false, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits, &abort_flag);
+    load_tiles<D, R, STAGES, false, STAGES>(a, cur, &kmap, &vmap, smem, full, empty, limits,
+                                            &abort_flag);
     if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
   } else {
     const int quad = lane >> 2, qc = (lane & 3) * 2;
@@ -973,10 +974,19 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
 //   S = Q K^T  128 x 128 x D, f32 in tensor memory,
 //   P          exp2 of the scaled scores, bf16, written over S,
 //   O += P V   P from tensor memory, V as it lies (MN-major), f32 in tensor memory.
-// Warps 0-3 turn A's scores into weights, a row a thread, warps 4-7 B's, warp 8
-// issues the products, warp 9 loads (10 and 11 fill the warp group).  While one row tile's weights are computed
-// the tensor cores work for the other: with both tiles a key tile costs 2 x 1024
-// tensor cycles and 2 x 1024 cycles of exponentials side by side.
+// Warps 0-3 turn A's scores into weights, a row a thread (its 128 scores stay in
+// registers), warps 4-7 B's, warp 8 issues the products, warp 9 loads.  While
+// one row tile's weights are computed the tensor cores work for the other.  A
+// block's products run in the order of their issue, so the next scores may be
+// issued behind the product that reads the weights they go over.
+// Bound by the chain of a row tile: 2350 cycles for a tile's weights (1024 of
+// them the exponential unit's, shared by both row tiles), 1300 for the value
+// product's second half and the next scores: 3650 cycles a key tile, against
+// 2 x 1024 tensor cycles.  8 trees of up to 64 drafts over up to 8192 tokens,
+// 16 query heads a KV head: 70 us, 41 GFLOP.  Scores in halves of 64 keys with
+// buffers of their own were slower (5300 cycles: products of 64 columns cost
+// nearly as much to issue and run as those of 128), as was one f32 mma.sync
+// kernel for all rows (185 us).
 // The running maximum moves only when it grows by more than 2^8 (weights stay
 // below 2^8, sums and bf16 lose nothing by that), so O is hardly ever rescaled.
 template <int D>
@@ -987,11 +997,7 @@ struct TcCfg {
   static constexpr int kTileBytes = kTile * D * 2;
   static constexpr int kQBytes = 2 * 128 * D * 2;
   static constexpr int kSmem = kStages * kTileBytes + kQBytes + 1024;
-  static constexpr int kThreads = 384;
-  // Registers a thread, launched with 65536 / 384 -> 168: the two weight groups
-  // take 216, the group of the other warps gives up all but 72 (2 * 216 + 72 =
-  // 3 * 168), so a row's 128 scores stay in registers.
-  static constexpr int kWeightRegs = 216, kOtherRegs = 72;
+  static constexpr int kThreads = 320;
   static constexpr uint32_t kO = 256;  // tensor memory columns: S/P A, S/P B, O A, O B
 };
 
@@ -1001,7 +1007,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t phase, int *ab
 }
 
 template <int D>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(320, 1)
     paged_attn_tc_kernel(const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap,
                          const __grid_constant__ PagedAttn a) {
@@ -1058,9 +1064,7 @@ __global__ void __launch_bounds__(384, 1)
   Cursor<R> cur = share;
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
-  if (warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
-   if (warp == 9) {
+  if (warp == 9) {
     load_tiles<D, R, STAGES, true, C::kLimits>(a, cur, &kmap, &vmap, ring, full, empty, limits,
                                                &abort_flag, &q_full[0]);
     if (*(volatile int *)&abort_flag) drain_ring(full, STAGES);
@@ -1145,10 +1149,8 @@ __global__ void __launch_bounds__(384, 1)
       while (!mbar_try_wait(&drain, 0) && nk_globaltimer() - start < 10000000ull) {
       }
     }
-   }
   } else {
     // ---------------------------------------------------------------- weights
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kWeightRegs));
     const int g = warp >> 2;
     const int r = threadIdx.x;  // row of the unit
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;

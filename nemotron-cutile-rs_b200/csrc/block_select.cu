@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
   constexpr int T = 32 * kScoreWarps;
   extern __shared__ __align__(16) uint8_t smem[];
   const int wide = (a.group + HEADS - 1) / HEADS * HEADS;
-  float4 *qs = reinterpret_cast<float4 *>(smem);             // [D][wide/2]: q+ of two heads, q- of both
+  // [D][wide/2]: q+ of two heads, q- of both
+  float4 *qs = reinterpret_cast<float4 *>(smem);
   float *qm = reinterpret_cast<float *>(qs + D * wide / 2);  // [D]: max_g |q|
   uint8_t *bounds = reinterpret_cast<uint8_t *>(qm + D);     // [low, high][block][kRow]
   const bool once = wide == HEADS;                           // one pass
@@ -589,7 +590,8 @@ static nk_status launch_scores_heads(const SelectArgs &a, dim3 grid, cudaStream_
                             227 * 1024, prepared);
   if (st != NK_OK) return st;
   const int64_t wide = ceil_div(a.group, HEADS) * HEADS;
-  block_scores_kernel<D, HEADS><<<grid, 32 * kScoreWarps, ScoreShared<D>::bytes(wide, HEADS), s>>>(a);
+  const size_t bytes = ScoreShared<D>::bytes(wide, HEADS);
+  block_scores_kernel<D, HEADS><<<grid, 32 * kScoreWarps, bytes, s>>>(a);
   return NK_OK;
 }
 
@@ -655,7 +657,8 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
     tls_error().actual = workspace_bytes;
     return st;
   }
-  if ((uintptr_t)workspace & 15) return fail(NK_INVALID_PARAMS, "workspace must be 16-byte aligned");
+  if ((uintptr_t)workspace & 15)
+    return fail(NK_INVALID_PARAMS, "workspace must be 16-byte aligned");
   SelectArgs a{};
   a.pool = page_pool(*kv);
   a.batch = page_batch(*batch);

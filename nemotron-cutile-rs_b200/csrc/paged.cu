@@ -524,31 +524,44 @@ nk_status nk_kv_pages_copy(const nk_kv_pages *kv, const int32_t *src_host,
   if (count < 0) return fail(NK_INVALID_SHAPE, "count >= 0");
   if (count == 0) return ok();
   if (!src_host || !dst_host) return fail(NK_INVALID_PARAMS, "src_host and dst_host are required");
-  // A bit per page: every page is written once and no page is both read and
-  // written, so the blocks of one launch need no order.
-  static thread_local std::vector<uint8_t> role;
+  // Every page is written once and no page is both read and written, so the
+  // blocks of one launch need no order.
+  for (int64_t i = 0; i < count; ++i) {
+    if (src_host[i] < 0 || src_host[i] >= kv->pages) return fail_page(src_host[i], kv->pages, i);
+    if (dst_host[i] < 0 || dst_host[i] >= kv->pages) return fail_page(dst_host[i], kv->pages, i);
+  }
+  int64_t bad = -1;
   try {
-    role.assign((size_t)kv->pages, 0);
+    if (kv->pages / 64 <= 1024 + 16 * count) {  // a bit a page
+      static thread_local std::vector<uint64_t> written;
+      written.assign((size_t)kv->pages / 64 + 1, 0);
+      for (int64_t i = 0; i < count && bad < 0; ++i) {
+        uint64_t &w = written[dst_host[i] >> 6];
+        const uint64_t bit = 1ull << (dst_host[i] & 63);
+        if (w & bit) bad = i;
+        w |= bit;
+      }
+      for (int64_t i = 0; i < count && bad < 0; ++i)
+        if (written[src_host[i] >> 6] >> (src_host[i] & 63) & 1) bad = i;
+    } else {  // few pairs of a huge pool
+      std::vector<int32_t> to(dst_host, dst_host + count);
+      std::sort(to.begin(), to.end());
+      if (std::adjacent_find(to.begin(), to.end()) != to.end())
+        for (int64_t i = 1; i < count && bad < 0; ++i)
+          if (std::find(dst_host, dst_host + i, dst_host[i]) != dst_host + i) bad = i;
+      for (int64_t i = 0; i < count && bad < 0; ++i)
+        if (std::binary_search(to.begin(), to.end(), src_host[i])) bad = i;
+    }
   } catch (...) {
     return fail(NK_DEVICE_ERROR, "out of host memory");
   }
-  for (int64_t i = 0; i < count; ++i) {
-    const int64_t a = src_host[i], b = dst_host[i];
-    if (a < 0 || a >= kv->pages) return fail_page(a, kv->pages, i);
-    if (b < 0 || b >= kv->pages) return fail_page(b, kv->pages, i);
-    role[a] |= 1;
-  }
-  for (int64_t i = 0; i < count; ++i) {
-    if (role[dst_host[i]]) {
-      st = fail(NK_INVALID_PARAMS, "a destination page appears twice or is a source too");
-      tls_error().index = (uint64_t)i;
-      tls_error().actual = (uint64_t)dst_host[i];
-      return st;
-    }
-    role[dst_host[i]] = 2;
+  if (bad >= 0) {
+    st = fail(NK_INVALID_PARAMS, "a destination page appears twice or is a source too");
+    tls_error().index = (uint64_t)bad;
+    return st;
   }
   cudaStream_t s = as_stream(stream);
-  // Parameter blocks of three sizes: a launch copies its parameters, so a
+  // Parameter blocks of four sizes: a launch copies its parameters, so a
   // single fork should not carry 32 KB of them.
   for (int64_t i = 0; i < count;) {
     const int64_t left = count - i;
@@ -559,6 +572,9 @@ nk_status nk_kv_pages_copy(const nk_kv_pages *kv, const int32_t *src_host,
     } else if (left <= 500) {
       n = (int)left;
       st = launch_copy<500>(*kv, src_host + i, dst_host + i, n, s);
+    } else if (left <= 2000) {
+      n = (int)left;
+      st = launch_copy<2000>(*kv, src_host + i, dst_host + i, n, s);
     } else {
       n = (int)(left < 4000 ? left : 4000);
       st = launch_copy<4000>(*kv, src_host + i, dst_host + i, n, s);
@@ -574,7 +590,8 @@ nk_status nk_kv_table_write(int32_t *dst, int64_t dst_len, const int64_t *offset
   if (count < 0 || dst_len < 0) return fail(NK_INVALID_SHAPE, "count, dst_len >= 0");
   if (count == 0) return ok();
   if (!dst || !value_host) return fail(NK_INVALID_PARAMS, "dst and value_host are required");
-  if (!offset_host && count > dst_len) return fail_length("dst", (uint64_t)count, (uint64_t)dst_len);
+  if (!offset_host && count > dst_len)
+    return fail_length("dst", (uint64_t)count, (uint64_t)dst_len);
   if (offset_host) {
     bool ascending = true;
     for (int64_t i = 0; i < count; ++i) {

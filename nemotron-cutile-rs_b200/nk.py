@@ -839,22 +839,15 @@ def _expect_ints(t, name, n, device):
         raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
 
 
-def _on_pages_device(fn):
-    """Runs a wrapper with the device of its first tensor (or of the pages)
-    current: libnk launches on the current device."""
-    import functools
+def _call_on(device, name, *args) -> None:
+    """call() with the tensors' device current: libnk launches on the current one."""
+    import torch
 
-    @functools.wraps(fn)
-    def run(*args, **kw):
-        import torch
-
-        index = (args[0] if args else next(iter(kw.values()))).device.index
-        if index is None or index == torch._C._cuda_getDevice():
-            return fn(*args, **kw)
-        with torch.cuda.device(index):
-            return fn(*args, **kw)
-
-    return run
+    if device.index == torch._C._cuda_getDevice():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 def _stream_of(device, stream) -> int:
@@ -929,8 +922,8 @@ class KvPages:
             a = NkPagedAttentionArgs(None, q_heads * self.head_dim, q_heads, None,
                                      16 if max_blocks else None, max_blocks, 0, 0.0, None, BF16)
             need = ctypes.c_size_t(0)
-            call("nk_attention_paged_workspace_bytes", self._ref, ctypes.byref(b),
-                 ctypes.byref(a), ctypes.byref(need))
+            _call_on(self.device, "nk_attention_paged_workspace_bytes", self._ref,
+                     ctypes.byref(b), ctypes.byref(a), ctypes.byref(need))
             if len(self._bytes) > 4096:
                 self._bytes.clear()
             size = self._bytes[key] = need.value
@@ -942,8 +935,8 @@ class KvPages:
         size = self._bytes.get(key)
         if size is None:
             need = ctypes.c_size_t(0)
-            call("nk_kv_block_select_workspace_bytes", self._ref, ctypes.byref(b),
-                 ctypes.byref(need))
+            _call_on(self.device, "nk_kv_block_select_workspace_bytes", self._ref,
+                     ctypes.byref(b), ctypes.byref(need))
             size = self._bytes[key] = need.value
         return size
 
@@ -958,7 +951,6 @@ class KvPages:
         return tokens, (q.stride(0) if tokens > 1 else width)
 
 
-@_on_pages_device
 def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max_kv=None,
                     rows=None, layer: int = 0, stream=None) -> None:
     """Stores new keys and values (bf16 [tokens, kv_heads * head_dim], any row
@@ -975,8 +967,8 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
             raise ValueError(f"{name} must be [tokens, {width}]")
     b = pages.batch(start, kv_len, tokens, max_new, max_kv, rows)
     ld_k, ld_v = (k_new.stride(0), v_new.stride(0)) if tokens > 1 else (width, width)
-    call("nk_kv_pages_append", pages._ref, layer, ctypes.byref(b), k_new.data_ptr(), ld_k,
-         v_new.data_ptr(), ld_v, _stream_of(pages.device, stream))
+    _call_on(pages.device, "nk_kv_pages_append", pages._ref, layer, ctypes.byref(b),
+             k_new.data_ptr(), ld_k, v_new.data_ptr(), ld_v, _stream_of(pages.device, stream))
 
 
 def _host_ints(a, dtype):
@@ -985,7 +977,6 @@ def _host_ints(a, dtype):
     return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
 
 
-@_on_pages_device
 def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
     """Page dst[i] becomes a copy of page src[i] in every layer
     (nk_kv_pages_copy); src, dst are host sequences of page ids."""
@@ -994,11 +985,10 @@ def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
     s, d = _host_ints(src, np.int32), _host_ints(dst, np.int32)
     if s.size != d.size:
         raise ValueError("src and dst must have one length")
-    call("nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size,
-         _stream_of(pages.device, stream))
+    _call_on(pages.device, "nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size,
+             _stream_of(pages.device, stream))
 
 
-@_on_pages_device
 def kv_table_write(dst, values, offsets=None, stream=None) -> None:
     """dst.view(-1)[offsets[i]] = values[i] (nk_kv_table_write; offsets None:
     the first len(values) entries); dst is a contiguous int32 device tensor,
@@ -1013,11 +1003,11 @@ def kv_table_write(dst, values, offsets=None, stream=None) -> None:
     o = None if offsets is None else _host_ints(offsets, np.int64)
     if o is not None and o.size != v.size:
         raise ValueError("offsets and values must have one length")
-    call("nk_kv_table_write", ptr(dst), dst.numel(), None if o is None else o.ctypes.data,
-         v.ctypes.data, v.size, _stream_of(dst.device, stream))
+    _call_on(dst.device, "nk_kv_table_write", ptr(dst), dst.numel(),
+             None if o is None else o.ctypes.data, v.ctypes.data, v.size,
+             _stream_of(dst.device, stream))
 
 
-@_on_pages_device
 def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, dst_table=None,
                      new_len=None, stream=None):
     """Token base[b] + keep[b, i] of sequence b moves to position base[b] + i
@@ -1049,7 +1039,7 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
     a = NkKvCompactArgs(n, ptr(rows), kv_len.data_ptr(), base.data_ptr(), keep.data_ptr(),
                         keep.stride(0) if n > 1 else width, n_keep.data_ptr(), width, dst, dst_ld,
                         new_len.data_ptr())
-    call("nk_kv_pages_compact", pages._ref, ctypes.byref(a), _stream_of(dev, stream))
+    _call_on(dev, "nk_kv_pages_compact", pages._ref, ctypes.byref(a), _stream_of(dev, stream))
     return new_len
 
 
@@ -1089,12 +1079,11 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
             _hold(stream, workspace)
     else:
         size = workspace.numel()
-    call("nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace), size,
-         _stream_of(dev, stream))
+    _call_on(dev, "nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace), size,
+             _stream_of(dev, stream))
     return out
 
 
-@_on_pages_device
 def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=None, max_kv=None,
                     tree_mask=None, blocks=None, rows=None, layer: int = 0, scale=None,
                     out_dtype=BF16, out=None, workspace=None, stream=None):
@@ -1117,7 +1106,6 @@ def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=Non
                    workspace, stream)
 
 
-@_on_pages_device
 def attention_paged_workspace_bytes(pages: KvPages, tokens: int, seqs: int, q_heads: int, *,
                                     max_q: int, max_kv: int, max_blocks: int = 0) -> int:
     """Scratch bytes of attention_paged for these bounds (max_blocks > 0: the
@@ -1142,12 +1130,12 @@ def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspac
     if workspace is None:
         workspace = torch.empty(pages._select_bytes(b), dtype=torch.uint8, device=dev)
         _hold(stream, workspace)
-    call("nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k, sink,
-         local, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(dev, stream))
+    _call_on(dev, "nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k,
+             sink, local, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+             _stream_of(dev, stream))
     return out
 
 
-@_on_pages_device
 def kv_block_select(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *, sink: int = 1,
                     local: int = 1, max_q=None, max_kv=None, rows=None, layer: int = 0, out=None,
                     workspace=None, stream=None):
@@ -1159,7 +1147,6 @@ def kv_block_select(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, 
     return _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspace, stream)
 
 
-@_on_pages_device
 def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, *,
                            sink: int = 1, local: int = 1, max_q=None, max_kv=None, rows=None,
                            layer: int = 0, scale=None, out_dtype=BF16, out=None, stream=None):

@@ -227,15 +227,16 @@ def test_contradicting_batches_are_reported(cuda, start, kv_len, rows, edit, cod
         assert (lists == 7).all()
 
 
-@pytest.mark.parametrize("lens,T,H,kv", [([2000], 1, 32, 2), ([300, 1200, 64], 2, 8, 8),
-                                         ([700], 64, 16, 1)])
-def test_captured_and_on_another_stream(cuda, lens, T, H, kv):
+@pytest.mark.parametrize("lens,T,H,kv,bound", [
+    ([2000], 1, 32, 2, 2000), ([300, 1200, 64], 2, 8, 8, 1200), ([700], 64, 16, 1, 700),
+    ([2000, 37], 1, 32, 2, 20000), ([300, 1200, 64], 2, 8, 8, 9000), ([900, 20], 9, 8, 2, 9000)])
+def test_captured_and_on_another_stream(cuda, lens, T, H, kv, bound):
     """Two graphs with workspaces of their own replayed in turn on new inputs,
     and two calls in flight on two streams."""
     c = Paged(4, lens, kv, 64, 64)
     pages, counts = c.device(), [T] * len(lens)
     args = (ints(starts(counts)), ints(lens), H)
-    kw = dict(max_q=T, max_kv=max(lens))
+    kw = dict(max_q=T, max_kv=bound)
     n = T * len(lens)
     qs = [torch.randn(n, H * 64, device="cuda").bfloat16() for _ in range(4)]
     want = [nk.attention_paged(q, pages, *args, **kw) for q in qs]
@@ -480,3 +481,101 @@ def test_block_select_with_infinite_bounds_and_queries(cuda, value):
                                  ints([n * ps]), 2, 20, max_q=1, max_kv=n * ps)
         nk.device_status()
         assert got.cpu().numpy()[0, 0].tolist() == want.tolist(), where
+
+
+@pytest.mark.parametrize("bound", [512, 8192])
+def test_captured_decode_steps_follow_the_device_lengths(cuda, bound):
+    """A decode step (append, attention, block lists, sparse attention) captured
+    once and replayed while the lengths and the table grow on the device."""
+    heads, group, d, ps, top_k = 2, 4, 64, 16, 5
+    H, lens = heads * group, [100, 31]
+    c = Paged(12, [n + 40 for n in lens], heads, ps, d, width=bound // ps)
+    pages = c.device()
+    k, v = torch.zeros(2, 2, heads * d, dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros(2, H * d, dtype=torch.bfloat16, device="cuda")
+    start, kv_len = ints([0, 1, 2]), ints(lens)
+    kw = dict(max_q=1, max_kv=bound)
+
+    def step():
+        nk.kv_pages_append(pages, k, v, start, kv_len, max_new=1, max_kv=bound)
+        return nk.attention_paged(q, pages, start, kv_len, H, **kw), \
+            nk.attention_paged_sparse(q, pages, start, kv_len, H, top_k, **kw)
+
+    # bounds of the cached tokens alone
+    c.lens = np.array(lens) - 1
+    c.lo[:], c.hi[:] = 0, 0
+    c.refresh_bounds()
+    pages.k_min.copy_(torch.from_numpy(c.lo))
+    pages.k_max.copy_(torch.from_numpy(c.hi))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        full, (sparse, blocks) = step()
+    for _ in range(36):
+        new = bf16(c.rng.standard_normal((2, 2, heads, d)))
+        qh = bf16(c.rng.standard_normal((2, H, d)))
+        k.copy_(torch.from_numpy(new[0].reshape(2, -1)))
+        v.copy_(torch.from_numpy(new[1].reshape(2, -1)))
+        q.copy_(torch.from_numpy(qh.reshape(2, -1)))
+        c.lens = c.lens + 1
+        kv_len.copy_(ints(c.lens))
+        for s in range(2):
+            page, slot = c.slot(s, int(c.lens[s]) - 1)
+            c.k[0, page, :, slot], c.v[0, page, :, slot] = new[0, s], new[1, s]
+        c.refresh_bounds()
+        g.replay()
+        torch.cuda.synchronize()
+        want, mag = _reference(c, qh, [1, 1], H, "causal")
+        _close(full, want, mag)
+        lists = np.full((2, heads, top_k), -1, np.int32)
+        for s in range(2):
+            n = -(-int(c.lens[s]) // ps)
+            for h in range(heads):
+                x = chosen_blocks(qh[s, h * group:(h + 1) * group], c.lo[0, c.table[s, :n], h],
+                                  c.hi[0, c.table[s, :n], h], n, top_k, 1, 1)
+                lists[s, h, :len(x)] = x
+        assert np.array_equal(blocks.cpu().numpy(), lists)
+        want, mag = _reference(c, qh, [1, 1], H, "blocks", lists=lists)
+        _close(sparse, want, mag)
+    nk.device_status()
+
+
+@pytest.mark.parametrize("group,kv,T", [(64, 1, 1), (40, 2, 3)])
+def test_many_query_heads_to_a_kv_head(cuda, group, kv, T):
+    """Block lists whose rows fill tensor-memory tiles, and the selection's limit."""
+    c = Paged(group, [700, 90], kv, 16, 128)
+    H, n = group * kv, 2 * T
+    q = bf16(c.rng.standard_normal((n, H, 128)))
+    out, blocks = nk.attention_paged_sparse(dev(q.reshape(n, -1)).bfloat16(), c.device(),
+                                            ints([0, T, n]), ints([700, 90]), H, 9, max_q=T,
+                                            max_kv=700)
+    nk.device_status()
+    lists = blocks.cpu().numpy()
+    for s in range(2):
+        for i in range(T):
+            m = (int(c.lens[s]) - T + i) // 16 + 1
+            for h in range(kv):
+                x = chosen_blocks(q[s * T + i, h * group:(h + 1) * group],
+                                  c.lo[0, c.table[s, :m], h], c.hi[0, c.table[s, :m], h], m, 9,
+                                  1, 1)
+                assert lists[s * T + i, h, :len(x)].tolist() == x.tolist()
+    want, mag = _reference(c, q, [T, T], H, "blocks", lists=lists)
+    _close(out, want, mag)
+
+
+def test_large_magnitudes_rescale(cuda):
+    """Scores that grow by hundreds along the sequence: the running maximum
+    moves and the sums so far shrink, in every kernel."""
+    for H, kv, T in ((2, 1, 1), (16, 1, 2), (8, 1, 20)):
+        c = Paged(H, [1000], kv, 64, 128)
+        ramp = np.linspace(0.01, 12.0, 1000)
+        for p in range(1000):
+            page, slot = c.slot(0, p)
+            c.k[0, page, :, slot] = bf16(c.k[0, page, :, slot] * ramp[p])
+        q = bf16(c.rng.standard_normal((T, H, 128)))
+        for bound in (1000, 9000):
+            got = nk.attention_paged(dev(q.reshape(T, -1)).bfloat16(), c.device(), ints([0, T]),
+                                     ints([1000]), H, max_q=T, max_kv=bound, out_dtype=nk.F32)
+            nk.device_status()
+            want, mag = _reference(c, q, [T], H, "causal")
+            # keys up to 12 times unit variance: 12 times the score's error bound
+            _close(got, want, mag * (1 + 12 * 2.0**-3), True)

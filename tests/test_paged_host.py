@@ -113,6 +113,14 @@ def test_copy_refusals():
     assert nk.last_error().index == 1
     assert call([0, 2], [2, 3]) == nk.INVALID_PARAMS  # a destination that is a source
     assert call([1], [1]) == nk.INVALID_PARAMS
+    kv.pages = 2**26  # a pool too large for a bit a page
+    kv.kv_heads = 1
+    assert call([0, 1, 2], [9, 2**25, 9]) == nk.INVALID_PARAMS
+    assert nk.last_error().index == 2
+    assert call([0, 2**25 + 7], [2**25 + 7, 3]) == nk.INVALID_PARAMS
+    assert nk.last_error().index == 1
+    assert call([0, 2**26], [2, 3]) == nk.PAGE_OUT_OF_RANGE
+    kv.pages, kv.kv_heads = 8, 2
     assert call([], [], -1) == nk.INVALID_SHAPE
     assert call([], []) == nk.OK
     assert lib.nk_kv_pages_copy(_r(kv), None, None, 1, None) == nk.INVALID_PARAMS

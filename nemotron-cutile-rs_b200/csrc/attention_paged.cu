@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
   __shared__ int per;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -640,12 +640,13 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
     }
     fence_mbar_init();
     abort_flag = 0;
-    if (a.jobs) a.jobs[blockIdx.x].parts = 0;
   }
   if (threadIdx.x == 256) {
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
+  wait_for_previous();
+  if (threadIdx.x == 0 && a.jobs) a.jobs[blockIdx.x].parts = 0;
   Cursor<R> cur;
   if (CLUSTER) {
     cur.b = blockIdx.x / (a.cluster * a.units_most);
@@ -1027,7 +1028,7 @@ __global__ void __launch_bounds__(320, 1)
   __shared__ int per;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_launch();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -1044,12 +1045,13 @@ __global__ void __launch_bounds__(320, 1)
     mbar_init(&drain, 1);
     fence_mbar_init();
     abort_flag = 0;
-    if (a.jobs) a.jobs[blockIdx.x].parts = 0;
   }
   if (threadIdx.x == 288) {
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
+  wait_for_previous();
+  if (threadIdx.x == 0 && a.jobs) a.jobs[blockIdx.x].parts = 0;
   if (warp == 8) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
@@ -1412,8 +1414,7 @@ __global__ void __launch_bounds__(512)
     paged_merge_kernel(const __grid_constant__ PagedAttn a, int R) {
   constexpr int V = D / 32, ROWS = 16 / SPLIT;
   __shared__ float sum[SPLIT > 1 ? SPLIT - 1 : 1][ROWS][32][V + 1];
-  // Launched while the attention runs: nothing is read before it has ended.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   const MergeJob j = a.jobs[blockIdx.x];
   const int lane = threadIdx.x & 31, row = (threadIdx.x >> 5) % ROWS;
   const int part = threadIdx.x / (32 * ROWS);
@@ -1582,23 +1583,9 @@ static nk_status launch_attention(Kernel kernel, int smem, int threads,
                                   cudaStream_t s) {
   nk_status st = allow_smem(reinterpret_cast<const void *>(kernel), smem, prepared);
   if (st != NK_OK) return st;
-  if (!p.cluster) {
-    kernel<<<p.blocks, threads, smem, s>>>(km, vm, a);
-    return check_launch("paged attention");
-  }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)p.blocks);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)p.cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, km, vm, a));
-  return ok();
+  st = launch_early(kernel, dim3((unsigned)p.blocks), dim3((unsigned)threads), (size_t)smem,
+                    p.cluster, s, km, vm, a);
+  return st != NK_OK ? st : ok();
 }
 
 template <int D, int MT>
@@ -1617,27 +1604,17 @@ template <int D>
 static nk_status launch_attention(const CUtensorMap &km, const CUtensorMap &vm,
                                   const PagedAttn &a, const AttnPlan &p, cudaStream_t s) {
   static std::atomic<uint64_t> prepared{0};
-  const nk_status st =
+  nk_status st =
       p.row_tiles == 1   ? launch_rows<D, 1>(km, vm, a, p, s)
       : p.row_tiles == 2 ? launch_rows<D, 2>(km, vm, a, p, s)
                          : launch_attention(paged_attn_tc_kernel<D>, TcCfg<D>::kSmem,
                                             TcCfg<D>::kThreads, prepared, km, vm, a, p, s);
   if (st != NK_OK || !p.merge) return st;
-  // The merge is launched while the attention runs and waits on the device for
-  // its end, which hides the launch.
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)p.blocks, (unsigned)ceil_div(p.unit_rows, p.row_tiles > 2 ? 16 : 4));
-  cfg.blockDim = dim3(512);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NK_CUDA_TRY(p.row_tiles > 2
-                  ? cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, 1>, a, 16 * p.row_tiles)
-                  : cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, 4>, a, 16 * p.row_tiles));
-  return ok();
+  const bool wide = p.row_tiles > 2;
+  const dim3 grid((unsigned)p.blocks, (unsigned)ceil_div(p.unit_rows, wide ? 16 : 4));
+  st = launch_early(wide ? paged_merge_kernel<D, 1> : paged_merge_kernel<D, 4>, grid, dim3(512), 0,
+                    1, s, a, 16 * p.row_tiles);
+  return st != NK_OK ? st : ok();
 }
 
 }  // namespace nk

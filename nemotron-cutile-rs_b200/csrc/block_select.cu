@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
   const bool once = wide == HEADS;                           // one pass
   float *sums = reinterpret_cast<float *>(bounds + (once ? 0 : S::kBounds));
                                                              // [HEADS + 1][warp][block]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_launch();
+  wait_for_previous();
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The first 8 channels of this thread's queries are on their way while the
   // sequence is found.
@@ -452,10 +453,10 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
 template <int D, int T>
 __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {
   __shared__ TopShared<T> sh;
+  let_next_launch();
+  wait_for_previous();
   Query x;
   if (!find_query(a, blockIdx.y, x, threadIdx.x == 0)) return;
-  // Launched while the scores are computed: nothing of them is read before.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int h = blockIdx.x, n = x.blocks;
   int32_t *out = a.blocks + (x.token * a.pool.heads + h) * (int64_t)a.top_k;
   if (n <= a.top_k) {
@@ -591,8 +592,7 @@ static nk_status launch_scores_heads(const SelectArgs &a, dim3 grid, cudaStream_
   if (st != NK_OK) return st;
   const int64_t wide = ceil_div(a.group, HEADS) * HEADS;
   const size_t bytes = ScoreShared<D>::bytes(wide, HEADS);
-  block_scores_kernel<D, HEADS><<<grid, 32 * kScoreWarps, bytes, s>>>(a);
-  return NK_OK;
+  return launch_early(block_scores_kernel<D, HEADS>, grid, dim3(32 * kScoreWarps), bytes, 1, s, a);
 }
 
 // Heads of a pass: as many as a list has, up to 16.
@@ -683,25 +683,16 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
                     (unsigned)batch->tokens);
     st = kv->head_dim == 128 ? launch_scores<128>(a, grid, s) : launch_scores<64>(a, grid, s);
     if (st != NK_OK) return st;
-    st = check_launch("block_scores_kernel");
-    if (st != NK_OK) return st;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)kv->kv_heads, (unsigned)batch->tokens);
   const bool small = width <= 1024;
-  cfg.blockDim = dim3(small ? 128 : 512);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = width > top_k ? 1 : 0;
+  const dim3 grid((unsigned)kv->kv_heads, (unsigned)batch->tokens), block(small ? 128 : 512);
   if (kv->head_dim == 128)
-    NK_CUDA_TRY(small ? cudaLaunchKernelEx(&cfg, block_topk_kernel<128, 128>, a)
-                      : cudaLaunchKernelEx(&cfg, block_topk_kernel<128, 512>, a));
+    st = launch_early(small ? block_topk_kernel<128, 128> : block_topk_kernel<128, 512>, grid,
+                      block, 0, 1, s, a);
   else
-    NK_CUDA_TRY(small ? cudaLaunchKernelEx(&cfg, block_topk_kernel<64, 128>, a)
-                      : cudaLaunchKernelEx(&cfg, block_topk_kernel<64, 512>, a));
+    st = launch_early(small ? block_topk_kernel<64, 128> : block_topk_kernel<64, 512>, grid, block,
+                      0, 1, s, a);
+  if (st != NK_OK) return st;
   return ok();
 }
 

@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(128)
   constexpr int C = D / 8, LANES = 128 / C;
   __shared__ uint4 sh_lo[128], sh_hi[128];
   __shared__ int sh_any[128];
+  let_next_launch();
   SeqView s;
   if (!load_seq(pool, batch, blockIdx.z, s, err, threadIdx.x == 0)) return;
   const int p0 = s.len - s.count;  // position of the first new token

@@ -60,6 +60,41 @@ inline nk_status allow_smem(const void *kernel, int bytes, std::atomic<uint64_t>
   return NK_OK;
 }
 
+// Kernels of this cache often follow one another in a stream (append, scores,
+// lists, attention, merge) and are short: each lets the next one be launched
+// while it runs (let_next_launch).  A kernel that is launched so (launch_early)
+// waits on the device for the end of the one before it (wait_for_previous)
+// ahead of its first access to global memory, on every path, and reads nothing
+// through the read-only cache.  The wait is for the whole grid and its writes,
+// which waited for the grid before it, so the stream's order holds.  Behind any
+// other kernel the launch is an ordinary one.
+__device__ __forceinline__ void let_next_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// cluster > 1: blocks of a cluster.
+template <typename... Params, typename... Args>
+nk_status launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, int cluster,
+                       cudaStream_t s, const Args &...args) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  NK_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return NK_OK;
+}
+
 // First error of a kernel stays in the device word.
 __device__ __forceinline__ void report(int *err, int code) { atomicCAS(err, 0, code); }
 

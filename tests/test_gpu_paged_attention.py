@@ -264,6 +264,50 @@ def test_captured_and_on_another_stream(cuda, lens, T, H, kv, bound):
     nk.device_status()
 
 
+def test_captured_behind_copies_and_other_streams(cuda):
+    """Calls captured behind a copy, a fill, an append and a join of two streams:
+    each sees what was written before it, at every replay."""
+    heads, d, ps, lens = 2, 64, 16, [700, 333]
+    H = heads * 4
+    c = Paged(21, lens, heads, ps, d)
+    pages = c.device()
+    start, kv_len = ints([0, 1, 2]), ints(lens)
+    kw = dict(max_q=1, max_kv=9000)
+    source = torch.zeros(2, H * d, dtype=torch.bfloat16, device="cuda")
+    q, q2 = torch.zeros_like(source), torch.zeros_like(source)
+    new = torch.zeros(2, 2, heads * d, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    nk.attention_paged(q, pages, start, kv_len, H, **kw)  # workspaces of the first call
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        q.copy_(source)
+        behind_copy = nk.attention_paged(q, pages, start, kv_len, H, **kw)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            q2.zero_()
+            q2.add_(source, alpha=2)
+        nk.kv_pages_append(pages, new[0], new[1], start, kv_len, max_new=1, max_kv=9000)
+        torch.cuda.current_stream().wait_stream(side)
+        joined = nk.attention_paged(q2, pages, start, kv_len, H, **kw)
+        sparse, blocks = nk.attention_paged_sparse(q2, pages, start, kv_len, H, 6, **kw)
+        again = nk.attention_paged(q, pages, start, kv_len, H, **kw)
+    for _ in range(6):
+        source.copy_(torch.from_numpy(bf16(c.rng.standard_normal((2, H * d)))))
+        new.copy_(torch.from_numpy(bf16(c.rng.standard_normal((2, 2, heads * d)))))
+        want_first = nk.attention_paged(source, pages, start, kv_len, H, **kw)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        twice = source * 2
+        assert torch.equal(behind_copy, want_first)
+        assert torch.equal(joined, nk.attention_paged(twice, pages, start, kv_len, H, **kw))
+        assert torch.equal(again, nk.attention_paged(source, pages, start, kv_len, H, **kw))
+        want = nk.attention_paged_sparse(twice, pages, start, kv_len, H, 6, **kw)
+        assert torch.equal(sparse, want[0]) and torch.equal(blocks, want[1])
+    nk.device_status()
+
+
 def test_explicit_workspace(cuda):
     c = Paged(4, [3000], 2, 64, 64)
     pages, q = c.device(), torch.randn(1, 256, device="cuda").bfloat16()

@@ -1481,6 +1481,43 @@ struct AttnPlan {
   size_t o_bytes, ml_bytes, bytes;
 };
 
+// Clusters of c blocks that the current device holds at once.  Asked once a
+// device: a GPC holds whole clusters only, so this is less than the SMs' number
+// over c (16 clusters of 8 with one block an SM do not fit 148 SMs).
+template <int D, int MT>
+static int resident_clusters(int c) {
+  using C = Cfg<D, MT>;
+  static std::atomic<int> known[64][4];  // 1 + the answer
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  std::atomic<int> &slot = known[dev & 63][__builtin_ctz((unsigned)c)];
+  const int seen = slot.load(std::memory_order_relaxed);
+  if (seen) return seen - 1;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)c;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)c);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const auto kernel = paged_attn_kernel<D, MT, true>;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) !=
+          cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  slot.store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
 static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
                                const nk_paged_attention_args &a) {
   AttnPlan p{};
@@ -1498,13 +1535,24 @@ static AttnPlan plan_attention(const nk_kv_pages &kv, const nk_kv_batch &b,
   const int most = num_sms() * (kv.head_dim == 64 && p.row_tiles <= 2 ? Cfg<64, 1>::kBlocks : 1);
   p.blocks = p.tiles < most ? (p.tiles < 1 ? 1 : (int)p.tiles) : most;
   p.units_most = (int)(kv.kv_heads * units < (1 << 30) ? kv.kv_heads * units : 1 << 30);
-  // Clusters: when every unit gets a block for two of its tiles or fewer and all
-  // of them are resident at once.  (Clusters of 16 found no room side by side:
-  // 8 units of 32 tiles took 22 us, as a list 11 us and 4 for the merge.)
-  if (p.row_tiles <= 2 && tiles <= 16) {
-    int c = 1;
-    while (c < 8 && c < tiles) c *= 2;
-    if ((double)b.seqs * p.units_most * c <= most) {
+  // Clusters, when every unit gets a block for four of its tiles or fewer and all
+  // clusters are resident at once: one launch, no workspace (1 sequence of 4096,
+  // 8 heads of 128: 9.7 us, 13.4 with the call's host time, as a list 10.2 and
+  // 17; 4 of 2048: 9.9 and 12.2).  Block lists of more than 16 tiles run as a
+  // tile list: its start hides behind the selection, and few SMs are slower on
+  // pages that lie far apart (64 pages of 131072 tokens: 34 us as clusters, 28).
+  // (Clusters of 16 found no room side by side: 8 units of 32 tiles 22 us.)
+  if (p.row_tiles <= 2 && tiles > 1 && tiles <= (a.blocks ? 16 : 32)) {
+    const double all = (double)b.seqs * p.units_most;
+    int c = 8;
+    while (c / 2 >= tiles) c /= 2;
+    for (; c * 4 >= tiles && c > 0; c /= 2) {
+      const int room = kv.head_dim == 128
+                           ? (p.row_tiles == 1 ? resident_clusters<128, 1>(c)
+                                               : resident_clusters<128, 2>(c))
+                           : (p.row_tiles == 1 ? resident_clusters<64, 1>(c)
+                                               : resident_clusters<64, 2>(c));
+      if (all > room) continue;
       p.cluster = c;
       p.blocks = (int)b.seqs * p.units_most * c;
       return p;

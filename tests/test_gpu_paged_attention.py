@@ -505,6 +505,49 @@ def test_block_select_with_scores_that_nearly_tie(cuda, ps, d, group, n, top_k, 
     assert got.cpu().numpy()[0, 0].tolist() == want.tolist()
 
 
+@pytest.mark.parametrize("n", [500, 1700])
+@pytest.mark.parametrize("alike", [2, 127, 128, 129, 300])
+@pytest.mark.parametrize("distinct", [False, True])
+def test_block_select_with_few_and_many_blocks_at_the_border(cuda, n, alike, distinct):
+    """Clear winners, clear losers, and `alike` blocks at the border that f32 sums
+    cannot tell apart: equal ones, or ones that differ by 2^-26 of a term."""
+    ps, d, winners = 16, 128, 9
+    c = Paged(n + alike, [n * ps], 1, ps, d)
+    order = 1 + c.rng.permutation(n - 2)  # the first and the last block are forced
+    low = np.full((n, d), -1.0, np.float32)
+    high = np.full((n, d), 1.0, np.float32)
+    high[order[:winners]] = 3.0
+    high[order[winners + alike:]] = 0.5
+    if distinct:  # q = 1 but for channel 7, where it is 2^-20
+        high[order[winners:winners + alike], 7] = bf16(
+            1 + np.arange(alike) % 64 / 64.0)[c.rng.permutation(alike)]
+    c.lo[0, c.table[0, :n], 0], c.hi[0, c.table[0, :n], 0] = low, high
+    q = np.ones((1, 2, d), np.float32)
+    q[..., 7] = 2.0**-20
+    for top_k in (2 + winners + 1, 2 + winners + alike - 1):
+        want = chosen_blocks(q[0], low, high, n, top_k, 1, 1)
+        got = nk.kv_block_select(dev(q.reshape(1, -1)).bfloat16(), c.device(), ints([0, 1]),
+                                 ints([n * ps]), 2, top_k, max_q=1, max_kv=n * ps)
+        nk.device_status()
+        assert got.cpu().numpy()[0, 0].tolist() == want.tolist()
+
+
+@pytest.mark.parametrize("n", [2000, 4096])
+@pytest.mark.parametrize("heads,seqs", [(1, 1), (8, 2), (2, 4)])
+def test_clusters_of_several_tiles_a_block(cuda, n, heads, seqs):
+    """Units of 16 to 32 tiles, which clusters take three and four tiles a block
+    where they fit and a tile list where not; lengths end inside tiles."""
+    lens = [n - 37 * s - 1 for s in range(seqs)]
+    c = Paged(heads + seqs, lens, heads, 64, 128)
+    H = heads * 2
+    q = bf16(c.rng.standard_normal((seqs, H, 128)))
+    got = nk.attention_paged(dev(q.reshape(seqs, -1)).bfloat16(), c.device(),
+                             ints(starts([1] * seqs)), ints(lens), H, max_q=1, max_kv=n)
+    nk.device_status()
+    want, mag = _reference(c, q, [1] * seqs, H, "causal")
+    _close(got, want, mag)
+
+
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 def test_block_select_with_infinite_bounds_and_queries(cuda, value):
     """What the definition makes of infinities and NaN, in a bound and in a

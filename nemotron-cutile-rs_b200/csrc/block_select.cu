@@ -326,8 +326,10 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 
 template <int T>
 struct TopShared {
-  static constexpr int kWarps = T / 32;
+  static constexpr int kWarps = T / 32, kDoubt = 128;
   int hist[256];
+  u64 doubt_key[kDoubt], from;
+  int doubt[kDoubt], doubts, ties;
   u64 ends[2][kWarps];
   int above[kWarps], equal[kWarps];
   int digit, need, whole;
@@ -445,11 +447,13 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
 
 // Block = (KV head x, token y).  With L the need-th largest lower end of the
 // intervals: a block whose upper end is below L is out, and when exactly `need`
-// upper ends reach L they are the list.  If not, with H the (need+1)-th largest
-// upper end, a block whose lower end is above H is in and those in between are
-// scored in 64 bits.  Then the list is written in ascending order: a warp holds
-// a contiguous run of blocks, 32 neighbours at a time.  T threads: 128 up to 1024
-// blocks (400 lists of 190: 16 us with 512, most of them idle), 512 beyond.
+// upper ends reach L they are the list.  If not, with H the largest upper end of
+// a block whose lower end is L or less, a block whose lower end is above H is in
+// (only blocks whose lower end is above L could beat it, `need` with itself at
+// most) and those in between are scored in 64 bits.  Then the list is written in
+// ascending order: a warp holds a contiguous run of blocks, 32 neighbours at a
+// time.  T threads: 128 up to 1024 blocks (400 lists of 190: 16 us with 512, most
+// of them idle), 512 beyond.
 template <int D, int T>
 __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {
   __shared__ TopShared<T> sh;
@@ -484,20 +488,20 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
     for (int j = j0; j < j1; j += 32) reach += is_free(j) && order_key(range[j].y) >= low;
     settled = block_sum<T>(reach, sh.above) == need;
     if (!settled) {
-      auto upper = [&](int j) { return is_free(j) ? order_key(range[j].y) : 0u; };
-      high = nth_largest<uint32_t, T>(j0, j1, upper, need + 1, sh, whole);
-      // A whole result may lie below H, which is the smallest key that reaches it.
-      uint32_t least = 0xffffffffu;
+      // H
+      uint32_t top = 0;
+#pragma unroll 4
       for (int j = j0; j < j1; j += 32) {
-        const uint32_t k = upper(j);
-        if (k >= high && k < least) least = k;
+        const uint32_t k = order_key(range[j].y);
+        if (is_free(j) && k >= low && order_key(range[j].x) <= low && k > top) top = k;
       }
-      least = warp_min(least);
-      if (lane == 0) sh.above[warp] = (int)least;
+      top = warp_max(top);
+      if (lane == 0) sh.above[warp] = (int)top;
+      if (threadIdx.x == 0) sh.doubts = 0;
       __syncthreads();
       for (int w = 0; w < T / 32; ++w)
-        least = (uint32_t)sh.above[w] < least ? (uint32_t)sh.above[w] : least;
-      high = least;
+        top = (uint32_t)sh.above[w] > top ? (uint32_t)sh.above[w] : top;
+      high = top;
       __syncthreads();
     }
   }
@@ -513,23 +517,57 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
   bool ties = false;  // and the first by index of those equal to it
   if (!settled) {
     int in = 0;
-    for (int j = j0; j - lane < j1; j += 32) {
-      const int k = j < j1 ? kind(j) : 0;
+    for (int j = j0; j < j1; j += 32) {
+      const int k = kind(j);
       in += k == 1 && is_free(j);
-      for (uint32_t doubt = __ballot_sync(0xffffffffu, k == 2); doubt; doubt &= doubt - 1) {
-        const int b = j - lane + __ffs(doubt) - 1;
-        const double v = exact_score<D>(a, x, h, b);
-        if (b == j) exact[b] = v;  // read again by this thread only
+      if (k == 2) {
+        const int i = atomicAdd(&sh.doubts, 1);
+        if (i < TopShared<T>::kDoubt) sh.doubt[i] = j;
       }
     }
-    const int left = need - block_sum<T>(in, sh.above);
-    bool whole = true;
+    const int left = need - block_sum<T>(in, sh.above), doubts = sh.doubts;
     from = ~0ull;  // no score is that large (it would be a NaN's)
-    if (left > 0)
+    if (left > 0 && doubts <= TopShared<T>::kDoubt) {
+      // A few: a warp each, and a thread each to rank it among them.
+      for (int i = warp; i < doubts; i += T / 32) {
+        const double v = exact_score<D>(a, x, h, sh.doubt[i]);
+        if (lane == 0) {
+          exact[sh.doubt[i]] = v;
+          sh.doubt_key[i] = order_key(v);
+        }
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < doubts) {
+        const u64 mine = sh.doubt_key[threadIdx.x];
+        int larger = 0, as_large = 0;
+#pragma unroll 2
+        for (int i = 0; i < doubts; ++i) {
+          const u64 k = sh.doubt_key[i];
+          larger += k > mine;
+          as_large += k >= mine;
+        }
+        if (larger < left && left <= as_large) {  // one value
+          sh.from = mine;
+          sh.ties = as_large > left;
+        }
+      }
+      __syncthreads();
+      from = sh.from;
+      ties = sh.ties != 0;
+    } else if (left > 0) {
+      for (int j = j0; j - lane < j1; j += 32)
+        for (uint32_t doubt = __ballot_sync(0xffffffffu, j < j1 && kind(j) == 2); doubt;
+             doubt &= doubt - 1) {
+          const int b = j - lane + __ffs(doubt) - 1;
+          const double v = exact_score<D>(a, x, h, b);
+          if (b == j) exact[b] = v;  // read again by this thread only
+        }
+      bool whole;
       from = nth_largest<u64, T>(
           j0, j1, [&](int j) { return kind(j) == 2 ? order_key(exact[j]) : 0ull; }, left, sh,
           whole);
-    ties = !whole;
+      ties = !whole;
+    }
   }
   // How a block counts: 0 out, 1 taken, 2 equal to the last score taken.
   auto verdict = [&](int j) {

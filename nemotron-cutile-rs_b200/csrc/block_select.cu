@@ -26,6 +26,7 @@ struct SelectArgs {
   int group;
   const uint16_t *k_min, *k_max;  // the layer's
   int top_k, sink, local;
+  bool scored;  // the scores are computed by the kernel before the lists
   int64_t score_ld;
   float2 *range;   // [tokens, kv_heads, score_ld]: the score lies in it
   double *exact;   // the same shape: 64-bit scores of the blocks in doubt
@@ -134,8 +135,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
   const bool once = wide == HEADS;                           // one pass
   float *sums = reinterpret_cast<float *>(bounds + (once ? 0 : S::kBounds));
                                                              // [HEADS + 1][warp][block]
-  let_next_launch();
   wait_for_previous();
+  let_next_launch();  // behind the wait: the lists read the batch without one
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The first 8 channels of this thread's queries are on their way while the
   // sequence is found.
@@ -464,9 +465,11 @@ template <int D, int T>
 __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {
   __shared__ TopShared<T> sh;
   let_next_launch();
-  wait_for_previous();
+  if (!a.scored) wait_for_previous();
   Query x;
-  if (!find_query(a, blockIdx.y, x, threadIdx.x == 0)) return;
+  const bool found = find_query(a, blockIdx.y, x, threadIdx.x == 0);
+  if (a.scored) wait_for_previous();
+  if (!found) return;
   const int h = blockIdx.x, n = x.blocks;
   int32_t *out = a.blocks + (x.token * a.pool.heads + h) * (int64_t)a.top_k;
   if (n <= a.top_k) {
@@ -482,98 +485,122 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
   const int run = ((n + T - 1) / T) * 32;
   const int j0 = warp * run + lane, j1 = (warp + 1) * run < n ? (warp + 1) * run : n;
   auto is_free = [&](int j) { return j >= lo && j < hi; };
-  uint32_t low = 1, high = 0xffffffffu;
-  bool settled = true;  // no block is in doubt
+  uint32_t low = 0xffffffffu;
   if (need > 0) {
     bool whole;
     // A `whole` result may lie below L: the blocks it keeps in play are more.
     low = nth_largest<uint32_t, T>(
         j0, j1, [&](int j) { return is_free(j) ? order_key(range[j].x) : 0u; }, need, sh, whole);
-    int reach = 0;
-#pragma unroll 4
-    for (int j = j0; j < j1; j += 32) reach += is_free(j) && order_key(range[j].y) >= low;
-    settled = block_sum<T>(reach, sh.above) == need;
-    if (!settled) {
-      // H
-      uint32_t top = 0;
-#pragma unroll 4
-      for (int j = j0; j < j1; j += 32) {
-        const uint32_t k = order_key(range[j].y);
-        if (is_free(j) && k >= low && order_key(range[j].x) <= low && k > top) top = k;
-      }
-      top = warp_max(top);
-      if (lane == 0) sh.above[warp] = (int)top;
-      if (threadIdx.x == 0) sh.doubts = 0;
-      __syncthreads();
-      for (int w = 0; w < T / 32; ++w)
-        top = (uint32_t)sh.above[w] > top ? (uint32_t)sh.above[w] : top;
-      high = top;
-      __syncthreads();
-    }
   }
+  // The forced blocks and those that reach L: the list, if they are top_k.
+  auto reaches = [&](int j) {
+    return j < j1 && (!is_free(j) || order_key(range[j].y) >= low);
+  };
+  const uint32_t below = (1u << lane) - 1;
+  uint32_t kept = 0;  // of the first 32 blocks of this thread
+  int mine = 0;
+#pragma unroll 1
+  for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
+    const bool r = reaches(j);
+    if (i < 32) kept |= (uint32_t)r << i;
+    mine += __popc(__ballot_sync(0xffffffffu, r));
+  }
+  if (lane == 0) sh.above[warp] = mine;
+  __syncthreads();
+  int reach = 0, at = 0;  // of the block, and before this warp's run
+#pragma unroll
+  for (int w = 0; w < T / 32; ++w) {
+    if (w < warp) at += sh.above[w];
+    reach += sh.above[w];
+  }
+  if (reach == a.top_k) {
+#pragma unroll 1
+    for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
+      const bool take = i < 32 ? kept >> i & 1 : reaches(j);
+      const uint32_t taken = __ballot_sync(0xffffffffu, take);
+      if (take) out[at + __popc(taken & below)] = j;
+      at += __popc(taken);
+    }
+    return;
+  }
+  __syncthreads();
+  // H
+  uint32_t top = 0, high;
+#pragma unroll 4
+  for (int j = j0; j < j1; j += 32) {
+    if (!is_free(j)) continue;
+    const uint32_t k = order_key(range[j].y);
+    if (k >= low && order_key(range[j].x) <= low && k > top) top = k;
+  }
+  top = warp_max(top);
+  if (lane == 0) sh.above[warp] = (int)top;
+  if (threadIdx.x == 0) sh.doubts = 0;
+  __syncthreads();
+  for (int w = 0; w < T / 32; ++w)
+    top = (uint32_t)sh.above[w] > top ? (uint32_t)sh.above[w] : top;
+  high = top;
+  __syncthreads();
   // 0: out, 1: in, 2: in doubt.
   auto kind = [&](int j) {
     if (!is_free(j)) return 1;
-    if (need == 0) return 0;
     const float2 r = range[j];
     if (order_key(r.y) < low) return 0;
-    return settled || order_key(r.x) > high ? 1 : 2;
+    return order_key(r.x) > high ? 1 : 2;
   };
-  u64 from = 0;       // blocks in doubt: taken above it,
-  bool ties = false;  // and the first by index of those equal to it
-  if (!settled) {
-    int in = 0;
-    for (int j = j0; j < j1; j += 32) {
-      const int k = kind(j);
-      in += k == 1 && is_free(j);
-      if (k == 2) {
-        const int i = atomicAdd(&sh.doubts, 1);
-        if (i < TopShared<T>::kDoubt) sh.doubt[i] = j;
+  int in = 0;
+  for (int j = j0; j < j1; j += 32) {
+    const int k = kind(j);
+    in += k == 1 && is_free(j);
+    if (k == 2) {
+      const int i = atomicAdd(&sh.doubts, 1);
+      if (i < TopShared<T>::kDoubt) sh.doubt[i] = j;
+    }
+  }
+  const int left = need - block_sum<T>(in, sh.above), doubts = sh.doubts;
+  // Blocks in doubt: taken above `from`, and the first by index of those equal to
+  // it.  (No score is that large: it would be a NaN's.)
+  u64 from = ~0ull;
+  bool ties = false;
+  if (left > 0 && doubts <= TopShared<T>::kDoubt) {
+    // A few: a warp each, and a thread each to rank it among them.
+    for (int i = warp; i < doubts; i += T / 32) {
+      const double v = exact_score<D>(a, x, h, sh.doubt[i]);
+      if (lane == 0) {
+        exact[sh.doubt[i]] = v;
+        sh.doubt_key[i] = order_key(v);
       }
     }
-    const int left = need - block_sum<T>(in, sh.above), doubts = sh.doubts;
-    from = ~0ull;  // no score is that large (it would be a NaN's)
-    if (left > 0 && doubts <= TopShared<T>::kDoubt) {
-      // A few: a warp each, and a thread each to rank it among them.
-      for (int i = warp; i < doubts; i += T / 32) {
-        const double v = exact_score<D>(a, x, h, sh.doubt[i]);
-        if (lane == 0) {
-          exact[sh.doubt[i]] = v;
-          sh.doubt_key[i] = order_key(v);
-        }
-      }
-      __syncthreads();
-      if ((int)threadIdx.x < doubts) {
-        const u64 mine = sh.doubt_key[threadIdx.x];
-        int larger = 0, as_large = 0;
+    __syncthreads();
+    if ((int)threadIdx.x < doubts) {
+      const u64 own = sh.doubt_key[threadIdx.x];
+      int larger = 0, as_large = 0;
 #pragma unroll 2
-        for (int i = 0; i < doubts; ++i) {
-          const u64 k = sh.doubt_key[i];
-          larger += k > mine;
-          as_large += k >= mine;
-        }
-        if (larger < left && left <= as_large) {  // one value
-          sh.from = mine;
-          sh.ties = as_large > left;
-        }
+      for (int i = 0; i < doubts; ++i) {
+        const u64 k = sh.doubt_key[i];
+        larger += k > own;
+        as_large += k >= own;
       }
-      __syncthreads();
-      from = sh.from;
-      ties = sh.ties != 0;
-    } else if (left > 0) {
-      for (int j = j0; j - lane < j1; j += 32)
-        for (uint32_t doubt = __ballot_sync(0xffffffffu, j < j1 && kind(j) == 2); doubt;
-             doubt &= doubt - 1) {
-          const int b = j - lane + __ffs(doubt) - 1;
-          const double v = exact_score<D>(a, x, h, b);
-          if (b == j) exact[b] = v;  // read again by this thread only
-        }
-      bool whole;
-      from = nth_largest<u64, T>(
-          j0, j1, [&](int j) { return kind(j) == 2 ? order_key(exact[j]) : 0ull; }, left, sh,
-          whole);
-      ties = !whole;
+      if (larger < left && left <= as_large) {  // one value
+        sh.from = own;
+        sh.ties = as_large > left;
+      }
     }
+    __syncthreads();
+    from = sh.from;
+    ties = sh.ties != 0;
+  } else if (left > 0) {
+    for (int j = j0; j - lane < j1; j += 32)
+      for (uint32_t doubt = __ballot_sync(0xffffffffu, j < j1 && kind(j) == 2); doubt;
+           doubt &= doubt - 1) {
+        const int b = j - lane + __ffs(doubt) - 1;
+        const double v = exact_score<D>(a, x, h, b);
+        if (b == j) exact[b] = v;  // read again by this thread only
+      }
+    bool whole;
+    from = nth_largest<u64, T>(
+        j0, j1, [&](int j) { return kind(j) == 2 ? order_key(exact[j]) : 0ull; }, left, sh,
+        whole);
+    ties = !whole;
   }
   // How a block counts: 0 out, 1 taken, 2 equal to the last score taken.
   auto verdict = [&](int j) {
@@ -583,7 +610,7 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
     return e == from ? (ties ? 2 : 1) : (e > from ? 1 : 0);
   };
   int above = 0, equal = 0;
-  uint32_t kept = 0;  // the verdicts of the first 16 blocks of this thread
+  kept = 0;  // the verdicts of the first 16 blocks of this thread
   for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
     const int v = j < j1 ? verdict(j) : 0;
     if (i < 16) kept |= (uint32_t)v << (2 * i);
@@ -595,7 +622,8 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
     sh.equal[warp] = equal;
   }
   __syncthreads();
-  int at = 0, eq = 0, all_above = 0;  // before this warp's run
+  int eq = 0, all_above = 0;  // before this warp's run
+  at = 0;
 #pragma unroll
   for (int w = 0; w < T / 32; ++w) {
     all_above += sh.above[w];
@@ -606,7 +634,6 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
   }
   const int room = a.top_k - all_above;  // equals that are taken
   at += eq < room ? eq : room;
-  const uint32_t below = (1u << lane) - 1;
   for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
     const int v = i < 16 ? (kept >> (2 * i)) & 3 : (j < j1 ? verdict(j) : 0);
     const uint32_t same = __ballot_sync(0xffffffffu, v == 2);
@@ -715,6 +742,7 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.top_k = (int)top_k;
   a.sink = (int)sink;
   a.local = (int)local;
+  a.scored = width > top_k;
   a.score_ld = width;
   a.exact = static_cast<double *>(workspace);
   a.range = reinterpret_cast<float2 *>(a.exact + batch->tokens * kv->kv_heads * width);

@@ -814,7 +814,8 @@ def attention_check(workspace, stream=None) -> int:
 # of a call is a few microseconds: they look at each property of a tensor once
 # and leave the wording of refusals to the slow path.
 def _is(t, dtype, dim, device) -> bool:
-    return t.dtype is dtype and t.dim() == dim and t.device == device and t.stride(-1) == 1
+    return t.dtype is dtype and t.dim() == dim and t.device == device and \
+        (t.is_contiguous() or t.stride(-1) == 1)
 
 
 def _expect(t, name, dtype, dim, device=None):
@@ -1031,7 +1032,7 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
             raise ValueError("dst_table must have a row for each sequence")
         dst, dst_ld = dst_table.data_ptr(), dst_table.stride(0) if n > 1 else dst_table.shape[1]
     if new_len is None:
-        new_len = torch.empty(n, dtype=torch.int32, device=dev)
+        new_len = torch.empty_like(kv_len, memory_format=torch.contiguous_format)
         _hold(stream, new_len)
     else:
         _expect_ints(new_len, "new_len", n, dev)
@@ -1060,8 +1061,11 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
             raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
         max_blocks = blocks.shape[2]
     if out is None:
-        out = torch.empty(q.shape, device=dev,
-                          dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
+        if out_dtype == BF16 and ld_q == q.shape[1]:
+            out = torch.empty_like(q)
+        else:
+            out = torch.empty(q.shape, device=dev,
+                              dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
         code = out_dtype
         _hold(stream, out)
     elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:

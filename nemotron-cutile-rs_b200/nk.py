@@ -972,10 +972,12 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
              k_new.data_ptr(), ld_k, v_new.data_ptr(), ld_v, _stream_of(pages.device, stream))
 
 
+# Host arrays go to the library as bytes, which ctypes passes by address: an
+# array's own address takes 2.5 us to ask for.
 def _host_ints(a, dtype):
     import numpy as np
 
-    return np.ascontiguousarray(a, dtype=dtype).reshape(-1)
+    return np.ascontiguousarray(a, dtype=dtype)
 
 
 def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
@@ -986,7 +988,7 @@ def kv_pages_copy(pages: KvPages, src, dst, stream=None) -> None:
     s, d = _host_ints(src, np.int32), _host_ints(dst, np.int32)
     if s.size != d.size:
         raise ValueError("src and dst must have one length")
-    _call_on(pages.device, "nk_kv_pages_copy", pages._ref, s.ctypes.data, d.ctypes.data, s.size,
+    _call_on(pages.device, "nk_kv_pages_copy", pages._ref, s.tobytes(), d.tobytes(), s.size,
              _stream_of(pages.device, stream))
 
 
@@ -1005,7 +1007,7 @@ def kv_table_write(dst, values, offsets=None, stream=None) -> None:
     if o is not None and o.size != v.size:
         raise ValueError("offsets and values must have one length")
     _call_on(dst.device, "nk_kv_table_write", ptr(dst), dst.numel(),
-             None if o is None else o.ctypes.data, v.ctypes.data, v.size,
+             None if o is None else o.tobytes(), v.tobytes(), v.size,
              _stream_of(dst.device, stream))
 
 

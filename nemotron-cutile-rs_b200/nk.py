@@ -977,6 +977,11 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
 def _host_ints(a, dtype):
     import numpy as np
 
+    if isinstance(a, np.ndarray) and a.dtype != dtype and a.size:
+        b = a.astype(dtype)
+        if a.dtype.kind not in "iu" or (b != a).any():
+            raise ValueError(f"{a.dtype} values do not fit {np.dtype(dtype)}")
+        a = b
     return np.ascontiguousarray(a, dtype=dtype)
 
 

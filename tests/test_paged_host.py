@@ -398,3 +398,16 @@ def test_bookkeeping_refusals_change_nothing():
         c.accept(step, [[0]])
     assert c.read(a)[:9] == list(range(9)) and c.length(a) == 11
     _check(c, {a: c.read(a), b: []})
+
+
+def test_host_arrays_that_do_not_fit_are_refused():
+    """A 64-bit page id or a fraction must not turn into another page."""
+    for bad in (np.array([2**32 + 1]), np.array([-2**31 - 1]), np.array([1.5])):
+        with pytest.raises(ValueError):
+            nk._host_ints(bad, np.int32)
+    with pytest.raises(OverflowError):
+        nk._host_ints([2**32 + 1], np.int32)
+    for good in ([], [3, 4], np.array([3, 4]), np.array([3, 4], np.int32)[::-1], np.zeros(0)):
+        got = nk._host_ints(good, np.int32)
+        assert got.dtype == np.int32 and got.flags.c_contiguous
+        assert got.tolist() == list(map(int, good))

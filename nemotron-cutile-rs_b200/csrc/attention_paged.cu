@@ -991,7 +991,8 @@ __global__ void __launch_bounds__(288, Cfg<D, MT>::kBlocks)
 // them the exponential unit's, shared by both row tiles), 1300 for the value
 // product's second half and the next scores: 3650 cycles a key tile, against
 // 2 x 1024 tensor cycles.  8 trees of up to 64 drafts over up to 8192 tokens,
-// 16 query heads a KV head: 70 us, 41 GFLOP.  Scores in halves of 64 keys with
+// 16 query heads a KV head: 72 us cold, 41 GFLOP; half of the exponentials left out
+// (to time the rest) gained 4 us.  Scores in halves of 64 keys with
 // buffers of their own were slower (5300 cycles: products of 64 columns cost
 // nearly as much to issue and run as those of 128), as was one f32 mma.sync
 // kernel for all rows (185 us).

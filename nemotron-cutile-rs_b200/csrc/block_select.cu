@@ -458,8 +458,8 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
 // ascending order: a warp holds a contiguous run of blocks, 32 neighbours at a
 // time.  T threads: 128 up to 1024 blocks, 512 beyond (400 lists of 190, scores and
 // attention included: 63 us a call with 512 threads, most of them idle, 58 with
-// 128).  Bound by the chain of the search's barriers: 8 lists of 2048 blocks 12 us
-// cold, 400 of 190 11 us.  Blocks in doubt add 5 us to a call; with a second search
+// 128).  Bound by the chain of the search's barriers: 8 lists of 2048 blocks 10 us
+// cold, 400 of 190 12 us.  Blocks in doubt add 5 us to a call; with a second search
 // for H and a third for the 64-bit scores it was 12.
 template <int D, int T>
 __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {

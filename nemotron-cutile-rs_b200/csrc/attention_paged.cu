@@ -435,6 +435,7 @@ __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
   const int box_rows = a.pool.ps, npg = kTile >> a.pool.ps_log2;  // pages of a tile
   const int boxes = npg * (D / 64) * 2;
   const int c = lane & (npg - 1), strip = (lane / npg) % (D / 64), is_v = lane / (npg * (D / 64));
+  fence_proxy_async_global();  // what the kernel before stored, ahead of the tile loads
   Piece p;
   int i = 0;
   while (cur.next(a, p)) {

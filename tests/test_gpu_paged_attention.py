@@ -308,6 +308,43 @@ def test_captured_behind_copies_and_other_streams(cuda):
     nk.device_status()
 
 
+@pytest.mark.parametrize("group,top_k", [(4, 3), (40, 9)])
+def test_steps_issued_back_to_back(cuda, group, top_k):
+    """Appends, attention and block lists of many steps in flight at once give
+    what the same steps give with a wait for the GPU after each call."""
+    heads, d, ps, steps, lens = 2, 64, 16, 60, [100, 31, 250]
+    n, H = len(lens), heads * group
+    results = []
+    for wait in (True, False):
+        c = Paged(31, [x + steps for x in lens], heads, ps, d)
+        pages = c.device()
+        start = ints(starts([1] * n))
+        now = [ints([x + i + 1 for x in lens]) for i in range(steps)]
+        gen = torch.Generator(device="cuda").manual_seed(5)
+        new = torch.empty(steps, 2, n, heads * d, dtype=torch.bfloat16,
+                          device="cuda").normal_(generator=gen)
+        q = torch.empty(steps, n, H * d, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+        got = []
+        torch.cuda.synchronize()
+
+        def done():
+            if wait:
+                torch.cuda.synchronize()
+        for i in range(steps):
+            kw = dict(max_q=1, max_kv=400)
+            nk.kv_pages_append(pages, new[i, 0], new[i, 1], start, now[i], max_new=1, max_kv=400)
+            done()
+            got.append(nk.attention_paged(q[i], pages, start, now[i], H, **kw))
+            done()
+            got += nk.attention_paged_sparse(q[i], pages, start, now[i], H, top_k, **kw)
+            done()
+        torch.cuda.synchronize()
+        nk.device_status()
+        results.append(got)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_explicit_workspace(cuda):
     c = Paged(4, [3000], 2, 64, 64)
     pages, q = c.device(), torch.randn(1, 256, device="cuda").bfloat16()

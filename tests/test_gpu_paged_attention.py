@@ -569,12 +569,14 @@ def test_block_select_with_few_and_many_blocks_at_the_border(cuda, n, alike, dis
         assert got.cpu().numpy()[0, 0].tolist() == want.tolist()
 
 
-@pytest.mark.parametrize("n", [2000, 4096])
-@pytest.mark.parametrize("heads,seqs", [(1, 1), (8, 2), (2, 4)])
+@pytest.mark.parametrize("n,heads,seqs", [
+    (2000, 1, 1), (2000, 8, 2), (2000, 2, 4), (4096, 1, 1), (4096, 8, 2), (4096, 2, 4),
+    (1000, 8, 8), (500, 8, 16), (130, 8, 18), (600, 8, 18), (600, 8, 19)])
 def test_clusters_of_several_tiles_a_block(cuda, n, heads, seqs):
-    """Units of 16 to 32 tiles, which clusters take three and four tiles a block
-    where they fit and a tile list where not; lengths end inside tiles."""
-    lens = [n - 37 * s - 1 for s in range(seqs)]
+    """Units of 2 to 32 tiles, which clusters of one to eight blocks take up to
+    four tiles a block where they fit, and a tile list where not; lengths end
+    inside tiles."""
+    lens = [max(1, n - 37 * s - 1) for s in range(seqs)]
     c = Paged(heads + seqs, lens, heads, 64, 128)
     H = heads * 2
     q = bf16(c.rng.standard_normal((seqs, H, 128)))

@@ -76,13 +76,11 @@ __device__ __forceinline__ void write_bounds(Bounds8 &b, bool any, uint4 *kmin, 
   }
 }
 
-// Block = (touched page and head x, sequence z): the new tokens of one page, so
+// Block = (touched page x, head y, sequence z): the new tokens of one page, so
 // that the page's bounds have one writer and need no atomics, and a key is read
-// once for the copy and the bounds.  The heads of a page run side by side, since
-// their 256-byte pieces of a token's row are neighbours in memory.  Bound by HBM
-// for a prefill (9000 tokens of 8 heads of 128, 74 MB: 13.8 us cold, with the
-// pages of a head side by side 15.6; 10.7 us with the tokens still in L2), by the
-// launch for a decode step (64 tokens: 2.8 us in a chain of calls).
+// once for the copy and the bounds.  Bound by HBM for a prefill (9000 tokens of 8
+// heads of 128, 74 MB: 15.5 us cold, 10.7 us with the tokens still in L2), by
+// the launch for a decode step (64 tokens: 2.6 us in a chain of calls).
 template <int D>
 __global__ void __launch_bounds__(128)
     pages_append_kernel(PagePool pool, PageBatch batch, const uint16_t *__restrict__ k_new,
@@ -96,8 +94,7 @@ __global__ void __launch_bounds__(128)
   SeqView s;
   if (!load_seq(pool, batch, blockIdx.z, s, err, threadIdx.x == 0)) return;
   const int p0 = s.len - s.count;  // position of the first new token
-  const int x = (int)blockIdx.x / pool.heads, h = (int)blockIdx.x - x * pool.heads;
-  const int j = (p0 >> pool.ps_log2) + x;
+  const int j = (p0 >> pool.ps_log2) + (int)blockIdx.x;
   const int page0 = j << pool.ps_log2;
   if (s.count == 0 || page0 >= s.len) return;
   const int page = s.table[j];
@@ -105,6 +102,7 @@ __global__ void __launch_bounds__(128)
     if (threadIdx.x == 0) report(err, NK_PAGE_OUT_OF_RANGE);
     return;
   }
+  const int h = blockIdx.y;
   const int a = p0 > page0 ? p0 : page0;
   const int e = s.len < page0 + pool.ps ? s.len : page0 + pool.ps;
   const int c = threadIdx.x % C, lane = threadIdx.x / C;
@@ -513,10 +511,8 @@ nk_status nk_kv_pages_append(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   const PagePool pool = page_pool(*kv);
   const PageBatch b = page_batch(*batch);
   // A run of max_new tokens touches at most this many pages, wherever it starts.
-  // (no more than there are: they are its own).
-  int64_t touched = (batch->max_new + kv->page_size - 2) / kv->page_size + 1;
-  if (touched > kv->pages) touched = kv->pages;
-  const dim3 grid((unsigned)(touched * kv->kv_heads), 1, (unsigned)batch->seqs);
+  const int64_t touched = (batch->max_new + kv->page_size - 2) / kv->page_size + 1;
+  const dim3 grid((unsigned)touched, (unsigned)kv->kv_heads, (unsigned)batch->seqs);
   const int64_t words = kv->pages * kv->kv_heads * kv->head_dim / 8;  // bounds of one layer
   uint4 *k = reinterpret_cast<uint4 *>(kv->k) + layer * words * kv->page_size;
   uint4 *v = reinterpret_cast<uint4 *>(kv->v) + layer * words * kv->page_size;

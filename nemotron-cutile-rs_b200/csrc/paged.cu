@@ -79,7 +79,8 @@ __device__ __forceinline__ void write_bounds(Bounds8 &b, bool any, uint4 *kmin, 
 // Block = (touched page x, head y, sequence z): the new tokens of one page, so
 // that the page's bounds have one writer and need no atomics, and a key is read
 // once for the copy and the bounds.  Bound by HBM for a prefill (9000 tokens of 8
-// heads of 128, 74 MB: 15.5 us cold, 10.7 us with the tokens still in L2), by
+// heads of 128, 74 MB: 16.8 us when the writes reach memory too, 10.7 us with all
+// of it in L2; the heads of a page side by side in the grid: 18.4 and 10.7), by
 // the launch for a decode step (64 tokens: 2.6 us in a chain of calls).
 template <int D>
 __global__ void __launch_bounds__(128)

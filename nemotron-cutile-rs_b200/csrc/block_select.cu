@@ -445,7 +445,10 @@ __device__ __forceinline__ K nth_largest(int j0, int j1, At at, int need, TopSha
     for (int i = threadIdx.x; i < 256; i += T) sh.hist[i] = 0;
     __syncthreads();  // the shared words are read, the bins are empty
     if (whole || shift == 0) return least;
-    most = least + (((K)1 << shift) - 1);
+    // The end of the bin, not past the largest key: least + span can pass the
+    // type's end (an infinite score's key is close to it).
+    const K span = ((K)1 << shift) - 1;
+    if (most - least > span) most = least + span;
   }
 }
 
@@ -518,7 +521,8 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
     for (int j = j0, i = 0; j - lane < j1; j += 32, ++i) {
       const bool take = i < 32 ? kept >> i & 1 : reaches(j);
       const uint32_t taken = __ballot_sync(0xffffffffu, take);
-      if (take) out[at + __popc(taken & below)] = j;
+      const int to = at + __popc(taken & below);
+      if (take && to < a.top_k) out[to] = j;
       at += __popc(taken);
     }
     return;
@@ -639,7 +643,8 @@ __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArg
     const uint32_t same = __ballot_sync(0xffffffffu, v == 2);
     const bool take = v == 1 || (v == 2 && eq + __popc(same & below) < room);
     const uint32_t taken = __ballot_sync(0xffffffffu, take);
-    if (take) out[at + __popc(taken & below)] = j;
+    const int to = at + __popc(taken & below);
+    if (take && to < a.top_k) out[to] = j;
     at += __popc(taken);
     eq += __popc(same);
   }

@@ -705,3 +705,32 @@ def test_large_magnitudes_rescale(cuda):
             want, mag = _reference(c, q, [T], H, "causal")
             # keys up to 12 times unit variance: 12 times the score's error bound
             _close(got, want, mag * (1 + 12 * 2.0**-3), True)
+
+
+@pytest.mark.parametrize("n,infinite,top_k", [(800, 200, 32), (1900, 129, 130), (1900, 700, 202),
+                                              (300, 200, 250)])
+@pytest.mark.parametrize("low", [8.0, 40.0, 2.0**100])
+def test_block_select_with_many_infinite_scores_among_finite_ones(cuda, n, infinite, top_k, low):
+    """A key channel that overflowed in many pages: more than 128 blocks in doubt, +inf
+    for some of them and large finite scores for the others, so that the search's
+    bins reach the last of the 64-bit keys.  Nothing is written behind a list."""
+    ps, d = 16, 64
+    c = Paged(n, [n * ps] * 2, 1, ps, d)
+    r = c.rng
+    low_, high = np.full((n, d), -1.0, np.float32), np.full((n, d), 0.0, np.float32)
+    high[:, 3] = bf16(low * (1 + r.random(n)))
+    high[1 + r.permutation(n - 2)[:infinite], 5] = np.inf
+    for s in range(2):
+        c.lo[0, c.table[s], 0], c.hi[0, c.table[s], 0] = low_, high
+    q = np.zeros((1, 2, d), np.float32)
+    q[:, :, 3], q[:, :, 5] = 1.0, 0.5
+    want = chosen_blocks(q[0], low_, high, n, top_k, 1, 1)
+    lists = torch.full((4, 1, top_k), -7, dtype=torch.int32, device="cuda")
+    nk.kv_block_select(dev(np.repeat(q.reshape(1, -1), 2, 0)).bfloat16(), c.device(),
+                       ints([0, 1, 2]), ints([n * ps] * 2), 2, top_k, max_q=1, max_kv=n * ps,
+                       out=lists[:2])
+    nk.device_status()
+    got = lists.cpu().numpy()
+    for s in range(2):
+        assert got[s, 0].tolist() == want.tolist()
+    assert (got[2:] == -7).all()

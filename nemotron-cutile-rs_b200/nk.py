@@ -859,12 +859,21 @@ def _stream_of(device, stream) -> int:
         torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _hold(stream, *tensors):
-    """Memory handed to an explicit stream is not given out again before the
-    stream's queued work is done with it."""
-    if stream is not None:
-        for t in tensors:
-            t.record_stream(stream)
+def _empty(shape, dtype, device, stream, result=True):
+    """New device memory for a call on `stream`.  On an explicit stream it comes
+    from that stream's memory: the current stream's may have been freed by work
+    that is still queued there.  result: the caller reads it on the current
+    stream, so it is not given out again before that stream's work is done with
+    it either."""
+    import torch
+
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if result:
+        t.record_stream(torch.cuda.current_stream(device))
+    return t
 
 
 class KvPages:
@@ -1039,8 +1048,7 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
             raise ValueError("dst_table must have a row for each sequence")
         dst, dst_ld = dst_table.data_ptr(), dst_table.stride(0) if n > 1 else dst_table.shape[1]
     if new_len is None:
-        new_len = torch.empty_like(kv_len, memory_format=torch.contiguous_format)
-        _hold(stream, new_len)
+        new_len = _empty(n, torch.int32, dev, stream)
     else:
         _expect_ints(new_len, "new_len", n, dev)
     width = keep.shape[1]
@@ -1068,13 +1076,12 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
             raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
         max_blocks = blocks.shape[2]
     if out is None:
-        if out_dtype == BF16 and ld_q == q.shape[1]:
+        if stream is None and out_dtype == BF16 and ld_q == q.shape[1]:
             out = torch.empty_like(q)
         else:
-            out = torch.empty(q.shape, device=dev,
-                              dtype=torch.float32 if out_dtype == F32 else torch.bfloat16)
+            out = _empty(q.shape, torch.float32 if out_dtype == F32 else torch.bfloat16, dev,
+                         stream)
         code = out_dtype
-        _hold(stream, out)
     elif out.shape != q.shape or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be contiguous, of q's shape and on its device")
     else:
@@ -1086,8 +1093,7 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
     if workspace is None:
         size = pages._attend_bytes(b, q_heads, max_blocks)
         if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-            _hold(stream, workspace)
+            workspace = _empty(size, torch.uint8, dev, stream, result=False)
     else:
         size = workspace.numel()
     _call_on(dev, "nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace), size,
@@ -1131,16 +1137,14 @@ def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspac
 
     dev, tokens = pages.device, q.shape[0]
     if out is None:
-        out = torch.empty(tokens, pages.kv_heads, max(top_k, 1), dtype=torch.int32, device=dev)
-        _hold(stream, out)
+        out = _empty((tokens, pages.kv_heads, max(top_k, 1)), torch.int32, dev, stream)
     else:
         _expect(out, "out", torch.int32, 3, dev)
         if out.shape != (tokens, pages.kv_heads, top_k) or not out.is_contiguous():
             raise ValueError("out must be contiguous [tokens, kv_heads, top_k]")
     br = ctypes.byref(b)
     if workspace is None:
-        workspace = torch.empty(pages._select_bytes(b), dtype=torch.uint8, device=dev)
-        _hold(stream, workspace)
+        workspace = _empty(pages._select_bytes(b), torch.uint8, dev, stream, result=False)
     _call_on(dev, "nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k,
              sink, local, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
              _stream_of(dev, stream))
@@ -1169,8 +1173,7 @@ def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k
     b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
     # One workspace for both: the selection is done with it when the attention starts.
     size = max(pages._select_bytes(b), pages._attend_bytes(b, q_heads, top_k))
-    workspace = torch.empty(size, dtype=torch.uint8, device=pages.device)
-    _hold(stream, workspace)
+    workspace = _empty(size, torch.uint8, pages.device, stream, result=False)
     blocks = _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, None, workspace,
                      stream)
     return _attend(pages, q, ld_q, b, q_heads, None, blocks, layer, scale, out_dtype, out,

@@ -93,10 +93,8 @@ class PagedKvCache:
     def _upload(self, values, stream):
         import torch
 
-        out = torch.empty(len(values), dtype=torch.int32, device=self.pages.device)
+        out = nk._empty(len(values), torch.int32, self.pages.device, stream)
         nk.kv_table_write(out, values, stream=stream)
-        if stream is not None:
-            out.record_stream(stream)
         return out
 
     # ---- state ------------------------------------------------------------------

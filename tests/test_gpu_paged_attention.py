@@ -734,3 +734,70 @@ def test_block_select_with_many_infinite_scores_among_finite_ones(cuda, n, infin
     for s in range(2):
         assert got[s, 0].tolist() == want.tolist()
     assert (got[2:] == -7).all()
+
+
+@pytest.mark.parametrize("call", ["attend", "select", "sparse", "compact", "step", "accept"])
+def test_a_call_on_another_stream_takes_no_memory_of_the_current_one(cuda, call):
+    """Blocks of every size the call needs are freed on the current stream while a
+    copy of them is still queued there; the call runs at once on its own stream."""
+    heads, d, ps, H, top_k, lens = 2, 64, 16, 8, 4, [9000, 333]
+    c = Paged(3, lens, heads, ps, d)
+    pages = c.device()
+    side = torch.cuda.Stream()
+    start, kv_len = ints([0, 1, 2]), ints(lens)
+    keep, n_keep, base = ints([[0], [0]]), ints([1, 1]), ints([n - 1 for n in lens])
+    q = torch.randn(2, H * d, device="cuda").bfloat16()
+    kw = dict(max_q=1, max_kv=9008)
+    sizes = [2 * H * d * 2, 2 * heads * top_k * 4, 8, 40, 4 * 7, 4 * 6,
+             nk.attention_paged_workspace_bytes(pages, 2, 2, H, max_q=1, max_kv=9008),
+             nk.attention_paged_workspace_bytes(pages, 2, 2, H, max_q=1, max_kv=9008,
+                                                max_blocks=top_k),
+             pages._select_bytes(pages.batch(start, kv_len, 2, 1, 9008))]
+    cache = nk_paged.PagedKvCache(9, heads, d, max_seqs=2, max_len=64, page_size=ps)
+    seqs = [cache.new_sequence(), cache.new_sequence()]
+    step = cache.step(seqs, [2, 2])
+
+    def run(stream):
+        if call == "attend":
+            return nk.attention_paged(q, pages, start, kv_len, H, stream=stream, **kw)
+        if call == "select":
+            return nk.kv_block_select(q, pages, start, kv_len, H, top_k, stream=stream, **kw)
+        if call == "sparse":
+            return nk.attention_paged_sparse(q, pages, start, kv_len, H, top_k, stream=stream, **kw)
+        if call == "compact":
+            return nk.kv_pages_compact(pages, kv_len, base, keep, n_keep, stream=stream)
+        if call == "step":
+            return cache.step(seqs, [1, 1], stream=stream)
+        return cache.accept(step, [[1], [0]], stream=stream)
+
+    planted = [torch.full((max(n, 1),), 90, dtype=torch.uint8, device="cuda")
+               for n in sizes for _ in range(2)]
+    copies = [torch.zeros_like(x) for x in planted]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)  # some 100 ms
+    for x, y in zip(planted, copies):
+        y.copy_(x)
+    del planted, x
+    got = run(side)
+    torch.cuda.synchronize()
+    nk.device_status()
+    assert all(bool((y == 90).all()) for y in copies)
+    del got
+
+
+def test_results_of_another_stream_live_until_they_are_read(cuda):
+    c = Paged(4, [700], 2, 16, 64)
+    pages, side = c.device(), torch.cuda.Stream()
+    qs = [torch.randn(1, 512, device="cuda").bfloat16() for _ in range(2)]
+    args, kw = (pages, ints([0, 1]), ints([700]), 8), dict(max_q=1, max_kv=700)
+    want = nk.attention_paged(qs[0], *args, **kw)
+    read = torch.empty_like(want)
+    torch.cuda.synchronize()
+    out = nk.attention_paged(qs[0], *args, stream=side, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda._sleep(200_000_000)
+    read.copy_(out)
+    del out
+    again = nk.attention_paged(qs[1], *args, stream=side, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(read, want) and not torch.equal(again, want)

@@ -119,8 +119,9 @@ __global__ void proj_simt_kernel(const void *__restrict__ x, int x_f32,
 // y[m, n] = act(Σ_s partial[s][m, n] + bias[n]), partial sums added in split order.
 // Launched as a programmatic dependent of the GEMM: its blocks are scheduled
 // while the GEMM runs and wait (griddepcontrol.wait) for its completion, so the
-// launch latency is hidden.  Loads of four splits are issued together.
-__global__ void splitk_reduce_kernel(const float *__restrict__ part, int splits, int64_t mn,
+// launch latency is hidden.  `part` is written while they wait: plain loads, not
+// the read-only path.  Loads of four splits are issued together.
+__global__ void splitk_reduce_kernel(const float *part, int splits, int64_t mn,
                                      int64_t n, const float *__restrict__ bias, int relu2,
                                      void *__restrict__ y, int y_f32) {
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -48,22 +48,26 @@ __device__ __forceinline__ void unpack16(const Packed16 &q, int8_t *, float (&v)
     v[i] = __uint_as_float(__byte_perm(w[i >> 2], 0x4B000000u, 0x7540 | (i & 3))) -
            8388736.0f;
 }
+// 16 elements of a token row.  Plain loads: the rows may have been written by the
+// kernel before, while this one was already launched, so they are not constant for
+// its lifetime as the read-only path asks (the weights are).
 __device__ __forceinline__ void load16(const __nv_bfloat16 *p, float (&v)[16]) {
   Packed16 q;
-  fetch16(p, q);
+  q.a = reinterpret_cast<const uint4 *>(p)[0];
+  q.b = reinterpret_cast<const uint4 *>(p)[1];
   unpack16(q, (__nv_bfloat16 *)nullptr, v);
 }
 __device__ __forceinline__ void load16(const float *p, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p) + i);
+    const float4 a = reinterpret_cast<const float4 *>(p)[i];
     v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
   }
 }
 
 // Block = 8 warps, warp w owns rows n0 + w*R .. +R-1; grid = (ceil(N / 8R), splits).
 template <typename WT, typename XT, int MT, int R>
-__global__ void __launch_bounds__(256, 2) gemv_kernel(const XT *__restrict__ x, int m,
+__global__ void __launch_bounds__(256, 2) gemv_kernel(const XT *x, int m,
                                                    const WT *__restrict__ w, int64_t n,
                                                    int64_t k, int64_t k_per_split, float w_scale,
                                                    const float *__restrict__ row_scale,

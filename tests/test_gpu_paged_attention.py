@@ -801,3 +801,60 @@ def test_results_of_another_stream_live_until_they_are_read(cuda):
     again = nk.attention_paged(qs[1], *args, stream=side, **kw)
     torch.cuda.synchronize()
     assert torch.equal(read, want) and not torch.equal(again, want)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4, 7])
+@pytest.mark.parametrize("bound", [64, 512, 9000])
+def test_projections_behind_attention_read_what_it_wrote(cuda, rows, bound):
+    """Attention into one buffer and the projection of it, many times back to back
+    (the projection is launched while the attention runs), give what they give with
+    a wait for the GPU between them."""
+    heads, H, d, steps = 2, 32, 128, 100
+    lens = [min(1 + 13 * s, bound) for s in range(rows)] if bound == 64 else [400 - 31 * s for s in range(rows)]
+    c = Paged(rows, lens, heads, 64, d)
+    pages, start, kv_len = c.device(), ints(starts([1] * rows)), ints(lens)
+    w = torch.randn(256, H * d, device="cuda").mul_(0.02).bfloat16()
+    qs = torch.randn(steps, rows, H * d, device="cuda").bfloat16()
+    out = torch.empty(rows, H * d, dtype=torch.bfloat16, device="cuda")
+    results = []
+    for wait in (True, False):
+        ys = []
+        for q in qs:
+            nk.attention_paged(q, pages, start, kv_len, H, max_q=1, max_kv=bound, out=out)
+            if wait:
+                torch.cuda.synchronize()
+            ys.append(nk.gemm(out, w, out_dtype=torch.float32))
+        torch.cuda.synchronize()
+        results.append(torch.stack(ys))
+    nk.device_status()
+    assert torch.equal(*results)
+    if max(lens) > 1:  # a single cached token is the output whatever the query
+        assert not torch.equal(results[0][0], results[0][1])
+
+
+@pytest.mark.parametrize("B", [1, 2])
+def test_decoder_of_one_and_two_rows_over_pages(cuda, B):
+    """Decode steps whose projections stream the weights: the same bar as for more
+    rows, and the same bits when each step waits for the one before."""
+    tiny = dict(vocab=512, hidden=128, pattern="*E*M", mamba_heads=4, mamba_head_dim=32,
+                mamba_groups=2, mamba_state=32, conv_kernel=4, experts=8, top_k=2, moe_inter=64,
+                shared_inter=128, q_heads=4, kv_heads=2, head_dim=64, std=0.08)
+    model = nk_model.Decoder(nk_model.DecoderConfig(**tiny))
+    T, steps = 21, 12
+    toks = dev(rng(5).integers(0, 512, (B, T + steps)).astype(np.int32))
+    feed = [(toks[:, :T].reshape(-1).contiguous(), T)] + \
+        [(toks[:, T + s].contiguous(), 1) for s in range(steps)]
+    plain = model.new_state(B, T + steps)
+    want = [model.forward(ids, B, n, plain) for ids, n in feed]
+    got = []
+    for wait in (True, False):
+        state = model.new_state(B, T + steps, page_size=16)
+        torch.cuda.synchronize()
+        got.append([])
+        for ids, n in feed:
+            got[-1].append(model.forward(ids, B, n, state))
+            if wait:
+                torch.cuda.synchronize()
+    nk.device_status()
+    for x, y, z in zip(want, *got):
+        assert rel_err(host(y), host(x)) <= 2e-2 and torch.equal(y, z)

@@ -195,10 +195,12 @@ struct Cursor {
       p.rows = a.group - g0 < R ? a.group - g0 : R;
       p.pos = p.prefix + token;
       p.list = a.blocks + ((int64_t)(seq.first + token) * a.pool.heads + p.head) * a.max_blocks;
-      // Entries behind the last block hold -1: no tiles for them.
+      // Entries behind the last block hold -1: no tiles for them.  The unit's
+      // tiles count an entry a block of the sequence; blocks that skipped entries
+      // push behind those belong to its last piece.
       const int e0 = (int)(((int64_t)p.t0 * kTile) >> a.pool.ps_log2);
       int64_t e1 = ((int64_t)p.t1 * kTile + a.pool.ps - 1) >> a.pool.ps_log2;
-      if (e1 > a.max_blocks) e1 = a.max_blocks;
+      if (p.last || e1 > a.max_blocks) e1 = a.max_blocks;
       int n_list = 0;
       for (int e = e0; e < e1; e += 32) {
         const int x = e + (int)(threadIdx.x & 31);
@@ -219,7 +221,7 @@ struct Cursor {
       }
     }
     const int have = (p.keys + kTile - 1) / kTile;
-    if (p.t1 > have) p.t1 = have > p.t0 ? have : p.t0;
+    if (p.t1 > have || (p.list && p.last)) p.t1 = have > p.t0 ? have : p.t0;
     left -= n;
     at += n;
     t += n;

@@ -858,3 +858,40 @@ def test_decoder_of_one_and_two_rows_over_pages(cuda, B):
     nk.device_status()
     for x, y, z in zip(want, *got):
         assert rel_err(host(y), host(x)) <= 2e-2 and torch.equal(y, z)
+
+
+@pytest.mark.parametrize("bound", [0, 9000])
+@pytest.mark.parametrize("ps,d,kv,group,lens", [
+    (128, 64, 2, 4, [256, 130, 1]), (16, 64, 2, 3, [700, 40, 333]), (64, 128, 1, 16, [1300, 64]),
+    (32, 64, 1, 40, [500, 77])])
+def test_lists_whose_blocks_stand_behind_skipped_entries(cuda, ps, d, kv, group, lens, bound):
+    """Negative, foreign and repeated entries before and between the blocks push
+    them past as many entries as the sequence has blocks, a tile or several."""
+    c = Paged(ps + group, lens, kv, ps, d)
+    n, H, r = len(lens), kv * group, c.rng
+    most = max(-(-x // ps) for x in lens)
+    width = 3 * most + 130
+    lists = np.full((n, kv, width), -1, np.int32)
+    clean = []
+    for s, x in enumerate(lens):
+        clean.append([])
+        held = -(-x // ps)
+        for h in range(kv):
+            keep = np.sort(r.choice(held, max(1, held // 2), replace=False))
+            at = np.sort(r.choice(width, len(keep), replace=False))
+            if h == 0:  # all of them at the list's end
+                at = np.arange(width - len(keep), width)
+            lists[s, h, at] = keep
+            if h and at[0] > 3:  # foreign ones in front
+                lists[s, h, :2] = [held, 10**6]
+            clean[-1].append(keep.tolist())
+    if lens[0] == 256:
+        lists[0, 0, :3], lists[0, 0, 3:], clean[0][0] = [-1, 0, 1], -1, [0, 1]
+        lists[1, 0, :4], lists[1, 0, 4:], clean[1][0] = [0, 0, 0, 1], -1, [0, 1]
+    q = bf16(r.standard_normal((n, H, d)))
+    got = nk.attention_paged(dev(q.reshape(n, -1)).bfloat16(), c.device(), ints(starts([1] * n)),
+                             ints(lens), H, max_q=1, max_kv=bound or max(lens), out_dtype=nk.F32,
+                             blocks=ints(lists))
+    nk.device_status()
+    want, mag = _reference(c, q, [1] * n, H, "blocks", lists=clean)
+    _close(got, want, mag, True)

@@ -1606,6 +1606,8 @@ static nk_status check_attention(const nk_kv_pages *kv, const nk_kv_batch *b,
     return fail(NK_UNSUPPORTED, "a tree holds at most 64 drafted tokens");
   if (a->blocks && (a->max_blocks <= 0 || a->max_blocks > (1 << 20)))
     return fail(NK_INVALID_PARAMS, "max_blocks must lie in 1 .. 2^20");
+  if (!a->blocks && a->max_blocks != 0)
+    return fail(NK_INVALID_PARAMS, "max_blocks without blocks");
   if (b->max_new * a->q_heads >= (1ll << 31) - 64)
     return fail(NK_UNSUPPORTED, "max_new * q_heads must be < 2^31 - 64");
   if (plan_attention(*kv, *b, *a).tiles >= 2147000000.0)

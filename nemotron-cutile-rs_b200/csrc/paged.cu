@@ -665,6 +665,8 @@ nk_status nk_kv_pages_compact(const nk_kv_pages *kv, const nk_kv_compact_args *a
     return fail(NK_INVALID_PARAMS, "more sequences than table rows");
   if (args->dst_table && (args->dst_ld <= 0 || args->dst_ld >= (1ll << 31)))
     return fail(NK_INVALID_PARAMS, "dst_ld must be positive and < 2^31");
+  if (!args->dst_table && args->dst_ld != 0)
+    return fail(NK_INVALID_PARAMS, "dst_ld without dst_table");
   int *err = device_error_ptr();
   if (!err) return fail(NK_DEVICE_ERROR, "cannot resolve device error word");
   const PagePool pool = page_pool(*kv);

@@ -1046,6 +1046,8 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
         _expect(dst_table, "dst_table", torch.int32, 2, dev)
         if dst_table.shape[0] != n:
             raise ValueError("dst_table must have a row for each sequence")
+        if dst_table.shape[1] == 0:  # its address would be none: in place
+            raise ValueError("dst_table must have a column")
         dst, dst_ld = dst_table.data_ptr(), dst_table.stride(0) if n > 1 else dst_table.shape[1]
     if new_len is None:
         new_len = _empty(n, torch.int32, dev, stream)
@@ -1074,7 +1076,9 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
         _expect(blocks, "blocks", torch.int32, 3, dev)
         if blocks.shape[:2] != (tokens, pages.kv_heads) or not blocks.is_contiguous():
             raise ValueError("blocks must be contiguous [tokens, kv_heads, n]")
-        max_blocks = blocks.shape[2]
+        if blocks.shape[2] == 0:  # its address would be none: attention without lists
+            raise ValueError("blocks must hold an entry a list")
+        max_blocks = blocks.shape[2] if tokens else 0
     if out is None:
         if stream is None and out_dtype == BF16 and ld_q == q.shape[1]:
             out = torch.empty_like(q)

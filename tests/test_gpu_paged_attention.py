@@ -895,3 +895,31 @@ def test_lists_whose_blocks_stand_behind_skipped_entries(cuda, ps, d, kv, group,
     nk.device_status()
     want, mag = _reference(c, q, [1] * n, H, "blocks", lists=clean)
     _close(got, want, mag, True)
+
+
+def test_empty_lists_and_tables_are_refused(cuda):
+    """A list of no entries is not attention without lists, a table of no columns
+    not a compaction in place."""
+    c = Paged(2, [40, 9], 2, 16, 64)
+    pages, start, kv_len = c.device(), ints([0, 1, 2]), ints([40, 9])
+    q = torch.randn(2, 256, device="cuda").bfloat16()
+    with pytest.raises(ValueError, match="an entry"):
+        nk.attention_paged(q, pages, start, kv_len, 4, max_q=1, max_kv=40,
+                           blocks=torch.empty(2, 2, 0, dtype=torch.int32, device="cuda"))
+    before = pages.k.clone()
+    with pytest.raises(ValueError, match="a column"):
+        nk.kv_pages_compact(pages, kv_len, ints([30, 0]), ints([[5], [1]]), ints([1, 1]),
+                            dst_table=torch.empty(2, 0, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(before.nan_to_num(), pages.k.nan_to_num())
+    # no tokens, no sequences: nothing to do
+    none, no = torch.empty(0, 256, dtype=torch.bfloat16, device="cuda"), ints([])
+    for lists in (None, torch.empty(0, 2, 8, dtype=torch.int32, device="cuda")):
+        out = nk.attention_paged(none, pages, ints([0, 0, 0]), kv_len, 4, max_q=0, blocks=lists)
+        assert out.shape == (0, 256)
+    out, lists = nk.attention_paged_sparse(none, pages, ints([0]), no, 4, 3, max_q=0)
+    assert out.shape == (0, 256) and lists.shape == (0, 2, 3)
+    got = nk.kv_pages_compact(pages, no, no, torch.empty(0, 3, dtype=torch.int32, device="cuda"),
+                              no, dst_table=torch.empty(0, 4, dtype=torch.int32, device="cuda"))
+    assert got.numel() == 0
+    nk.device_status()

@@ -411,3 +411,16 @@ def test_host_arrays_that_do_not_fit_are_refused():
         got = nk._host_ints(good, np.int32)
         assert got.dtype == np.int32 and got.flags.c_contiguous
         assert got.tolist() == list(map(int, good))
+
+
+def test_a_width_without_its_array_is_refused():
+    """An empty list or table has no address, which would mean none was given."""
+    lib, kv, n = nk.lib(), _pages(), ctypes.c_size_t()
+    for width in (1, 8, -1):
+        a = _attn(max_blocks=width)
+        assert lib.nk_attention_paged(_r(kv), 0, _r(_batch()), _r(a), None, 0, None) == \
+            nk.INVALID_PARAMS
+        assert lib.nk_attention_paged_workspace_bytes(_r(kv), _r(_batch()), _r(a), _r(n)) == \
+            nk.INVALID_PARAMS
+        c = nk.NkKvCompactArgs(2, None, 256, 256, 256, 4, 256, 4, None, width, None)
+        assert lib.nk_kv_pages_compact(_r(kv), _r(c), None) == nk.INVALID_PARAMS

@@ -500,6 +500,7 @@ __device__ __forceinline__ void load_tiles(const PagedAttn &a, Cursor<R> cur,
         }
         const bool now = load && (!SPLIT || is_v == half);
         const uint32_t mine = __ballot_sync(0xffffffffu, now);
+        __syncwarp();  // the limits of all lanes, ahead of the arrival that shows them
         if (lane == 0)
           mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(mine) * (uint32_t)box_rows * 128u);
         __syncwarp();

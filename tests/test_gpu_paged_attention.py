@@ -923,3 +923,34 @@ def test_empty_lists_and_tables_are_refused(cuda):
                               no, dst_table=torch.empty(0, 4, dtype=torch.int32, device="cuda"))
     assert got.numel() == 0
     nk.device_status()
+
+
+@pytest.mark.parametrize("ps,d,group", [(16, 64, 4), (32, 128, 16), (16, 128, 40), (64, 64, 48)])
+def test_tiles_without_pages_between_full_ones(cuda, ps, d, group):
+    """Lists whose tiles change between whole ones, ones with a page or two, ones
+    that end inside a page and ones with nothing to load (whose keys are counted
+    by the loader alone): the formula's result, the same bits fifty times."""
+    lens = [128 * 9 - 3, 128 * 5 + 1]
+    c = Paged(group, lens, 2, ps, d)
+    H, per, r = 2 * group, 128 // ps, c.rng
+    width = 12 * per
+    lists, clean = np.full((2, 2, width), -1, np.int32), [[], []]
+    for s, n in enumerate(lens):
+        held = -(-n // ps)
+        for h in range(2):
+            tiles = [x for x in range(12) if x % 3 != h]
+            slots = np.array([t * per + i for t in tiles for i in range(per)
+                              if t % 4 != 1 or i % per == t % per])[:held]
+            keep = np.sort(r.choice(held - 1, min(len(slots), held) - 1, replace=False)).tolist()
+            keep.append(held - 1)  # the sequence's last block, partly filled
+            lists[s, h, slots[:len(keep)]] = keep
+            clean[s].append(keep)
+    q = bf16(r.standard_normal((2, H, d)))
+    want, mag = _reference(c, q, [1, 1], H, "blocks", lists=clean)
+    args = (dev(q.reshape(2, -1)).bfloat16(), c.device(), ints([0, 1, 2]), ints(lens), H)
+    kw = dict(max_q=1, out_dtype=nk.F32, blocks=ints(lists))
+    for bound in (max(lens), 9000):
+        got = [nk.attention_paged(*args, max_kv=bound, **kw) for _ in range(50)]
+        nk.device_status()
+        _close(got[0], want, mag, True)
+        assert all(torch.equal(got[0], x) for x in got[1:])

@@ -1035,7 +1035,7 @@ __global__ void __launch_bounds__(320, 1)
   __shared__ __align__(16) int limits[C::kLimits][8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int odd[4];  // per piece: a value that only some rows see is no finite number
+  __shared__ int odd;  // some piece so far: a value that only some rows see is no finite number
   __shared__ Cursor<R> share;
   __shared__ int per;
 
@@ -1057,6 +1057,7 @@ __global__ void __launch_bounds__(320, 1)
     mbar_init(&drain, 1);
     fence_mbar_init();
     abort_flag = 0;
+    odd = 0;
   }
   if (threadIdx.x == 288) {
     tma_prefetch_desc(&kmap);
@@ -1183,8 +1184,6 @@ __global__ void __launch_bounds__(320, 1)
       // together.
       if (mine && ends_g > 0 && !warp_wait(&e_done[g], (ends_g - 1) & 1, &abort_flag)) break;
       if (mine && n > 0) {
-        // A is at most two pieces ahead of B, so four flags are enough.
-        if (threadIdx.x == 0) odd[piece & 3] = 0;
         // Queries: neighbouring threads load neighbouring 16 bytes of a row, 8
         // rows' loads in flight.
         uint8_t *qt = qs + g * (128 * D * 2);
@@ -1234,7 +1233,7 @@ __global__ void __launch_bounds__(320, 1)
             if (!live) break;
             if (clean_values<D>(ring + stage % STAGES * C::kTileBytes, r, 0, 1, lim,
                                 partial ? all_see - t * kTile : kTile))
-              odd[piece & 3] = 1;
+              odd = 1;
             __syncwarp();
           }
           // Keys of a chunk of 32 that this row sees, a bit each.
@@ -1339,7 +1338,10 @@ __global__ void __launch_bounds__(320, 1)
       if (mine) {
         const float f = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
         if (!whole && ok_row) a.part_ml[(int64_t)slot * R + r] = make_float2(m, l);
-        const bool bad = n > 0 && odd[piece & 3];
+        // One flag, never cleared: A may be any number of pieces ahead of B, which
+        // skips pieces without rows of its own.  For a piece that took nothing out
+        // poison adds 0.
+        const bool bad = n > 0 && *(volatile int *)&odd;
         // Through shared memory (the queries' tile is free): a thread holds a
         // row, a store instruction writes 4 rows of 32 columns.
         float4 *stage = reinterpret_cast<float4 *>(qs + g * (128 * D * 2) + (warp & 3) * 4096);

@@ -954,3 +954,36 @@ def test_tiles_without_pages_between_full_ones(cuda, ps, d, group):
         nk.device_status()
         _close(got[0], want, mag, True)
         assert all(torch.equal(got[0], x) for x in got[1:])
+
+
+@pytest.mark.parametrize("value", [1.0, np.inf, np.nan])
+@pytest.mark.parametrize("kind", ["tree", "causal"])
+def test_more_wide_units_than_blocks(cuda, kind, value):
+    """Units of up to 256 rows, several to a block one after the other, whole ones
+    and parts, two row tiles and one in turn; a value of some drafts is no finite
+    number, which rows of other branches and earlier tokens do not see."""
+    kv, group, d, ps = 2, 4, 64, 32
+    counts = [(64, 3, 64, 20, 1, 33, 9, 64, 0, 40)[s % 10] for s in range(110)]
+    r = np.random.default_rng(11)
+    lens = [t + int(r.integers(0, 300)) for t in counts]
+    lens[17] = 2500
+    c = Paged(77, [max(1, n) for n in lens], kv, ps, d)
+    lens = c.lens
+    H, T = kv * group, sum(counts)
+    masks, words = [], []
+    for s, t in enumerate(counts):
+        w, seen = tree_masks(c.rng, t)
+        masks.append(seen)
+        words.append(w)
+        if t and s % 3 == 0:
+            p, x = c.slot(s, int(lens[s]) - t + t // 2)
+            c.v[0, p, s % kv, x, s % d] = value
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    tree = torch.from_numpy(np.concatenate(words)).cuda() if kind == "tree" else None
+    want, mag = _reference(c, q, counts, H, kind, masks)
+    args = (dev(q.reshape(T, -1)).bfloat16(), c.device(), ints(starts(counts)), ints(lens), H)
+    got = [nk.attention_paged(*args, max_q=64, max_kv=2500, tree_mask=tree, out_dtype=nk.F32)
+           for _ in range(3)]
+    nk.device_status()
+    _close(got[0], want, np.where(np.isfinite(mag), mag, 0), True)
+    assert all(torch.equal(got[0].nan_to_num(7.0), x.nan_to_num(7.0)) for x in got[1:])

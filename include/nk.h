@@ -770,7 +770,9 @@ nk_status nk_kv_table_write(int32_t *dst, int64_t dst_len, const int64_t *offset
  * Otherwise the tokens go to the pages of dst_table [seqs, dst_ld] (a context
  * thinned into fresh pages); a page written must not be read as a source.
  * Refused entries (not ascending, past kv_len) leave their slot unwritten.
- * A page that is written must belong to one sequence of the call only. */
+ * A page that is written must belong to one sequence of the call only, and
+ * new_len must not share memory with an array that the call reads (refused: the
+ * blocks of a call read the lengths in no order). */
 typedef struct nk_kv_compact_args {
   int64_t seqs;             /* <= 65535 */
   const int32_t *rows;      /* [seqs] table row of each sequence; NULL: row b */

@@ -447,6 +447,12 @@ nk_status check_batch(const nk_kv_pages *kv, const nk_kv_batch *b) {
   return NK_OK;
 }
 
+// Whether two arrays of int32 share memory.
+static bool overlap(const int32_t *a, int64_t na, const int32_t *b, int64_t nb) {
+  return a && b && na > 0 && nb > 0 && (uintptr_t)a < (uintptr_t)(b + nb) &&
+         (uintptr_t)b < (uintptr_t)(a + na);
+}
+
 static nk_status fail_page(int64_t page, int64_t pages, int64_t index) {
   nk_status st = fail(NK_PAGE_OUT_OF_RANGE, "page id out of range");
   tls_error().actual = (uint64_t)page;
@@ -667,6 +673,14 @@ nk_status nk_kv_pages_compact(const nk_kv_pages *kv, const nk_kv_compact_args *a
     return fail(NK_INVALID_PARAMS, "dst_ld must be positive and < 2^31");
   if (!args->dst_table && args->dst_ld != 0)
     return fail(NK_INVALID_PARAMS, "dst_ld without dst_table");
+  // One block writes a sequence's new length while others still read its arrays.
+  const int64_t n = args->seqs;
+  if (overlap(args->new_len, n, args->rows, n) || overlap(args->new_len, n, args->kv_len, n) ||
+      overlap(args->new_len, n, args->base, n) || overlap(args->new_len, n, args->n_keep, n) ||
+      overlap(args->new_len, n, args->keep, (n - 1) * args->keep_ld + args->max_keep) ||
+      overlap(args->new_len, n, args->dst_table, n * args->dst_ld) ||
+      overlap(args->new_len, n, kv->table, kv->table_rows * kv->table_ld))
+    return fail(NK_INVALID_PARAMS, "new_len must not overlap the arrays that the call reads");
   int *err = device_error_ptr();
   if (!err) return fail(NK_DEVICE_ERROR, "cannot resolve device error word");
   const PagePool pool = page_pool(*kv);

@@ -1030,7 +1030,8 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
     """Token base[b] + keep[b, i] of sequence b moves to position base[b] + i
     (nk_kv_pages_compact), in place or into the pages of dst_table; all
     arguments int32 on the device, keep [n, max_keep] strictly ascending.
-    Returns the new lengths base + n_keep."""
+    Returns the new lengths base + n_keep, in new_len where it is given (not an
+    array that the call reads)."""
     import torch
 
     n, dev = kv_len.numel(), pages.device

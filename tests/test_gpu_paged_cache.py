@@ -403,3 +403,18 @@ def test_cache_grows_forks_and_frees(cuda):
     for s in sorted(model):
         cache.free(s)
     assert cache.free_pages == 40
+
+
+def test_new_lengths_beside_the_other_arrays(cuda):
+    """The batch arrays of a call cut from one buffer, new_len next to them."""
+    c = Paged(5, [40, 30], 1, 16, 64, filler=0.0)
+    buf = ints([40, 30, 38, 20, 1, 2, -1, -1, 1, 0, 0, 9])
+    kv_len, base, n_keep, new_len = (buf[i:i + 2] for i in (0, 2, 4, 6))
+    got = nk.kv_pages_compact(c.device(), kv_len, base, buf[8:].view(2, 2), n_keep,
+                              new_len=new_len)
+    nk.device_status()
+    assert got.data_ptr() == new_len.data_ptr()
+    assert buf.tolist() == [40, 30, 38, 20, 1, 2, 39, 22, 1, 0, 0, 9]
+    with pytest.raises(nk.NkError) as e:
+        nk.kv_pages_compact(c.device(), kv_len, base, buf[8:].view(2, 2), n_keep, new_len=kv_len)
+    assert e.value.code == nk.INVALID_PARAMS

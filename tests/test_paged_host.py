@@ -424,3 +424,16 @@ def test_a_width_without_its_array_is_refused():
             nk.INVALID_PARAMS
         c = nk.NkKvCompactArgs(2, None, 256, 256, 256, 4, 256, 4, None, width, None)
         assert lib.nk_kv_pages_compact(_r(kv), _r(c), None) == nk.INVALID_PARAMS
+
+
+@pytest.mark.parametrize("name,at", [
+    ("kv_len", 0), ("kv_len", 8), ("kv_len", -8), ("base", 0), ("n_keep", 4), ("rows", -4),
+    ("keep", 0), ("keep", 36), ("dst_table", 56), ("table", 60)])
+def test_new_lengths_over_an_array_that_is_read_are_refused(name, at):
+    lib, kv = nk.lib(), _pages()
+    f = dict(seqs=3, rows=2048, kv_len=4096, base=8192, keep=16384, keep_ld=4, n_keep=32768,
+             max_keep=2, dst_table=65536, dst_ld=5)
+    f["new_len"] = (256 if name == "table" else f[name]) + at
+    a = nk.NkKvCompactArgs(*(f[n] for n, _ in nk.NkKvCompactArgs._fields_))
+    assert lib.nk_kv_pages_compact(_r(kv), _r(a), None) == nk.INVALID_PARAMS
+    assert b"new_len" in nk.last_error().message

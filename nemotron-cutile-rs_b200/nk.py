@@ -903,9 +903,12 @@ class KvPages:
         self.k, self.v, self.table, self.k_min, self.k_max = k, v, table, k_min, k_max
         self.layers, self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.device = dev
+        # The library takes a row for table_ld entries long.  Where rows lie further
+        # apart, max_kv holds a batch to the columns that are there.
+        ld = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+        self._apart = ld > table.shape[1]
         self._struct = NkKvPages(*k.shape, ptr(k), ptr(v), ptr(k_min), ptr(k_max), ptr(table),
-                                 table.shape[0], table.stride(0) if table.shape[0] > 1
-                                 else table.shape[1])
+                                 table.shape[0], ld)
         self._ref = ctypes.byref(self._struct)
         self._bytes = {}  # bounds of an attention call -> its workspace bytes
 
@@ -918,8 +921,9 @@ class KvPages:
         _expect_ints(kv_len, "kv_len", n, self.device)
         if rows is not None:
             _expect_ints(rows, "rows", n, self.device)
-        if max_kv is None:
-            max_kv = self.table.shape[1] * self.page_size
+        if max_kv is None or self._apart:
+            held = self.table.shape[1] * self.page_size
+            max_kv = held if max_kv is None else min(max_kv, held)
         return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(),
                          None if rows is None else rows.data_ptr(), max_new, max_kv)
 
@@ -1025,6 +1029,17 @@ def kv_table_write(dst, values, offsets=None, stream=None) -> None:
              _stream_of(dst.device, stream))
 
 
+def _rows_together(table, stream):
+    """A page table that the call only reads, its rows one behind the other: the
+    device checks lengths against the distance of rows."""
+    import torch
+
+    if table.shape[0] <= 1 or table.stride(0) == table.shape[1]:
+        return table
+    with torch.cuda.stream(stream):  # None: the current one
+        return table.contiguous()
+
+
 def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, dst_table=None,
                      new_len=None, stream=None):
     """Token base[b] + keep[b, i] of sequence b moves to position base[b] + i
@@ -1049,7 +1064,8 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
             raise ValueError("dst_table must have a row for each sequence")
         if dst_table.shape[1] == 0:  # its address would be none: in place
             raise ValueError("dst_table must have a column")
-        dst, dst_ld = dst_table.data_ptr(), dst_table.stride(0) if n > 1 else dst_table.shape[1]
+        dst_table = _rows_together(dst_table, stream)
+        dst, dst_ld = dst_table.data_ptr(), dst_table.shape[1]
     if new_len is None:
         new_len = _empty(n, torch.int32, dev, stream)
     else:
@@ -1058,7 +1074,13 @@ def kv_pages_compact(pages: KvPages, kv_len, base, keep, n_keep, *, rows=None, d
     a = NkKvCompactArgs(n, ptr(rows), kv_len.data_ptr(), base.data_ptr(), keep.data_ptr(),
                         keep.stride(0) if n > 1 else width, n_keep.data_ptr(), width, dst, dst_ld,
                         new_len.data_ptr())
-    _call_on(dev, "nk_kv_pages_compact", pages._ref, ctypes.byref(a), _stream_of(dev, stream))
+    kv = pages._ref
+    if pages._apart:
+        table = _rows_together(pages.table, stream)
+        kv = NkKvPages.from_buffer_copy(pages._struct)
+        kv.table, kv.table_ld = table.data_ptr(), table.shape[1]
+        kv = ctypes.byref(kv)
+    _call_on(dev, "nk_kv_pages_compact", kv, ctypes.byref(a), _stream_of(dev, stream))
     return new_len
 
 

@@ -418,3 +418,57 @@ def test_new_lengths_beside_the_other_arrays(cuda):
     with pytest.raises(nk.NkError) as e:
         nk.kv_pages_compact(c.device(), kv_len, base, buf[8:].view(2, 2), n_keep, new_len=kv_len)
     assert e.value.code == nk.INVALID_PARAMS
+
+
+def _apart(a, extra, device="cuda"):
+    """The table as columns of a wider buffer, whose other entries are valid pages."""
+    wide = torch.zeros(a.shape[0], a.shape[1] + extra, dtype=torch.int32, device=device)
+    wide[:, :a.shape[1]] = ints(a)
+    return wide[:, :a.shape[1]]
+
+
+def test_tables_whose_rows_lie_apart(cuda):
+    """The same results as with a table of its own, and lengths past the table's
+    columns are refused although its rows are longer in memory."""
+    lens, base, n_keep = [60, 33], [20, 0], [18, 30]
+    c = Paged(4, lens, 1, 16, 64, spare=12, width=4, filler=0.0)
+    dst = c.spare[:8].reshape(2, 4)
+    keeps = ints([sorted(c.rng.choice(n - b, 30, replace=False)) for n, b in zip(lens, base)])
+    kn, vn = torch.randn(2, 5, 64, device="cuda").bfloat16()
+    q = torch.randn(5, 128, device="cuda").bfloat16()
+    pools = []
+    for apart in (False, True):
+        pages = c.device()
+        if apart:
+            pages = nk.KvPages(pages.k, pages.v, _apart(c.table, 7), k_min=pages.k_min,
+                               k_max=pages.k_max)
+        nk.kv_pages_append(pages, kn, vn, ints([0, 2, 5]), ints(lens), max_new=3, max_kv=100)
+        out = nk.attention_paged(q, pages, ints([0, 2, 5]), ints(lens), 2, max_q=3, max_kv=100)
+        sparse = nk.attention_paged_sparse(q, pages, ints([0, 2, 5]), ints(lens), 2, 2, max_q=3)
+        moved = nk.kv_pages_compact(pages, ints(lens), ints(base), keeps, ints(n_keep),
+                                    dst_table=_apart(dst, 5) if apart else ints(dst))
+        nk.device_status()
+        pools.append([pages.k, pages.v, pages.k_min, pages.k_max, out, *sparse, moved])
+        nk.kv_pages_compact(pages, ints(lens), ints(base), keeps, ints(n_keep))
+        nk.device_status()
+        # 66 tokens do not fit four columns of 16
+        before = [x.clone() for x in pools[-1]]
+        for call in (
+                lambda: nk.kv_pages_append(pages, kn, vn, ints([0, 2, 5]), ints([33, 66]),
+                                           max_new=3, max_kv=100, rows=ints([0, 1])),
+                lambda: nk.kv_pages_compact(pages, ints([66, 66]), ints([60, 60]), ints([[5], [5]]),
+                                            ints([1, 1])),
+                lambda: nk.kv_pages_compact(pages, ints([60, 33]), ints([0, 0]),
+                                            ints([list(range(40))] * 2), ints([0, 33]),
+                                            dst_table=_apart(dst[:, :2], 9)),
+                lambda: nk.attention_paged(q, pages, ints([0, 2, 5]), ints([66, 66]), 2, max_q=3,
+                                           max_kv=100, out=pools[-1][4]),
+                lambda: nk.kv_block_select(q, pages, ints([0, 2, 5]), ints([66, 66]), 2, 2, max_q=3,
+                                           max_kv=100, out=pools[-1][6])):
+            call()
+            with pytest.raises(nk.NkError) as e:
+                nk.device_status()
+            assert e.value.code == nk.INVALID_PARAMS
+        assert all(torch.equal(x, y) for x, y in zip(before[4:], pools[-1][4:]))
+    for x, y in zip(*pools):
+        assert torch.equal(x, y)

@@ -915,7 +915,8 @@ class KvPages:
     def batch(self, start, kv_len, tokens, max_new, max_kv=None, rows=None) -> NkKvBatch:
         """The ragged batch of one step (nk_kv_batch): start int32 [n + 1],
         kv_len int32 [n], rows int32 [n] or None on the pages' device; max_kv
-        defaults to what the table can hold."""
+        defaults to what the table can hold, max_new None is all tokens, or
+        max_kv where a sequence cannot hold them all."""
         n = kv_len.numel()
         _expect_ints(start, "start", n + 1, self.device)
         _expect_ints(kv_len, "kv_len", n, self.device)
@@ -924,6 +925,8 @@ class KvPages:
         if max_kv is None or self._apart:
             held = self.table.shape[1] * self.page_size
             max_kv = held if max_kv is None else min(max_kv, held)
+        if max_new is None:
+            max_new = min(tokens, max_kv)
         return NkKvBatch(n, tokens, start.data_ptr(), kv_len.data_ptr(),
                          None if rows is None else rows.data_ptr(), max_new, max_kv)
 
@@ -1139,13 +1142,15 @@ def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=Non
     (int64 [tokens], bit j: the sequence's new token j) every cached position
     and the drafts of its branch; with blocks (int32 [tokens, kv_heads, n],
     kv_block_select) the listed blocks.  max_q and max_kv bound the new tokens
-    and the length of a sequence (defaults: all tokens, the table's width);
-    close bounds cost less.  Returns [tokens, q_heads * head_dim] in bf16, or
-    f32 with out_dtype=F32; rows that belong to no sequence stay as they were
-    (a new `out` is not initialised).  workspace: optional uint8 device tensor
-    of attention_paged_workspace_bytes."""
+    and the length of a sequence (defaults: all tokens, but no more than max_kv
+    and, with tree_mask, 64; the table's width); close bounds cost less.  Returns
+    [tokens, q_heads * head_dim] in bf16, or f32 with out_dtype=F32; rows that
+    belong to no sequence stay as they were (a new `out` is not initialised).
+    workspace: optional uint8 device tensor of attention_paged_workspace_bytes."""
     tokens, ld_q = pages._queries(q, q_heads)
-    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    b = pages.batch(start, kv_len, tokens, max_q, max_kv, rows)
+    if max_q is None and tree_mask is not None and b.max_new > 64:
+        b.max_new = 64
     return _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dtype, out,
                    workspace, stream)
 
@@ -1185,7 +1190,7 @@ def kv_block_select(q, pages: KvPages, start, kv_len, q_heads: int, top_k: int, 
     kv_heads, top_k], ascending, -1 behind the last; the first `sink` and last
     `local` blocks and those whose key bounds allow the largest scores."""
     tokens, ld_q = pages._queries(q, q_heads)
-    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    b = pages.batch(start, kv_len, tokens, max_q, max_kv, rows)
     return _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspace, stream)
 
 
@@ -1197,7 +1202,7 @@ def attention_paged_sparse(q, pages: KvPages, start, kv_len, q_heads: int, top_k
     import torch
 
     tokens, ld_q = pages._queries(q, q_heads)
-    b = pages.batch(start, kv_len, tokens, tokens if max_q is None else max_q, max_kv, rows)
+    b = pages.batch(start, kv_len, tokens, max_q, max_kv, rows)
     # One workspace for both: the selection is done with it when the attention starts.
     size = max(pages._select_bytes(b), pages._attend_bytes(b, q_heads, top_k))
     workspace = _empty(size, torch.uint8, pages.device, stream, result=False)

@@ -987,3 +987,29 @@ def test_more_wide_units_than_blocks(cuda, kind, value):
     nk.device_status()
     _close(got[0], want, np.where(np.isfinite(mag), mag, 0), True)
     assert all(torch.equal(got[0].nan_to_num(7.0), x.nan_to_num(7.0)) for x in got[1:])
+
+
+def test_default_bounds_of_a_batch_longer_than_a_sequence(cuda):
+    """More tokens in all than one sequence can hold, without bounds given."""
+    lens = [16, 7, 1] * 8
+    c = Paged(9, lens, 2, 16, 64)
+    n, H = len(lens), 4
+    q = bf16(c.rng.standard_normal((n, H, 64)))
+    args = (dev(q.reshape(n, -1)).bfloat16(), c.device(), ints(starts([1] * n)), ints(lens), H)
+    want, mag = _reference(c, q, [1] * n, H, "causal")
+    _close(nk.attention_paged(*args), want, mag)
+    out, blocks = nk.attention_paged_sparse(*args, 2)
+    _close(out, want, mag)
+    assert torch.equal(blocks, nk.kv_block_select(*args, 2))
+    _close(nk.attention_paged(*args, max_kv=20, out_dtype=nk.F32), want, mag, True)
+    nk.device_status()
+    # trees of 30 drafts, 90 in all
+    c, counts = Paged(10, [100, 30, 64], 2, 16, 64), [30, 30, 30]
+    trees = [tree_masks(c.rng, 30) for _ in counts]
+    q = bf16(c.rng.standard_normal((90, H, 64)))
+    got = nk.attention_paged(dev(q.reshape(90, -1)).bfloat16(), c.device(), ints(starts(counts)),
+                             ints([100, 30, 64]), H,
+                             tree_mask=torch.from_numpy(np.concatenate([w for w, _ in trees])).cuda())
+    nk.device_status()
+    want, mag = _reference(c, q, counts, H, "tree", [m for _, m in trees])
+    _close(got, want, mag)

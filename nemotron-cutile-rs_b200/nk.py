@@ -10,6 +10,7 @@ and the same error variants, raised as NkError with the variant's payload.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 from dataclasses import dataclass
@@ -993,7 +994,13 @@ def kv_pages_append(pages: KvPages, k_new, v_new, start, kv_len, *, max_new, max
 def _host_ints(a, dtype):
     import numpy as np
 
-    if isinstance(a, np.ndarray) and a.dtype != dtype and a.size:
+    if isinstance(a, (list, tuple, range)):  # an array.array takes whole numbers that fit
+        try:
+            return np.frombuffer(array.array("i" if dtype is np.int32 else "q", a), dtype)
+        except TypeError:
+            raise ValueError(f"not a sequence of whole numbers: {a}") from None
+    a = np.asarray(a)
+    if a.dtype != dtype and a.size:
         b = a.astype(dtype)
         if a.dtype.kind not in "iu" or (b != a).any():
             raise ValueError(f"{a.dtype} values do not fit {np.dtype(dtype)}")

@@ -437,3 +437,17 @@ def test_new_lengths_over_an_array_that_is_read_are_refused(name, at):
     a = nk.NkKvCompactArgs(*(f[n] for n, _ in nk.NkKvCompactArgs._fields_))
     assert lib.nk_kv_pages_compact(_r(kv), _r(a), None) == nk.INVALID_PARAMS
     assert b"new_len" in nk.last_error().message
+
+
+@pytest.mark.parametrize("bad", [
+    [1.5], [1, 2.0], (0.0,), [np.float32(3)], [None], ["1"], [2**70], [[1], [2.5]],
+    np.array([2.5], object), np.array([True])])
+def test_host_lists_that_are_no_whole_numbers_are_refused(bad):
+    """A list of fractions must not turn into the pages below them."""
+    with pytest.raises((ValueError, OverflowError, TypeError)):
+        nk._host_ints(bad, np.int32)
+    for good in ([1, np.int64(2)], (3,), range(4), [], 7, [2**31 - 1, -2**31]):
+        assert nk._host_ints(good, np.int32).tolist() == np.atleast_1d(good).tolist()
+    with pytest.raises(OverflowError):
+        nk._host_ints([2**31], np.int32)
+    assert nk._host_ints([2**40], np.int64).tolist() == [2**40]

@@ -939,12 +939,7 @@ class KvPages:
             # of the pointers only whether they are there is read
             a = NkPagedAttentionArgs(None, q_heads * self.head_dim, q_heads, None,
                                      16 if max_blocks else None, max_blocks, 0, 0.0, None, BF16)
-            need = ctypes.c_size_t(0)
-            _call_on(self.device, "nk_attention_paged_workspace_bytes", self._ref,
-                     ctypes.byref(b), ctypes.byref(a), ctypes.byref(need))
-            if len(self._bytes) > 4096:
-                self._bytes.clear()
-            size = self._bytes[key] = need.value
+            size = self._ask_bytes(key, "nk_attention_paged_workspace_bytes", b, ctypes.byref(a))
         return size
 
     def _select_bytes(self, b):
@@ -952,10 +947,15 @@ class KvPages:
         key = (b.tokens, b.seqs, b.max_new, b.max_kv)
         size = self._bytes.get(key)
         if size is None:
-            need = ctypes.c_size_t(0)
-            _call_on(self.device, "nk_kv_block_select_workspace_bytes", self._ref,
-                     ctypes.byref(b), ctypes.byref(need))
-            size = self._bytes[key] = need.value
+            size = self._ask_bytes(key, "nk_kv_block_select_workspace_bytes", b)
+        return size
+
+    def _ask_bytes(self, key, name, b, *args):
+        need = ctypes.c_size_t(0)
+        _call_on(self.device, name, self._ref, ctypes.byref(b), *args, ctypes.byref(need))
+        if len(self._bytes) > 4096:  # lengths that grow with each step
+            self._bytes.clear()
+        size = self._bytes[key] = need.value
         return size
 
     def _queries(self, q, q_heads):

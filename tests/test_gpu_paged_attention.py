@@ -1013,3 +1013,16 @@ def test_default_bounds_of_a_batch_longer_than_a_sequence(cuda):
     nk.device_status()
     want, mag = _reference(c, q, counts, H, "tree", [m for _, m in trees])
     _close(got, want, mag)
+
+
+def test_workspace_sizes_kept_are_bounded(cuda):
+    """A bound that grows with every step does not grow the host's memory, and the
+    sizes are those that the library asks for."""
+    pages = Paged(1, [20], 1, 16, 64).device()
+    start, kv_len = ints([0, 1]), ints([20])
+    for n in range(1, 9001):
+        assert pages._select_bytes(pages.batch(start, kv_len, 1, 1, n)) == -(-n // 16) * 16
+        assert len(pages._bytes) <= 4097
+    sizes = [nk.attention_paged_workspace_bytes(pages, 1, 1, 2, max_q=1, max_kv=n)
+             for n in (100, 5000, 100)]
+    assert sizes[0] == sizes[2] == 0 < sizes[1]

@@ -877,6 +877,16 @@ def _empty(shape, dtype, device, stream, result=True):
     return t
 
 
+def _bytes_of(workspace, device) -> int:
+    """Size of a workspace that the caller may have given."""
+    import torch
+
+    if workspace.dtype is not torch.uint8 or workspace.device != device or \
+            not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 memory of {device}")
+    return workspace.numel()
+
+
 class KvPages:
     """A pool of KV pages and the table that strings them into sequences
     (nk_kv_pages): k, v bf16 [layers, pages, kv_heads, page_size, head_dim],
@@ -1132,7 +1142,7 @@ def _attend(pages, q, ld_q, b, q_heads, tree_mask, blocks, layer, scale, out_dty
         if size:
             workspace = _empty(size, torch.uint8, dev, stream, result=False)
     else:
-        size = workspace.numel()
+        size = _bytes_of(workspace, dev)
     _call_on(dev, "nk_attention_paged", pages._ref, layer, br, ar, ptr(workspace), size,
              _stream_of(dev, stream))
     return out
@@ -1185,7 +1195,7 @@ def _select(pages, q, ld_q, b, q_heads, top_k, sink, local, layer, out, workspac
     if workspace is None:
         workspace = _empty(pages._select_bytes(b), torch.uint8, dev, stream, result=False)
     _call_on(dev, "nk_kv_block_select", pages._ref, layer, br, q.data_ptr(), ld_q, q_heads, top_k,
-             sink, local, out.data_ptr(), workspace.data_ptr(), workspace.numel(),
+             sink, local, out.data_ptr(), workspace.data_ptr(), _bytes_of(workspace, dev),
              _stream_of(dev, stream))
     return out
 

@@ -1026,3 +1026,22 @@ def test_workspace_sizes_kept_are_bounded(cuda):
     sizes = [nk.attention_paged_workspace_bytes(pages, 1, 1, 2, max_q=1, max_kv=n)
              for n in (100, 5000, 100)]
     assert sizes[0] == sizes[2] == 0 < sizes[1]
+
+
+def test_workspaces_of_another_device_or_type_are_refused(cuda):
+    c = Paged(4, [300], 1, 16, 64)
+    pages, q = c.device(), torch.randn(1, 128, device="cuda").bfloat16()
+    args, kw = (q, pages, ints([0, 1]), ints([300]), 2), dict(max_q=1, max_kv=9000)
+    need = nk.attention_paged_workspace_bytes(pages, 1, 1, 2, max_q=1, max_kv=9000)
+    for bad in (torch.empty(need, dtype=torch.uint8), torch.empty(need, device="cuda"),
+                torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            nk.attention_paged(*args, workspace=bad, **kw)
+        with pytest.raises(ValueError, match="workspace"):
+            nk.kv_block_select(*args, 3, workspace=bad, **kw)
+    ws = torch.empty(need + (1 << 20), dtype=torch.uint8, device="cuda")
+    assert torch.equal(nk.attention_paged(*args, workspace=ws, **kw),
+                       nk.attention_paged(*args, **kw))
+    assert torch.equal(nk.kv_block_select(*args, 3, workspace=ws, **kw),
+                       nk.kv_block_select(*args, 3, **kw))
+    nk.device_status()

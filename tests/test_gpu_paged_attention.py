@@ -1045,3 +1045,57 @@ def test_workspaces_of_another_device_or_type_are_refused(cuda):
     assert torch.equal(nk.kv_block_select(*args, 3, workspace=ws, **kw),
                        nk.kv_block_select(*args, 3, **kw))
     nk.device_status()
+
+
+@pytest.mark.parametrize("kv,group,bound", [(2, 4, 0), (2, 4, 9000), (1, 24, 9000), (1, 40, 0),
+                                            (2, 40, 9000)])
+def test_more_sequences_than_threads(cuda, kv, group, bound):
+    """700 sequences, whose tiles the threads of a block count in runs of two or
+    three; some have no new token, one is much longer than the others."""
+    n, d, ps = 700, 64, 16
+    r = np.random.default_rng(kv + group)
+    lens = 1 + r.integers(0, 150, n)
+    lens[[0, 333, 699]] = [129, 1900, 64]
+    counts = [0 if s % 7 == 3 else 1 for s in range(n)]
+    c = Paged(group, lens, kv, ps, d)
+    H, T = kv * group, sum(counts)
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    want, mag = _reference(c, q, counts, H, "causal")
+    got = nk.attention_paged(dev(q.reshape(T, -1)).bfloat16(), c.device(), ints(starts(counts)),
+                             ints(lens), H, max_q=1, max_kv=bound or 1900)
+    nk.device_status()
+    _close(got, want, mag)
+    out, blocks = nk.attention_paged_sparse(dev(q.reshape(T, -1)).bfloat16(), c.device(),
+                                            ints(starts(counts)), ints(lens), H, 3, max_q=1,
+                                            max_kv=bound or 1900)
+    nk.device_status()
+    want, mag = _reference(c, q, counts, H, "blocks", lists=blocks.cpu().numpy())
+    _close(out, want, mag)
+
+
+@pytest.mark.parametrize("kv,group,d,ps,lens,counts", [
+    (2, 16, 64, 64, [1300], [1300]),                        # one prompt, 164 units
+    (1, 8, 128, 32, [700, 1, 2100, 900], [700, 1, 600, 899]),  # behind cached prefixes too
+    (4, 16, 64, 16, [200] * 12 + [31, 1], [200] * 12 + [30, 1])])
+def test_prompts_of_more_units_than_blocks(cuda, kv, group, d, ps, lens, counts):
+    """Prompt chunks whose row tiles outnumber the SMs: a block runs several
+    units, whole ones and parts, each up to its own causal limit."""
+    c = Paged(kv + d, lens, kv, ps, d)
+    H, T = kv * group, sum(counts)
+    q = bf16(c.rng.standard_normal((T, H, d)))
+    args = (dev(q.reshape(T, -1)).bfloat16(), c.device(), ints(starts(counts)), ints(lens), H)
+    kw = dict(max_q=max(counts), max_kv=max(lens))
+    outs = [nk.attention_paged(*args, **kw) for _ in range(2)]
+    nk.device_status()
+    assert torch.equal(*outs)
+    got, at = outs[0].view(T, H, d), 0
+    for s, t in enumerate(counts):
+        n = int(lens[s])
+        k, v = c.tokens(c.k, s).astype(np.float64), c.tokens(c.v, s).astype(np.float64)
+        seen = np.tri(t, n, n - t, dtype=bool)
+        for h in range(H):
+            x = q[at:at + t, h].astype(np.float64) @ k[h // group].T * d**-0.5
+            w = np.where(seen, np.exp(x - np.where(seen, x, -np.inf).max(1, keepdims=True)), 0)
+            w /= w.sum(1, keepdims=True)
+            _close(got[at:at + t, h], w @ v[h // group], w @ np.abs(v[h // group]))
+        at += t

@@ -26,7 +26,6 @@ struct SelectArgs {
   int group;
   const uint16_t *k_min, *k_max;  // the layer's
   int top_k, sink, local;
-  bool scored;  // the scores are computed by the kernel before the lists
   int64_t score_ld;
   float2 *range;   // [tokens, kv_heads, score_ld]: the score lies in it
   double *exact;   // the same shape: 64-bit scores of the blocks in doubt
@@ -135,8 +134,8 @@ __global__ void __launch_bounds__(32 * kScoreWarps) block_scores_kernel(const Se
   const bool once = wide == HEADS;                           // one pass
   float *sums = reinterpret_cast<float *>(bounds + (once ? 0 : S::kBounds));
                                                              // [HEADS + 1][warp][block]
+  let_next_launch();
   wait_for_previous();
-  let_next_launch();  // behind the wait: the lists read the batch without one
   const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The first 8 channels of this thread's queries are on their way while the
   // sequence is found.
@@ -468,11 +467,9 @@ template <int D, int T>
 __global__ void __launch_bounds__(T, 1024 / T) block_topk_kernel(const SelectArgs a) {
   __shared__ TopShared<T> sh;
   let_next_launch();
-  if (!a.scored) wait_for_previous();
+  wait_for_previous();
   Query x;
-  const bool found = find_query(a, blockIdx.y, x, threadIdx.x == 0);
-  if (a.scored) wait_for_previous();
-  if (!found) return;
+  if (!find_query(a, blockIdx.y, x, threadIdx.x == 0)) return;
   const int h = blockIdx.x, n = x.blocks;
   int32_t *out = a.blocks + (x.token * a.pool.heads + h) * (int64_t)a.top_k;
   if (n <= a.top_k) {
@@ -747,7 +744,6 @@ nk_status nk_kv_block_select(const nk_kv_pages *kv, int64_t layer, const nk_kv_b
   a.top_k = (int)top_k;
   a.sink = (int)sink;
   a.local = (int)local;
-  a.scored = width > top_k;
   a.score_ld = width;
   a.exact = static_cast<double *>(workspace);
   a.range = reinterpret_cast<float2 *>(a.exact + batch->tokens * kv->kv_heads * width);

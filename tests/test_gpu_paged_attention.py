@@ -1099,3 +1099,32 @@ def test_prompts_of_more_units_than_blocks(cuda, kv, group, d, ps, lens, counts)
             w /= w.sum(1, keepdims=True)
             _close(got[at:at + t, h], w @ v[h // group], w @ np.abs(v[h // group]))
         at += t
+
+
+def test_lists_follow_lengths_written_just_before(cuda):
+    """The batch's arrays are rewritten by the kernel ahead of each selection, in
+    the same memory: every kernel of the call reads the new ones."""
+    heads, H, ps, top_k, steps = 2, 8, 16, 6, 80
+    results = []
+    for wait in (True, False):
+        c = Paged(13, [400, 1500, 900], heads, ps, 64)
+        pages = c.device()
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        q = torch.empty(steps, 3, H * 64, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+        start, kv_len, rows = ints([0, 1, 2, 3]), ints([200, 700, 20]), ints([0, 1, 2])
+        got = []
+        torch.cuda.synchronize()
+        for i in range(steps):
+            kv_len.add_(1 + i % 3)
+            rows.copy_(rows.roll(1) if i % 16 == 15 else rows)
+            kv_len.clamp_(max=400)
+            for _ in range(3):
+                got.append(nk.kv_block_select(q[i], pages, start, kv_len, H, top_k, rows=rows,
+                                              max_q=1, max_kv=1500))
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        nk.device_status()
+        results.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert not torch.equal(results[0][0], results[0][-1])

@@ -1341,7 +1341,7 @@ __global__ void __launch_bounds__(320, 1)
         // One flag, never cleared: A may be any number of pieces ahead of B, which
         // skips pieces without rows of its own.  For a piece that took nothing out
         // poison adds 0.
-        const bool bad = n > 0 && *(volatile int *)&odd;
+        const bool bad = n > 0 && odd;
         // Through shared memory (the queries' tile is free): a thread holds a
         // row, a store instruction writes 4 rows of 32 columns.
         float4 *stage = reinterpret_cast<float4 *>(qs + g * (128 * D * 2) + (warp & 3) * 4096);

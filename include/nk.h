@@ -733,7 +733,7 @@ typedef struct nk_kv_batch {
   const int32_t *start;  /* [seqs + 1] */
   const int32_t *kv_len; /* [seqs], the new tokens included */
   const int32_t *rows;   /* [seqs] table row of each sequence; NULL: row b */
-  int64_t max_new;       /* bound of start[b+1] - start[b] */
+  int64_t max_new;       /* bound of start[b+1] - start[b]; <= tokens and <= max_kv */
   int64_t max_kv;        /* bound of kv_len[b] */
 } nk_kv_batch;
 
@@ -766,7 +766,8 @@ nk_status nk_kv_table_write(int32_t *dst, int64_t dst_len, const int64_t *offset
  * recomputed over the positions below base[b] + n_keep[b]; new_len[b] (may be
  * NULL) is set to that sum.  All arrays are device arrays, so that the
  * outcome of a verification needs no host.
- * dst_table NULL: in place (the accepted path of a draft tree closes up).
+ * dst_table NULL (dst_ld 0): in place (the accepted path of a draft tree closes
+ * up).
  * Otherwise the tokens go to the pages of dst_table [seqs, dst_ld] (a context
  * thinned into fresh pages); a page written must not be read as a source.
  * Refused entries (not ascending, past kv_len) leave their slot unwritten.
@@ -800,10 +801,13 @@ nk_status nk_kv_pages_compact(const nk_kv_pages *kv, const nk_kv_compact_args *a
  *   - with blocks [tokens, kv_heads, max_blocks], the positions up to its own
  *     that lie in the listed blocks of page_size tokens.  Entries are
  *     ascending; one that is negative, past the token's position or not
- *     larger than the entry before it is skipped.
+ *     larger than the entry before it is skipped, wherever it stands.  Without
+ *     blocks max_blocks is 0.
  * A token that may attend nothing gets 0.  Positions it may not attend do
  * not reach its output, whatever they hold (infinities and NaN too).  Rows of
- * out behind the last sequence stay as they were.
+ * out behind the last sequence stay as they were.  Scores, softmax statistics
+ * and sums are f32; each weight is rounded to bf16 for the product with the
+ * values (2^-8 of it at most), with f32 results too.
  * workspace: nk_attention_paged_workspace_bytes for the same batch bounds
  * (0 bytes: NULL). */
 typedef struct nk_paged_attention_args {

@@ -78,10 +78,12 @@ __device__ __forceinline__ void write_bounds(Bounds8 &b, bool any, uint4 *kmin, 
 
 // Block = (touched page x, head y, sequence z): the new tokens of one page, so
 // that the page's bounds have one writer and need no atomics, and a key is read
-// once for the copy and the bounds.  Bound by HBM for a prefill (9000 tokens of 8
-// heads of 128, 74 MB: 16.8 us when the writes reach memory too, 10.7 us with all
-// of it in L2; the heads of a page side by side in the grid: 18.4 and 10.7), by
-// the launch for a decode step (64 tokens: 2.6 us in a chain of calls).
+// once for the copy and the bounds.  For a prefill bound by HBM and by the lookups
+// (start, length, row, table) that each block of 16 KB makes ahead of its first
+// load (9000 tokens of 8 heads of 128, 74 MB: 16.8 us when the writes reach memory
+// too, 10.7 us with all of it in L2; the heads of a page side by side in the grid:
+// 18.4 and 10.7), by the launch for a decode step (64 tokens: 2.6 us in a chain of
+// calls).
 template <int D>
 __global__ void __launch_bounds__(128)
     pages_append_kernel(PagePool pool, PageBatch batch, const uint16_t *__restrict__ k_new,
@@ -325,7 +327,8 @@ __global__ void __launch_bounds__(128)
 // that are all read before any is written never read a slot that an earlier
 // round has overwritten.  One block keeps that order without flags between
 // blocks; the few kept tokens of a verified draft are a round or two, bound by
-// its chain of dependent loads (keep, table, key): 10.5 us cold, 6.5 us in a
+// two chains of dependent loads, one behind the other (keep, table, key; then for
+// the bounds table, keys and the join of the lanes): 9.5 us cold, 6.4 us in a
 // chain of calls for 64 sequences of 6 layers and 2 heads.
 template <int D>
 __global__ void __launch_bounds__(256)

@@ -813,7 +813,9 @@ def attention_check(workspace, stream=None) -> int:
 # ------------------------------------------------------------- paged KV cache
 # The wrappers below are called several times a decode step, where the GPU work
 # of a call is a few microseconds: they look at each property of a tensor once
-# and leave the wording of refusals to the slow path.
+# and leave the wording of refusals to the slow path.  With stream= the inputs
+# must be ready on that stream; results may be read on the current one once it
+# waits for the other.
 def _is(t, dtype, dim, device) -> bool:
     return t.dtype is dtype and t.dim() == dim and t.device == device and \
         (t.is_contiguous() or t.stride(-1) == 1)
@@ -1163,6 +1165,7 @@ def attention_paged(q, pages: KvPages, start, kv_len, q_heads: int, *, max_q=Non
     and, with tree_mask, 64; the table's width); close bounds cost less.  Returns
     [tokens, q_heads * head_dim] in bf16, or f32 with out_dtype=F32; rows that
     belong to no sequence stay as they were (a new `out` is not initialised).
+    Weights are rounded to bf16 for the product with the values in both.
     workspace: optional uint8 device tensor of attention_paged_workspace_bytes."""
     tokens, ld_q = pages._queries(q, q_heads)
     b = pages.batch(start, kv_len, tokens, max_q, max_kv, rows)

@@ -1128,3 +1128,73 @@ def test_lists_follow_lengths_written_just_before(cuda):
         results.append(got)
     assert all(torch.equal(a, b) for a, b in zip(*results))
     assert not torch.equal(results[0][0], results[0][-1])
+
+
+def test_captured_on_a_stream_that_joins_the_capture(cuda):
+    """Calls captured with stream= on a stream forked from the capturing one, their
+    results read behind the join; replayed on new inputs with other graphs between."""
+    lens, H = [700, 90, 333], 8
+    c = Paged(14, lens, 2, 16, 64)
+    pages, start, kv_len = c.device(), ints([0, 1, 2, 3]), ints(lens)
+    kw = dict(max_q=1, max_kv=9000)
+    q = torch.zeros(3, H * 64, dtype=torch.bfloat16, device="cuda")
+    side, graphs = torch.cuda.Stream(), []
+    nk.attention_paged_sparse(q, pages, start, kv_len, H, 5, stream=side, **kw)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            side.wait_stream(torch.cuda.current_stream())
+            full = nk.attention_paged(q, pages, start, kv_len, H, stream=side, **kw)
+            out, blocks = nk.attention_paged_sparse(q, pages, start, kv_len, H, 5, stream=side,
+                                                    **kw)
+            torch.cuda.current_stream().wait_stream(side)
+            both = full + out
+        graphs.append((g, both, blocks))
+    for i in range(4):
+        q.normal_()
+        full = nk.attention_paged(q, pages, start, kv_len, H, **kw)
+        out, blocks = nk.attention_paged_sparse(q, pages, start, kv_len, H, 5, **kw)
+        g, both, lists = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(both, full + out) and torch.equal(lists, blocks)
+    nk.device_status()
+
+
+def test_calls_of_two_threads_at_once(cuda):
+    """Two host threads, a stream each, over one cache."""
+    import threading
+
+    lens, H = [2000, 64, 700], 8
+    c = Paged(15, lens, 2, 16, 64)
+    pages, start, kv_len = c.device(), ints([0, 1, 2, 3]), ints(lens)
+    q = torch.randn(2, 40, 3, H * 64, device="cuda").bfloat16()
+
+    def calls(x, i, stream=None):
+        kw = dict(max_q=1, max_kv=2000 + 64 * i, stream=stream)
+        full = nk.attention_paged(x, pages, start, kv_len, H, **kw)
+        return [full, *nk.attention_paged_sparse(x, pages, start, kv_len, H, 3 + i % 4, **kw)]
+
+    want = [[calls(x, i) for i, x in enumerate(q[t])] for t in range(2)]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(t):
+        try:
+            s = torch.cuda.Stream()
+            got[t] = [calls(x, i, s) for i, x in enumerate(q[t])]
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert all(torch.equal(m, n) for m, n in zip(x, y))
+    nk.device_status()

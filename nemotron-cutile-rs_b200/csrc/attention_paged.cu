@@ -1621,7 +1621,8 @@ static nk_status check_attention(const nk_kv_pages *kv, const nk_kv_batch *b,
 // [rows, D] bf16 as boxes of 64 channels x box_rows tokens, 128-byte swizzle.
 static nk_status page_map(const uint16_t *base, int64_t rows, int64_t d, int box_rows,
                           CUtensorMap *map) {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};  // calls of many threads
+  PFN_cuTensorMapEncodeTiled_v12000 fn = known.load(std::memory_order_relaxed);
   if (!fn) {
     void *p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -1629,6 +1630,7 @@ static nk_status page_map(const uint16_t *base, int64_t rows, int64_t d, int box
             cudaSuccess || q != cudaDriverEntryPointSuccess)
       return fail(NK_DEVICE_ERROR, "cuTensorMapEncodeTiled unavailable");
     fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    known.store(fn, std::memory_order_relaxed);
   }
   const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)d * 2};

@@ -67,7 +67,10 @@ class PagedKvCache:
             hi = torch.zeros_like(lo)
         table = torch.zeros(max_seqs, self.width, dtype=torch.int32, device=device)
         self._init_host(pages, max_seqs)
+        self._bounds = bool(bounds)
         self._bind(k, v, table, lo, hi)
+
+    _bounds = True  # key bounds are kept
 
     def _bind(self, k, v, table, lo, hi):
         self.pages = nk.KvPages(k, v, table, k_min=lo, k_max=hi)
@@ -280,11 +283,13 @@ class PagedKvCache:
         n = len(keep)
         if n == 0:
             return
-        # Slots that the move writes must not be shared with a fork.
+        # Slots and bounds that the move writes must not be shared with a fork.
         jobs, need, left = [], 0, {}
         for s, c, length, row in zip(step.seqs, step.counts, step.lens, keep):
             base = length - c
             first, end = base // self.page_size, self._blocks(base + len(row))
+            if not row and not self._bounds:
+                end = first
             for b in range(first, end):
                 page = int(self._table[s, b])
                 refs = left.get(page, int(self._refs[page]))
@@ -318,7 +323,8 @@ class PagedKvCache:
 
     def truncate(self, seq, length, stream=None) -> None:
         """Drops the tokens from position `length` on; the bounds of the last
-        page left are taken anew over what it still holds."""
+        page left are taken anew over what it still holds (in a copy, which
+        takes a free page, when a fork shares it)."""
         self._check(seq)
         old = int(self._len[seq])
         if not 0 <= length <= old:

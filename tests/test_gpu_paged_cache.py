@@ -472,3 +472,28 @@ def test_tables_whose_rows_lie_apart(cuda):
         assert all(torch.equal(x, y) for x, y in zip(before[4:], pools[-1][4:]))
     for x, y in zip(*pools):
         assert torch.equal(x, y)
+
+
+def test_truncation_of_forks_with_and_without_bounds(cuda):
+    """A fork cut back inside a shared page and grown again leaves the other alone."""
+    for bounds in (True, False):
+        cache = nk_paged.PagedKvCache(8, 1, 64, max_seqs=3, max_len=64, page_size=16, bounds=bounds)
+        a = cache.new_sequence()
+        first = torch.randn(2, 32, 64, device="cuda").bfloat16()
+        cache.append(cache.step([a], [32]), first[0], first[1])
+        b = cache.fork(a)
+        cache.truncate(b, 20)
+        assert cache.free_pages == (5 if bounds else 6)
+        more = torch.randn(2, 5, 64, device="cuda").bfloat16()
+        cache.append(cache.step([b], [5]), more[0], more[1])
+        nk.device_status()
+        for s, want in ((a, first), (b, torch.cat([first[:, :20], more], 1))):
+            ids = torch.tensor(cache.page_ids(s), device="cuda")
+            n = want.shape[1]
+            for pool, x in ((cache.pages.k, want[0]), (cache.pages.v, want[1])):
+                assert torch.equal(pool[0, ids, 0].reshape(-1, 64)[:n], x)
+            if bounds:
+                for j in range(2):
+                    x = want[0, 16 * j:16 * j + 16]
+                    assert torch.equal(cache.pages.k_min[0, ids[j], 0], x.amin(0))
+                    assert torch.equal(cache.pages.k_max[0, ids[j], 0], x.amax(0))

@@ -451,3 +451,31 @@ def test_host_lists_that_are_no_whole_numbers_are_refused(bad):
     with pytest.raises(OverflowError):
         nk._host_ints([2**31], np.int32)
     assert nk._host_ints([2**40], np.int64).tolist() == [2**40]
+
+
+def test_truncation_without_bounds_takes_no_page():
+    """Nothing of a shared page is written when no bounds are kept."""
+    class NoBounds(HostCache):
+        _bounds = False
+
+        def _compact(self, step, base, keep, n_keep, stream):
+            for i, s in enumerate(step.seqs):
+                for j in range(n_keep[i]):
+                    assert self._refs[self.slot(s, base[i] + j)[0]] == 1
+            self.moved = n_keep
+
+    for kind, need in ((NoBounds, 0), (HostCache, 1)):
+        c = kind(4, 3, 32, 4)
+        a = c.new_sequence()
+        c.write(c.step([a], [12]), list(range(12)))
+        b = c.fork(a)  # three shared pages, one free
+        d = c.new_sequence()
+        c.write(c.step([d], [1 - need]), [77][need:])
+        if need:
+            assert c.free_pages == 1
+        c.truncate(b, 6)
+        assert c.free_pages == 0 and c.read(b) == list(range(6))
+        _check(c, {a: list(range(12)), b: list(range(6)), d: c.read(d)})
+        if not need:  # a write asks for the page
+            with pytest.raises(RuntimeError, match="out of pages"):
+                c.step([b], [1])
